@@ -1,0 +1,326 @@
+// Global gradient norm over many tensors, and clipping: bn_gradient_set_* of include/bn_hip.h.
+//
+//   norm = sqrt(sum over all tensors and elements of g^2)
+//   out  = g * (norm > max_norm ? max_norm / norm : 1)
+//
+// Bound by memory: every gradient is read for the norm and, since no element can be scaled before the
+// last one has been seen, read again for the copy.  A set lists its tensors once, cut into chunks of
+// at most 16 KiB that one wave streams with 16-byte loads; tensors of any number, size and type are
+// then two launches (785 tables of 20 elements cost what one tensor of that size costs).  Neighbours
+// in memory are joined before they are cut, so a model whose tables are slices of one buffer is one
+// tensor to the kernels.
+//
+// Squares are summed in double: the square of any float32 is finite there, and the conversions keep
+// up with the loads several times over.  A wave's chunks, a block's waves and the blocks are summed
+// in an order that depends on the set alone - no atomics, the same bits every time.
+#include "../../include/bn_hip.h"
+
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <string>
+#include <vector>
+
+#include <hip/hip_runtime.h>
+
+#include "error.h"
+#include "row_values.h"
+
+namespace {
+
+using namespace bn_rows;
+
+struct Chunk {
+  const void* source;
+  void* output;
+  int32_t count;  // elements
+  int32_t dtype;
+};
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int64_t kChunkBytes = 16384;
+constexpr int kMaxBlocks = 2048;  // 8 blocks of 4 waves on each of 256 CUs
+
+template <typename T>
+__device__ __forceinline__ double chunk_squares(const Chunk& c, int lane) {
+  constexpr int V = Value<T>::kVec;
+  const T* g = static_cast<const T*>(c.source);
+  double sum = 0.0;
+  const int packs = c.count / V;
+#pragma unroll 4
+  for (int i = lane; i < packs; i += 64) {
+    const Pack<T> p = load_pack(g + (size_t)i * V);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const double x = (double)Value<T>::widen(p.v[j]);
+      sum = fma(x, x, sum);
+    }
+  }
+  const int i = packs * V + lane;
+  if (i < c.count) {
+    const double x = (double)Value<T>::widen(g[i]);
+    sum = fma(x, x, sum);
+  }
+  return sum;
+}
+
+template <typename T>
+__device__ __forceinline__ T scaled(T v, double factor) {
+  // one product in double; the 16-bit types pass through float32 on the way, whose step is 2^-13 (half)
+  // and 2^-16 (bfloat16) of theirs
+  return Value<T>::round((typename Value<T>::Wide)((double)Value<T>::widen(v) * factor));
+}
+
+template <typename T>
+__device__ __forceinline__ void chunk_scale(const Chunk& c, int lane, double factor) {
+  constexpr int V = Value<T>::kVec;
+  const T* g = static_cast<const T*>(c.source);
+  T* out = static_cast<T*>(c.output);
+  const int packs = c.count / V;
+#pragma unroll 4
+  for (int i = lane; i < packs; i += 64) {
+    Pack<T> p = load_pack(g + (size_t)i * V);
+#pragma unroll
+    for (int j = 0; j < V; ++j) p.v[j] = scaled<T>(p.v[j], factor);
+    store_pack(out + (size_t)i * V, p);
+  }
+  const int i = packs * V + lane;
+  if (i < c.count) out[i] = scaled<T>(g[i], factor);
+}
+
+// sum over the block, the same in every thread
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+  v = lanes_sum<64>(v);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double total = 0.0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) total += lds[w];
+  return total;
+}
+
+__global__ void __launch_bounds__(kThreads) gradient_squares(const Chunk* __restrict__ chunks, int64_t n_chunks,
+                                                            double* __restrict__ partials) {
+  __shared__ double lds[kWaves];
+  const int lane = threadIdx.x & 63;
+  double sum = 0.0;
+  for (int64_t k = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); k < n_chunks; k += (int64_t)gridDim.x * kWaves) {
+    const Chunk c = chunks[k];
+    switch (c.dtype) {
+      case BN_F32: sum += chunk_squares<float>(c, lane); break;
+      case BN_F64: sum += chunk_squares<double>(c, lane); break;
+      case BN_F16: sum += chunk_squares<__half>(c, lane); break;
+      default: sum += chunk_squares<__hip_bfloat16>(c, lane); break;
+    }
+  }
+  const double total = block_sum(sum, lds);
+  if (threadIdx.x == 0) partials[blockIdx.x] = total;
+}
+
+__device__ __forceinline__ double norm_of(const double* __restrict__ partials, int n_partials, double* lds) {
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < n_partials; i += kThreads) sum += partials[i];
+  return sqrt(block_sum(sum, lds));
+}
+
+__global__ void __launch_bounds__(kThreads) gradient_norm_finish(const double* __restrict__ partials, int n_partials,
+                                                                double* __restrict__ norm_out) {
+  __shared__ double lds[kWaves];
+  const double norm = norm_of(partials, n_partials, lds);
+  if (threadIdx.x == 0) *norm_out = norm;
+}
+
+__global__ void __launch_bounds__(kThreads) gradient_scale(const Chunk* __restrict__ chunks, int64_t n_chunks,
+                                                          const double* __restrict__ partials, int n_partials,
+                                                          double max_norm, double* __restrict__ norm_out) {
+  __shared__ double lds[kWaves];
+  const double norm = norm_of(partials, n_partials, lds);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
+  // a NaN norm leaves no gradient usable: every element becomes NaN; an infinite one gives factor 0
+  const double factor = norm <= max_norm ? 1.0 : max_norm / norm;
+  const int lane = threadIdx.x & 63;
+  for (int64_t k = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); k < n_chunks; k += (int64_t)gridDim.x * kWaves) {
+    const Chunk c = chunks[k];
+    switch (c.dtype) {
+      case BN_F32: chunk_scale<float>(c, lane, factor); break;
+      case BN_F64: chunk_scale<double>(c, lane, factor); break;
+      case BN_F16: chunk_scale<__half>(c, lane, factor); break;
+      default: chunk_scale<__hip_bfloat16>(c, lane, factor); break;
+    }
+  }
+}
+
+struct Range {
+  uintptr_t begin, end;
+  int32_t tensor;
+};
+
+}  // namespace
+
+struct bn_gradient_set {
+  int device = 0;
+  int64_t n_chunks = 0;
+  int blocks = 1;
+  Chunk* d_chunks = nullptr;
+};
+
+namespace {
+
+using bn::fail;
+
+#define BN_HIP_CHECK(expr)                                                            \
+  do {                                                                                \
+    hipError_t err__ = (expr);                                                        \
+    if (err__ != hipSuccess)                                                          \
+      return fail(BN_ERR_HIP, std::string(#expr) + ": " + hipGetErrorString(err__));  \
+  } while (0)
+
+// Every output must be its own gradient's memory or memory that nothing else in the set uses: a block
+// that scales one tensor must not change what another still reads or writes.
+int check_overlap(int32_t n, const int32_t* dtypes, const int64_t* sizes, const void* const* sources,
+                  void* const* outputs) {
+  std::vector<Range> out, in;
+  for (int32_t t = 0; t < n; ++t) {
+    if (sizes[t] == 0) continue;
+    const uintptr_t bytes = (uintptr_t)sizes[t] * dtype_bytes(dtypes[t]);
+    const uintptr_t o = reinterpret_cast<uintptr_t>(outputs[t]), s = reinterpret_cast<uintptr_t>(sources[t]);
+    out.push_back({o, o + bytes, t});
+    in.push_back({s, s + bytes, t});
+  }
+  const auto by_begin = [](const Range& a, const Range& b) { return a.begin < b.begin; };
+  std::sort(out.begin(), out.end(), by_begin);
+  std::sort(in.begin(), in.end(), by_begin);
+  for (size_t i = 1; i < out.size(); ++i)
+    if (out[i].begin < out[i - 1].end)
+      return fail(BN_ERR_INVALID, "outputs " + std::to_string(out[i - 1].tensor) + " and " +
+                                      std::to_string(out[i].tensor) + " share memory");
+  // outputs are disjoint from here on; sweep both lists for outputs that meet a gradient not their own
+  size_t first = 0;
+  for (const Range& s : in) {
+    while (first < out.size() && out[first].end <= s.begin) ++first;
+    for (size_t i = first; i < out.size() && out[i].begin < s.end; ++i)
+      if (out[i].tensor != s.tensor || out[i].begin != s.begin)
+        return fail(BN_ERR_INVALID, "output " + std::to_string(out[i].tensor) + " lies over gradient " +
+                                        std::to_string(s.tensor));
+  }
+  return BN_OK;
+}
+
+int build_set(int32_t n, const int32_t* dtypes, const int64_t* sizes, const void* const* sources,
+              void* const* outputs, bn_gradient_set* set) {
+  if (int rc = check_overlap(n, dtypes, sizes, sources, outputs)) return rc;
+  std::vector<Chunk> chunks;
+  int32_t t = 0;
+  while (t < n) {
+    const int64_t es = (int64_t)dtype_bytes(dtypes[t]);
+    const char* s = static_cast<const char*>(sources[t]);
+    char* o = static_cast<char*>(outputs[t]);
+    int64_t count = sizes[t];
+    int32_t last = t;
+    // the next tensor continues this one in both arrays: one run
+    while (count > 0 && last + 1 < n && dtypes[last + 1] == dtypes[t] && sizes[last + 1] > 0 &&
+           static_cast<const char*>(sources[last + 1]) == s + count * es &&
+           static_cast<char*>(outputs[last + 1]) == o + count * es)
+      count += sizes[++last];
+    for (int64_t done = 0; done < count; done += kChunkBytes / es) {
+      const int64_t here = std::min(count - done, kChunkBytes / es);
+      chunks.push_back({s + done * es, o + done * es, (int32_t)here, dtypes[t]});
+    }
+    t = last + 1;
+  }
+  set->n_chunks = (int64_t)chunks.size();
+  set->blocks = (int)std::min<int64_t>(std::max<int64_t>((set->n_chunks + kWaves - 1) / kWaves, 1), kMaxBlocks);
+  BN_HIP_CHECK(hipGetDevice(&set->device));
+  if (!chunks.empty()) {
+    BN_HIP_CHECK(hipMalloc(reinterpret_cast<void**>(&set->d_chunks), chunks.size() * sizeof(Chunk)));
+    BN_HIP_CHECK(hipMemcpy(set->d_chunks, chunks.data(), chunks.size() * sizeof(Chunk), hipMemcpyHostToDevice));
+  }
+  return BN_OK;
+}
+
+int launch_squares(const bn_gradient_set* set, double* partials, hipStream_t s) {
+  int device = -1;
+  if (hipGetDevice(&device) != hipSuccess || device != set->device)
+    return fail(BN_ERR_STATE, "the gradient set belongs to another HIP device than the current one");
+  hipLaunchKernelGGL(gradient_squares, dim3(set->blocks), dim3(kThreads), 0, s, set->d_chunks, set->n_chunks, partials);
+  BN_HIP_CHECK(hipGetLastError());
+  return BN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int bn_gradient_set_create(int32_t num_tensors, const int32_t* dtypes, const int64_t* sizes,
+                           const void* const* gradients_dev, void* const* outputs_dev, bn_gradient_set** out_set) {
+  if (!out_set) return fail(BN_ERR_INVALID, "out_set is null");
+  *out_set = nullptr;
+  if (num_tensors < 0) return fail(BN_ERR_INVALID, "negative number of tensors");
+  if (num_tensors > 0 && (!dtypes || !sizes || !gradients_dev || !outputs_dev))
+    return fail(BN_ERR_INVALID, "null argument");
+  for (int32_t t = 0; t < num_tensors; ++t) {
+    const size_t es = dtype_bytes(dtypes[t]);
+    if (es == 0) return fail(BN_ERR_INVALID, "dtype must be BN_F32, BN_F64, BN_F16 or BN_BF16");
+    if (sizes[t] < 0 || sizes[t] > ((int64_t)1 << 48)) return fail(BN_ERR_INVALID, "bad tensor size");
+    if (sizes[t] == 0) continue;
+    if (!gradients_dev[t] || !outputs_dev[t]) return fail(BN_ERR_INVALID, "null tensor address");
+    if (reinterpret_cast<uintptr_t>(gradients_dev[t]) % es || reinterpret_cast<uintptr_t>(outputs_dev[t]) % es)
+      return fail(BN_ERR_INVALID, "tensor address not aligned to its type");
+  }
+  bn_gradient_set* set = new (std::nothrow) bn_gradient_set();
+  if (!set) return fail(BN_ERR_INVALID, "out of host memory");
+  int rc;
+  try {
+    rc = build_set(num_tensors, dtypes, sizes, gradients_dev, outputs_dev, set);
+  } catch (const std::bad_alloc&) {
+    rc = fail(BN_ERR_INVALID, "out of host memory");
+  }
+  if (rc) {
+    if (set->d_chunks) (void)hipFree(set->d_chunks);
+    delete set;
+    return rc;
+  }
+  *out_set = set;
+  return BN_OK;
+}
+
+int bn_gradient_set_destroy(bn_gradient_set* set) {
+  if (!set) return BN_OK;
+  int prev = 0;
+  (void)hipGetDevice(&prev);
+  (void)hipSetDevice(set->device);
+  if (set->d_chunks) (void)hipFree(set->d_chunks);
+  (void)hipSetDevice(prev);
+  delete set;
+  return BN_OK;
+}
+
+int64_t bn_gradient_set_workspace_bytes(const bn_gradient_set* set) {
+  return set ? (int64_t)set->blocks * (int64_t)sizeof(double) : -1;
+}
+
+int bn_gradient_set_norm(bn_gradient_set* set, void* workspace_dev, double* norm_out_dev, void* stream) {
+  if (!set || !workspace_dev || !norm_out_dev) return fail(BN_ERR_INVALID, "null argument");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  double* partials = static_cast<double*>(workspace_dev);
+  if (int rc = launch_squares(set, partials, s)) return rc;
+  hipLaunchKernelGGL(gradient_norm_finish, dim3(1), dim3(kThreads), 0, s, partials, set->blocks, norm_out_dev);
+  BN_HIP_CHECK(hipGetLastError());
+  return BN_OK;
+}
+
+int bn_gradient_set_clip(bn_gradient_set* set, double max_norm, void* workspace_dev, double* norm_out_dev,
+                         void* stream) {
+  if (!set || !workspace_dev || !norm_out_dev) return fail(BN_ERR_INVALID, "null argument");
+  if (!(max_norm > 0.0) || std::isinf(max_norm)) return fail(BN_ERR_INVALID, "max_norm must be positive and finite");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  double* partials = static_cast<double*>(workspace_dev);
+  if (int rc = launch_squares(set, partials, s)) return rc;
+  hipLaunchKernelGGL(gradient_scale, dim3(set->blocks), dim3(kThreads), 0, s, set->d_chunks, set->n_chunks, partials,
+                     set->blocks, max_norm, norm_out_dev);
+  BN_HIP_CHECK(hipGetLastError());
+  return BN_OK;
+}
+
+}  // extern "C"

@@ -24,6 +24,14 @@ class BnError(RuntimeError):
     pass
 
 
+class DrawFilters(ctypes.Structure):
+    """bn_draw_filters: each setting as a number, or as a device array with one per row."""
+
+    _fields_ = [("temperature", c_double), ("top_k", c_int64), ("top_p", c_double), ("min_p", c_double),
+                ("temperature_dev", c_void_p), ("top_k_dev", c_void_p), ("top_p_dev", c_void_p),
+                ("min_p_dev", c_void_p)]
+
+
 def lib_path() -> str:
     return _LIB_PATH
 
@@ -136,6 +144,29 @@ def _declare(lib):
     lib.bn_sampler_walk_order.argtypes = [c_int32, i32p, i32p, i32p, c_int32, i32p]
     lib.bn_sampler_sample.restype = c_int
     lib.bn_sampler_sample.argtypes = [c_void_p, c_void_p, i32p, c_int32, c_int64, c_uint64, c_void_p, c_void_p, c_void_p]
+    lib.bn_draw_states_workspace_bytes.restype = c_int64
+    lib.bn_draw_states_workspace_bytes.argtypes = [c_int, c_int64, c_int64]
+    lib.bn_draw_states.restype = c_int
+    lib.bn_draw_states.argtypes = [c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p,
+                                   POINTER(DrawFilters), c_void_p, c_void_p, c_void_p]
+    lib.bn_states_log_likelihood.restype = c_int
+    lib.bn_states_log_likelihood.argtypes = [c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int32,
+                                             c_void_p, c_void_p, c_void_p]
+    lib.bn_states_log_likelihood_gradient.restype = c_int
+    lib.bn_states_log_likelihood_gradient.argtypes = [c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                                                      c_int32, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
+                                                      c_int64, c_void_p]
+    lib.bn_gradient_set_create.restype = c_int
+    lib.bn_gradient_set_create.argtypes = [c_int32, i32p, POINTER(c_int64), POINTER(c_void_p), POINTER(c_void_p),
+                                           POINTER(c_void_p)]
+    lib.bn_gradient_set_destroy.restype = c_int
+    lib.bn_gradient_set_destroy.argtypes = [c_void_p]
+    lib.bn_gradient_set_workspace_bytes.restype = c_int64
+    lib.bn_gradient_set_workspace_bytes.argtypes = [c_void_p]
+    lib.bn_gradient_set_norm.restype = c_int
+    lib.bn_gradient_set_norm.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p]
+    lib.bn_gradient_set_clip.restype = c_int
+    lib.bn_gradient_set_clip.argtypes = [c_void_p, c_double, c_void_p, c_void_p, c_void_p]
     lib.bn_profile_enable.restype = c_int
     lib.bn_profile_enable.argtypes = [c_int32]
     lib.bn_profile_only.restype = c_int
@@ -156,6 +187,10 @@ EXPORTS = (
     "bn_exact_log_likelihood", "bn_exact_marginal",
     "bn_sampler_create", "bn_sampler_destroy", "bn_sampler_cpt_elements", "bn_sampler_workspace_bytes",
     "bn_sampler_walk_order", "bn_sampler_sample",
+    "bn_draw_states_workspace_bytes", "bn_draw_states",
+    "bn_states_log_likelihood", "bn_states_log_likelihood_gradient",
+    "bn_gradient_set_create", "bn_gradient_set_destroy", "bn_gradient_set_workspace_bytes", "bn_gradient_set_norm",
+    "bn_gradient_set_clip",
     "bn_profile_enable", "bn_profile_report", "bn_profile_only", "bn_profile_stride",
 )
 
@@ -194,6 +229,20 @@ def build_cardinality_pack(states: int) -> str:
 def check(rc: int):
     if rc != 0:
         raise BnError(load().bn_last_error().decode("utf-8", "replace"))
+
+
+# element types of the operators on rows of logits and on gradients
+DTYPE_CODES = {torch.float32: 0, torch.float64: 1, torch.float16: 2, torch.bfloat16: 3}
+
+
+def pointer(tensor):
+    """The tensor's device address; None stays a null pointer."""
+    return None if tensor is None else c_void_p(tensor.data_ptr())
+
+
+def stream_of(device):
+    """The stream torch enqueues on at this moment, as the library takes it."""
+    return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
 def i32_array(values):

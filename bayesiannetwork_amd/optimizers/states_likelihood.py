@@ -1,0 +1,114 @@
+"""Log-likelihood of observed states under rows of logits, with its gradient.
+
+EM learns CPTs from expected counts.  A distribution whose logits come from somewhere else - a CPT row
+as the softmax of free parameters, a network that maps features to a node's states, the class posterior
+of a discriminatively trained model - is learned by the gradient of this log-likelihood instead
+(``bn_states_log_likelihood`` and ``bn_states_log_likelihood_gradient`` of ``include/bn_hip.h``).
+``HipGradientClipper`` bounds the step.  There is no CPU path.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from .. import rows as _rows
+from ..inference_machines.hip_spa import _native
+
+_STATE_BYTES = {torch.uint8: 1, torch.int32: 4, torch.int64: 8}
+
+
+def _ll_dtype(logits: torch.Tensor) -> torch.dtype:
+    return torch.float64 if logits.dtype == torch.float64 else torch.float32
+
+
+def _row_arguments(logits, counts, states):
+    return (_native.DTYPE_CODES[logits.dtype], _native.pointer(logits), logits.shape[0], logits.shape[1],
+            logits.stride(0), _native.pointer(counts), _native.pointer(states), _STATE_BYTES[states.dtype])
+
+
+def _forward(logits, states, counts, with_totals):
+    ll = torch.empty((logits.shape[0],), device=logits.device, dtype=_ll_dtype(logits))
+    totals = torch.empty((logits.shape[0], 2), device=logits.device, dtype=torch.float64) if with_totals else None
+    with torch.cuda.device(logits.device):
+        _native.check(_native.load().bn_states_log_likelihood(
+            *_row_arguments(logits, counts, states), _native.pointer(ll), _native.pointer(totals),
+            _native.stream_of(logits.device)))
+    return ll, totals
+
+
+def _gradient(logits, states, counts, totals, weights, ll, out):
+    with torch.cuda.device(logits.device):
+        _native.check(_native.load().bn_states_log_likelihood_gradient(
+            *_row_arguments(logits, counts, states), _native.pointer(totals), _native.pointer(weights),
+            0 if weights is None else weights.stride(0), _native.pointer(ll), _native.pointer(out), out.stride(0),
+            _native.stream_of(logits.device)))
+
+
+class _StatesLogLikelihood(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, states, counts):
+        ll, totals = _forward(logits, states, counts, True)
+        ctx.save_for_backward(logits, states, totals, *(() if counts is None else (counts,)))
+        return ll
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, weights):
+        logits, states, totals, *counts = ctx.saved_tensors
+        out = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+        _gradient(logits, states, counts[0] if counts else None, totals, weights, None, out)
+        return out, None, None
+
+
+def _check(logits, states, num_states):
+    _rows.check_logits(logits)
+    _rows.check_per_row(states, logits, tuple(_STATE_BYTES), "states")
+    return states.contiguous(), _rows.row_states(num_states, logits)
+
+
+def states_log_likelihood(logits: torch.Tensor, states: torch.Tensor, *,
+                          num_states: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``log softmax(logits[r])[states[r]]`` for every row: float32 ``[rows]`` (float64 for float64
+    logits), differentiable in ``logits``.
+
+    ``logits``: ``[rows, states]``, float32, float64, float16 or bfloat16, rows any distance apart.
+    ``states``: uint8, int32 or int64 ``[rows]``; one that is none of its row's states (negative or too
+    large) means the row was not observed: log-likelihood 0, gradient 0.  ``num_states`` (int32 /
+    int64 ``[rows]``): how many states each row has, the rest being padding that is not read and gets
+    gradient 0.  Logits of ``-inf`` are impossible states; a row with NaN or ``+inf`` gives NaN.
+    """
+    states, counts = _check(logits, states, num_states)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _StatesLogLikelihood.apply(logits, states, counts)
+    return _forward(logits, states, counts, False)[0]
+
+
+def states_log_likelihood_and_gradient(logits: torch.Tensor, states: torch.Tensor,
+                                       weights: Optional[torch.Tensor] = None, *,
+                                       num_states: Optional[torch.Tensor] = None,
+                                       out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The log-likelihoods ``ll`` of ``states_log_likelihood`` and the gradient of
+    ``(weights * ll).sum()`` (no weights: 1 each) in the logits, in one call that reads the logits
+    once where a row fits a block's registers.  Nothing is recorded for autograd.
+
+    ``weights``: ``[rows]`` of ll's type.  ``out``: where the gradient goes, of the logits' shape
+    and type; it may be ``logits`` itself, whose values the gradient then replaces.
+    """
+    states, counts = _check(logits, states, num_states)
+    logits = logits.detach()
+    if weights is not None:
+        _rows.check_per_row(weights, logits, (_ll_dtype(logits),), "weights")
+        weights = weights.detach()
+    if out is None:
+        out = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+    else:
+        _rows.check_logits(out, "out")
+        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+            raise ValueError("out must have the logits' shape, type and device")
+        if out.requires_grad:
+            raise ValueError("out must not require a gradient (pass its .detach())")
+    ll = torch.empty((logits.shape[0],), device=logits.device, dtype=_ll_dtype(logits))
+    _gradient(logits, states, counts, None, weights, ll, out)
+    return ll, out

@@ -36,7 +36,9 @@ extern "C" {
 
 typedef struct bn_plan bn_plan;
 
-enum { BN_F32 = 0, BN_F64 = 1 };
+/* Plans, the exact machine and the sampler take BN_F32 / BN_F64; the operators on rows of logits and on
+ * gradients take all four. */
+enum { BN_F32 = 0, BN_F64 = 1, BN_F16 = 2, BN_BF16 = 3 };
 
 enum {
   BN_OK = 0,
@@ -484,6 +486,118 @@ int64_t bn_sampler_workspace_bytes(bn_sampler* sampler, const int32_t* nodes, in
  */
 int bn_sampler_sample(bn_sampler* sampler, const void* cpts_dev, const int32_t* nodes, int32_t num_requested,
                       int64_t num_samples, uint64_t seed, void* workspace_dev, int32_t* out_dev, void* stream);
+
+/*
+ * Draw one state per row of logits, at a uniform number given for each row.  The counterpart of
+ * bn_sampler_sample for rows that no CPT holds: posteriors' logarithms, or what a network of the
+ * caller's computes.  (The reference draws from CPT rows with torch.multinomial,
+ * samplers/torch_sampler.py:43-60, and has no filters.)
+ *
+ *   w_i   = exp((x_i - max x) / temperature), states in the order of decreasing logit, ties by
+ *           ascending index
+ *   top_k   keeps the first top_k states of the order                              (0 = all)
+ *   top_p   of those, keeps the shortest prefix that holds top_p of their weight   (1 = all)
+ *   min_p   of those, keeps the states with w_i >= min_p                           (0 = all)
+ *   out     the first kept state, in ascending index, at which the cumulative weight of the kept
+ *           states exceeds u times their total; the last kept state of positive weight if none does
+ * temperature 0 takes the largest logit, the lowest index among equals.  A logit of -inf is an
+ * impossible state.  -1 is written for a row that has nothing to draw from: no states, only -inf, a
+ * NaN or +inf among its states, a u that is not in [0, 1], or a temperature of its own that is
+ * negative, infinite or NaN.
+ *
+ * Each setting is a number for the whole call, or an array with one per row when its _dev address is
+ * not NULL (doubles; int64 for top_k).  Numbers outside their range are refused with BN_ERR_INVALID;
+ * values in an array mean: top_k <= 0 off; top_p >= 1 or NaN off, <= 0 the first state only;
+ * min_p <= 0 or NaN off, > 1 taken as 1.
+ */
+typedef struct bn_draw_filters {
+  double temperature;
+  int64_t top_k;
+  double top_p;
+  double min_p;
+  const double* temperature_dev;
+  const int64_t* top_k_dev;
+  const double* top_p_dev;
+  const double* min_p_dev;
+} bn_draw_filters;
+
+/* Bytes of device workspace bn_draw_states needs; -1 on a bad argument. */
+int64_t bn_draw_states_workspace_bytes(int dtype, int64_t rows, int64_t num_states);
+/*
+ *   dtype            of the logits: BN_F32, BN_F64, BN_F16 or BN_BF16
+ *   num_states       1..2^24 states of a full row; row r starts row_stride * r elements into
+ *                    logits_dev (0 = every row reads the same states), its states lie side by side
+ *   row_states_dev   states of each row (int64, clamped to 0..num_states; the rest of the row is not
+ *                    read), or NULL when every row has num_states
+ *   uniform_dtype    BN_F32 or BN_F64, of uniforms_dev[rows]
+ *   out_dev          int32 [rows]
+ * Rows need no alignment beyond their type's.  The call allocates nothing and may be captured into a
+ * graph; calls that may overlap need a workspace each.  Sums are taken in one fixed order: the same
+ * inputs give the same states.
+ */
+int bn_draw_states(int dtype, const void* logits_dev, int64_t rows, int64_t num_states, int64_t row_stride,
+                   const int64_t* row_states_dev, int uniform_dtype, const void* uniforms_dev,
+                   const bn_draw_filters* filters, void* workspace_dev, int32_t* out_dev, void* stream);
+
+/*
+ * Log-likelihood of one observed state per row of logits:
+ *   ll_out_dev[r] = x[r][s_r] - log sum_i exp(x[r][i])
+ * and the sums themselves, for the gradient below, to totals_out_dev[rows][2]: the row's largest logit and
+ * sum_i exp(x[r][i] - largest), as doubles (may be NULL).  Rows, row_stride and row_states_dev as in bn_draw_states; states_dev[rows] are unsigned bytes
+ * (state_bytes 1), int32 (4) or int64 (8).  ll_out_dev is float for BN_F32, BN_F16 and BN_BF16,
+ * double for BN_F64.  A state that is none of its row's states means "not observed", as in
+ * bn_enter_evidence_states: log-likelihood 0, gradient 0.  A row of -inf only has -inf (and gradient
+ * 0), a row with a NaN or +inf among its states NaN.  With the rows' softmax as CPT rows, this
+ * is the term a fully observed child adds to the reference's log-likelihood
+ * (spa_v3/spa_inference_machine.py:121-137); the reference learns by EM only and has no gradient.
+ */
+int bn_states_log_likelihood(int dtype, const void* logits_dev, int64_t rows, int64_t num_states, int64_t row_stride,
+                             const int64_t* row_states_dev, const void* states_dev, int32_t state_bytes,
+                             void* ll_out_dev, double* totals_out_dev, void* stream);
+/*
+ * The gradient of sum_r weight_r * ll_r:
+ *   gradient_out_dev[r][i] = weight_r * ([i = s_r] - softmax(x[r])[i])
+ * in the logits' type, 0 beyond a row's states, rows gradient_stride elements apart.  weights_dev is
+ * of ll_out's type, weights_stride elements apart (0 = one weight for all rows), NULL = 1.
+ *   totals_dev given   the backward pass of an earlier bn_states_log_likelihood: reads the logits
+ *                      once; ll_out_dev must be NULL
+ *   totals_dev NULL    log-likelihood (to ll_out_dev, may be NULL) and gradient in one call
+ * The gradient may replace the logits (same address and stride); any other overlap with them is
+ * refused.  Neither call allocates; both may be captured into a graph.
+ */
+int bn_states_log_likelihood_gradient(int dtype, const void* logits_dev, int64_t rows, int64_t num_states,
+                                      int64_t row_stride, const int64_t* row_states_dev, const void* states_dev,
+                                      int32_t state_bytes, const double* totals_dev, const void* weights_dev,
+                                      int64_t weights_stride, void* ll_out_dev, void* gradient_out_dev,
+                                      int64_t gradient_stride, void* stream);
+
+/*
+ * The global norm of many gradient tensors, and clipping by it:
+ *   norm = sqrt(sum over all tensors and elements of g^2)
+ *   out  = g * (max_norm / norm if norm > max_norm, else 1)
+ * A set names its tensors once (addresses, sizes and types, which may differ from tensor to tensor);
+ * every call is then two launches, however many tensors there are (the reference's models have
+ * one CPT per node, 785 in dev_experiments/mnist/mnist.py, and no gradient).  Squares are summed in
+ * double, in an order that depends on the set alone.  A NaN norm makes every output NaN; an infinite
+ * one gives factor 0 (so infinite gradients become NaN, the others 0): callers look at the norm.
+ *   sizes        elements of each tensor (contiguous; 0 is skipped)
+ *   outputs_dev  where each tensor's clipped copy goes: its own address (in place) or memory that no
+ *                tensor of the set overlaps; anything else is refused
+ * Creation allocates and copies a table (not under graph capture).  A set is bound to the device it was created on, and the tensors must stay where they
+ * are while it is used.  The other calls allocate nothing, may be captured, and need a
+ * workspace each when they may overlap.  0 < max_norm < inf.
+ */
+typedef struct bn_gradient_set bn_gradient_set;
+int bn_gradient_set_create(int32_t num_tensors, const int32_t* dtypes, const int64_t* sizes,
+                           const void* const* gradients_dev, void* const* outputs_dev, bn_gradient_set** out_set);
+int bn_gradient_set_destroy(bn_gradient_set* set);
+/* Bytes of device workspace the calls below need (-1 for NULL). */
+int64_t bn_gradient_set_workspace_bytes(const bn_gradient_set* set);
+/* *norm_out_dev = the norm; the outputs are not touched. */
+int bn_gradient_set_norm(bn_gradient_set* set, void* workspace_dev, double* norm_out_dev, void* stream);
+/* *norm_out_dev = the norm before clipping; every tensor's scaled copy to its output. */
+int bn_gradient_set_clip(bn_gradient_set* set, double max_norm, void* workspace_dev, double* norm_out_dev,
+                         void* stream);
 
 /*
  * Per-kernel timing for benchmarks (process-wide switch): while enabled, every kernel any

@@ -1,0 +1,269 @@
+"""Draws from rows of logits against the definition in 64 bits, at the lengths where the kernels change
+hands, with ties, masks, padding and every filter.
+
+The states have to be equal.  Both sides sum in double (the kept set's borders partly in integers
+of 2^-38 of a weight or finer), so they can only differ where a border lies within 1e-10 of the target;
+the oracle says how far its borders are, and no test row here is nearer than that unless all its sums are
+exact (equal weights)."""
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.float64, torch.float16, torch.bfloat16]
+
+
+def _oracle(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(state, distance of the nearest border that decided it, relative to the sums)"""
+    x = np.asarray(x, dtype=np.float64)
+    n = x.size
+    if n == 0 or np.isnan(x).any() or np.isposinf(x).any() or np.isneginf(x).all() or not 0 <= u <= 1:
+        return -1, 1.0
+    if temperature == 0:
+        return int(np.argmax(x)), 1.0
+    w = np.exp((x - x.max()) / temperature)
+    order = np.argsort(-x, kind="stable")
+    margin = 1.0
+    if 0 < top_k < n:
+        order = order[:top_k]
+    if top_p < 1:
+        upto = np.cumsum(w[order])
+        before = np.concatenate([[0.0], upto[:-1]])
+        margin = min(margin, np.abs(upto / upto[-1] - top_p).min())
+        order = order[before < top_p * upto[-1]] if top_p > 0 else order[:1]
+    if min_p > 0:
+        margin = min(margin, np.abs(w[order] - min(min_p, 1.0)).min() if min_p < 1 else 1.0)
+        order = order[w[order] >= min(min_p, 1.0)]
+    order = np.sort(order)
+    upto = np.cumsum(w[order])
+    target = u * upto[-1]
+    margin = min(margin, np.abs(upto[:-1] - target).min() / upto[-1] if order.size > 1 else 1.0)
+    at = np.searchsorted(upto, target, side="right")
+    if at == order.size:
+        at = np.flatnonzero(w[order])[-1]
+    return int(order[at]), margin
+
+
+def _check(got, rows, uniforms, settings, exact_sums=False):
+    got = got.cpu().numpy()
+    for r, x in enumerate(rows):
+        want, margin = _oracle(x, float(uniforms[r]), **{k: v[r] if hasattr(v, "__len__") else v
+                                                         for k, v in settings.items()})
+        assert exact_sums or margin > 1e-10, (r, margin)
+        assert got[r] == want, (r, got[r], want, margin)
+
+
+SETTINGS = {
+    "none": {},
+    "greedy": dict(temperature=0.0),
+    "cold": dict(temperature=0.3),
+    "top_k": dict(top_k=5),
+    "top_k 300": dict(top_k=300, temperature=2.0),
+    "top_p": dict(temperature=1.5, top_p=0.9),
+    "top_p small": dict(top_p=0.05),
+    "min_p": dict(min_p=0.1),
+    "all": dict(temperature=1.2, top_k=40, top_p=0.8, min_p=0.02),
+}
+
+
+@pytest.mark.parametrize("setting", SETTINGS, ids=list(SETTINGS))
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("states", [1, 2, 3, 8, 9, 17, 33, 64, 65, 200, 513, 1024, 1025, 4099, 20001])
+def test_follows_the_definition(states, dtype, setting):
+    from bayesiannetwork_amd.samplers import draw_states
+
+    gen = torch.Generator().manual_seed(states)
+    rows = 37 if states < 2000 else 5
+    x = (2.5 * torch.randn((rows, states), generator=gen)).to(dtype)
+    u = torch.rand((rows,), generator=gen, dtype=torch.float64)
+    got = draw_states(x.cuda(), u.cuda(), **SETTINGS[setting])
+    assert got.shape == (rows,) and got.dtype == torch.int32
+    _check(got, x.double().numpy(), u.numpy(), SETTINGS[setting])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("states", [11, 64, 700, 6001])
+def test_settings_and_lengths_of_every_row(states, dtype):
+    """One call with greedy, unfiltered and filtered rows, rows of 0 states to all of them, settings
+    beyond their range (off), in a buffer whose padding holds NaN and infinities."""
+    from bayesiannetwork_amd.samplers import draw_states
+
+    gen = torch.Generator().manual_seed(7 * states)
+    rows = 60
+    x = (2.0 * torch.randn((rows, states), generator=gen)).to(dtype)
+    u = torch.rand((rows,), generator=gen, dtype=torch.float32)
+    counts = torch.randint(0, states + 1, (rows,), generator=gen)
+    counts[:4] = torch.tensor([0, 1, states, states + 5])  # more than the row: all of it
+    padded = x.clone()
+    for r in range(rows):
+        padded[r, int(counts[r]):] = [float("nan"), float("inf"), 3.0][r % 3]
+    pick = lambda values: torch.tensor([values[int(i)] for i in torch.randint(0, len(values), (rows,), generator=gen)])
+    settings = dict(temperature=pick([0.0, 0.7, 1.0, 1.9]).double(), top_k=pick([0, 1, 7, 50, 10**12, -3]),
+                    top_p=pick([1.0, 0.9, 0.35, 1.7]).double(), min_p=pick([0.0, 0.05, -1.0]).double())
+    got = draw_states(padded.cuda(), u.cuda(), num_states=counts.cuda(), **{k: v.cuda() for k, v in settings.items()})
+    plain = {k: v.numpy() for k, v in settings.items()}
+    _check(got, [x[r, : int(counts[r])].double().numpy() for r in range(rows)], u.double().numpy(), plain)
+
+
+@pytest.mark.parametrize("states", [10, 64, 300, 5000])
+def test_equal_logits_are_taken_by_index(states):
+    """All weights are 1 and all sums exact: the borders themselves are tested.  Half the states lie on one
+    key, the other half far below."""
+    from bayesiannetwork_amd.samplers import draw_states
+
+    x = torch.full((1, states), -200.0)
+    x[0, 1::2] = 3.0  # the weight of the others is exp(-203): none of them moves a sum
+    top = states // 2
+    u = torch.tensor([0.0, 0.25, 0.5, 0.75, 1.0], dtype=torch.float64)
+    rows = x.expand(u.numel(), states)  # row stride 0
+    for settings in (dict(), dict(top_k=3), dict(top_k=top), dict(top_p=0.5), dict(top_p=0.5, top_k=4), dict(min_p=1.0)):
+        got = draw_states(rows.cuda(), u.cuda(), **settings)
+        _check(got, rows.double().numpy(), u.numpy(), settings, exact_sums=True)
+    assert draw_states(rows.cuda(), u.cuda(), top_k=1).cpu().tolist() == [1] * 5
+    assert draw_states(rows.cuda(), u.cuda(), temperature=0.0).cpu().tolist() == [1] * 5
+
+
+@pytest.mark.parametrize("states", [5, 40, 300, 3000])
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=2), dict(top_p=0.9), dict(temperature=0.0)], ids=str)
+def test_masks_and_values_that_are_no_numbers(states, settings):
+    from bayesiannetwork_amd.samplers import draw_states
+
+    inf, low = float("inf"), torch.finfo(torch.float32).min
+    rows = torch.zeros((9, states))
+    rows[0] = -inf  # nothing possible
+    rows[1] = -inf
+    rows[1, states - 1] = -4.0  # one state possible
+    rows[2, 2] = float("nan")
+    rows[3, 0] = inf
+    rows[4] = low  # masked with the type's lowest value: equal weights
+    rows[5] = low
+    rows[5, 3] = 1.0
+    rows[6, ::2] = -0.0  # one key with 0
+    rows[7, 1:] = -inf
+    rows[8] = torch.finfo(torch.float32).max
+    rows[8, 1] = low  # the difference overflows float32
+    u = torch.full((9,), 0.625, dtype=torch.float64)
+    got = draw_states(rows.cuda(), u.cuda(), **settings)
+    _check(got, rows.double().numpy(), u.numpy(), settings, exact_sums=True)
+    assert got[:4].cpu().tolist() == [-1, states - 1, -1, -1]
+
+
+def test_uniform_numbers_and_settings_of_a_row_that_cannot_be_drawn():
+    from bayesiannetwork_amd.samplers import draw_states
+
+    nan, inf = float("nan"), float("inf")
+    x = torch.zeros((6, 8), device="cuda")
+    u = torch.tensor([nan, -0.1, 1.1, 0.0, 1.0, 0.5], device="cuda")
+    assert draw_states(x, u).cpu().tolist() == [-1, -1, -1, 0, 7, 4]
+    u = torch.full((6,), 0.99, device="cuda")
+    t = torch.tensor([nan, -1.0, inf, 0.0, 1.0, 1e-300], device="cuda", dtype=torch.float64)
+    assert draw_states(x, u, temperature=t).cpu().tolist() == [-1, -1, -1, 0, 7, 7]
+    p = torch.tensor([nan, 0.0, -2.0, 0.25, 1.0, 9.0], device="cuda")
+    assert draw_states(x, u, top_p=p).cpu().tolist() == [7, 0, 0, 1, 7, 7]
+    m = torch.tensor([nan, 0.0, 5.0, 1.0, -1.0, 0.5], device="cuda")
+    assert draw_states(x, u, min_p=m).cpu().tolist() == [7] * 6
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("states", [13, 1500])
+def test_rows_anywhere_in_a_buffer(states, dtype):
+    """Odd row strides and first elements: the same states as from a copy."""
+    from bayesiannetwork_amd.samplers import draw_states
+
+    gen = torch.Generator().manual_seed(3)
+    buffer = torch.randn((21, states + 7), generator=gen).to(dtype).cuda()
+    u = torch.rand((21,), generator=gen).cuda()
+    for first in (0, 1, 3, 6):
+        view = buffer[:, first : first + states]
+        for settings in (dict(), dict(top_p=0.8), dict(top_k=9)):
+            assert torch.equal(draw_states(view, u, **settings), draw_states(view.contiguous(), u, **settings))
+    assert torch.equal(draw_states(view, u[::2].repeat_interleave(2)[:21]),
+                       draw_states(view, torch.stack([u[::2].repeat_interleave(2)[:21]] * 2, dim=1)[:, 0]))
+
+
+def test_refusals():
+    from bayesiannetwork_amd.samplers import draw_states
+
+    x, u = torch.zeros((3, 4), device="cuda"), torch.zeros(3, device="cuda")
+    for call, error in [
+        (lambda: draw_states(x.t(), u), ValueError),
+        (lambda: draw_states(x, u[:2]), ValueError),
+        (lambda: draw_states(x, u.half()), TypeError),
+        (lambda: draw_states(x, u.cpu()), ValueError),
+        (lambda: draw_states(x, u, temperature=-1), ValueError),
+        (lambda: draw_states(x, u, top_p=0.0), ValueError),
+        (lambda: draw_states(x, u, min_p=1.5), ValueError),
+        (lambda: draw_states(x, u, top_k=-1), ValueError),
+        (lambda: draw_states(x, u, top_k=2.5), ValueError),
+        (lambda: draw_states(x, u, top_k=u), TypeError),
+        (lambda: draw_states(x, u, temperature=u[:1]), ValueError),
+        (lambda: draw_states(x, u, num_states=u), TypeError),
+    ]:
+        with pytest.raises(error):
+            call()
+    assert draw_states(x[:0], u[:0]).shape == (0,)
+
+
+def test_long_rows_of_flat_and_peaked_distributions():
+    """A flat row keeps most of its states, a peaked one few: 131 072 states in bfloat16 (many ties) and
+    100 003 in float32."""
+    from bayesiannetwork_amd.samplers import draw_states
+
+    gen = torch.Generator().manual_seed(5)
+    for states, dtype in ((131072, torch.bfloat16), (100003, torch.float32)):
+        x = torch.randn((6, states), generator=gen)
+        x[:2] *= 0.01
+        x[2:4] *= 6.0
+        x = x.to(dtype)
+        u = torch.rand((6,), generator=gen, dtype=torch.float64)
+        for settings in (dict(), dict(top_p=0.97), dict(top_k=5000), dict(top_k=20000, top_p=0.5, min_p=1e-4)):
+            _check(draw_states(x.cuda(), u.cuda(), **settings), x.double().numpy(), u.numpy(), settings)
+
+
+def test_frequencies_of_a_posterior():
+    """Draws from a machine's posterior follow it (chi-square, alpha = 0.001)."""
+    from scipy import stats
+
+    from bayesiannetwork_amd.samplers import draw_states
+
+    p = torch.tensor([0.05, 0.1, 0.0, 0.4, 0.45], dtype=torch.float64)
+    n = 200_000
+    u = torch.rand((n,), generator=torch.Generator().manual_seed(9), dtype=torch.float32)
+    got = draw_states(p.log().float().cuda().expand(n, 5), u.cuda()).cpu().long()
+    counts = torch.bincount(got, minlength=5).double()
+    assert counts[2] == 0
+    keep = p > 0
+    _, level = stats.chisquare(counts[keep].numpy(), (p[keep] / p[keep].sum() * n).numpy())
+    assert level > 0.001
+
+
+@pytest.mark.parametrize("states", [10, 300, 40000])
+def test_captured_and_on_another_stream(states):
+    """Two graphs and eager calls, replayed in turn with new inputs: each replay equals an eager call."""
+    from bayesiannetwork_amd.samplers import draw_states
+
+    gen = torch.Generator().manual_seed(1)
+    x = torch.randn((16, states), generator=gen).cuda()
+    u = torch.rand((16,), generator=gen).cuda()
+    settings = dict(top_k=20, top_p=0.9)
+    draw_states(x, u, **settings)
+    graphs = []
+    for kwargs in (settings, dict(temperature=0.5)):
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            draw_states(x, u, **kwargs)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = draw_states(x, u, **kwargs)
+        graphs.append((graph, out, kwargs))
+    for step in range(4):
+        x.copy_(torch.randn((16, states), generator=gen))
+        u.copy_(torch.rand((16,), generator=gen))
+        for graph, out, kwargs in graphs:
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, draw_states(x, u, **kwargs))

@@ -7,7 +7,7 @@ OBJ   := build
 # -MMD: every object depends on exactly the headers it includes (build/*.d)
 FLAGS := -O3 -std=c++17 -fPIC --offload-arch=$(ARCH) -Wall -Wno-unused-function -Iinclude -MMD -MP
 # the operators on rows of logits and on gradients are compiled without packed float32 instructions
-ROW_OBJS := $(OBJ)/draw_states.o $(OBJ)/states_likelihood.o $(OBJ)/gradient_clip.o
+ROW_OBJS := $(OBJ)/draw_states.o $(OBJ)/draw_f32.o $(OBJ)/draw_f64.o $(OBJ)/draw_f16.o $(OBJ)/draw_bf16.o $(OBJ)/states_likelihood.o $(OBJ)/gradient_clip.o
 $(ROW_OBJS): FLAGS += -Xclang -target-feature -Xclang -packed-fp32-ops
 OBJS  := $(ROW_OBJS) $(OBJ)/api.o $(OBJ)/leaf_f32.o $(OBJ)/leaf_f64.o $(OBJ)/exact.o $(OBJ)/sampler.o $(OBJ)/plan.o $(OBJ)/packs.o
 # Cardinality packs built with the library (csrc/cardinality_pack.h): the fused kernels for wide parents

@@ -46,7 +46,7 @@ extern "C" {
 int64_t bn_draw_states_workspace_bytes(int dtype, int64_t rows, int64_t num_states) {
   if (dtype_bytes(dtype) == 0 || rows < 0 || rows > (int64_t)1 << 40 || num_states < 1 || num_states > kMaxStates) return -1;
   const int64_t key_bytes = dtype == BN_F64 ? 8 : 4;
-  return std::max<int64_t>(rows * blocks_per_row(num_states) * (8 + key_bytes), 8);
+  return rows * blocks_per_row(num_states) * (8 + key_bytes);
 }
 
 int bn_draw_states(int dtype, const void* logits_dev, int64_t rows, int64_t num_states, int64_t row_stride,
@@ -67,13 +67,16 @@ int bn_draw_states(int dtype, const void* logits_dev, int64_t rows, int64_t num_
   if (uniform_dtype != BN_F32 && uniform_dtype != BN_F64)
     return fail(BN_ERR_INVALID, "uniform_dtype must be BN_F32 or BN_F64");
   if (rows == 0) return BN_OK;
-  if (!logits_dev || !uniforms_dev || !workspace_dev || !out_dev) return fail(BN_ERR_INVALID, "null argument");
+  a.blocks_per_row = blocks_per_row(num_states);
+  if (!logits_dev || !uniforms_dev || !out_dev || (a.blocks_per_row > 0 && !workspace_dev))
+    return fail(BN_ERR_INVALID, "null argument");
   if (reinterpret_cast<uintptr_t>(logits_dev) % dtype_bytes(dtype))
     return fail(BN_ERR_INVALID, "row address not aligned to its type");
   if (reinterpret_cast<uintptr_t>(workspace_dev) % 8) return fail(BN_ERR_INVALID, "workspace not aligned to 8 bytes");
-  a.blocks_per_row = blocks_per_row(num_states);
-  a.block_sums = static_cast<double*>(workspace_dev);
-  a.block_keys = a.block_sums + rows * a.blocks_per_row;
+  if (a.blocks_per_row > 0) {
+    a.block_sums = static_cast<double*>(workspace_dev);
+    a.block_keys = a.block_sums + rows * a.blocks_per_row;
+  }
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case BN_F32: BN_HIP_CHECK(launch_f32(a, s)); break;

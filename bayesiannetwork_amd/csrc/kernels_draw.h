@@ -161,27 +161,6 @@ __device__ __forceinline__ double Weight::of_key<uint64_t>(uint64_t k) const {
 
 // ---- lanes ------------------------------------------------------------------------------------
 
-// A 32-bit word of the lane whose number differs by MASK: quad permutations and row mirrors in the
-// register file, the LDS crossbar for the rest.
-template <int MASK>
-__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
-  if constexpr (MASK == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true);
-  else if constexpr (MASK == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true);
-  else if constexpr (MASK == 3) return __builtin_amdgcn_mov_dpp(v, 0x1B, 0xF, 0xF, true);
-  else if constexpr (MASK == 7) return __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, true);
-  else if constexpr (MASK == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, true);
-  else if constexpr (MASK == 15) return __builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, true);
-  else return (uint32_t)__shfl_xor((int)v, MASK, 64);
-}
-template <int MASK>
-__device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
-  return ((uint64_t)lane_xor<MASK>((uint32_t)(v >> 32)) << 32) | lane_xor<MASK>((uint32_t)v);
-}
-template <int MASK>
-__device__ __forceinline__ double lane_xor(double v) {
-  return __longlong_as_double((long long)lane_xor<MASK>((uint64_t)__double_as_longlong(v)));
-}
-
 // Exclusive prefix sum over the G lanes of a group, and the group's total.
 template <int G>
 __device__ __forceinline__ double group_scan(double v, double* total) {

@@ -68,24 +68,75 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T>& v) {
   *reinterpret_cast<Pack<T>*>(p) = v;
 }
 
-template <int WIDTH>
-__device__ __forceinline__ float lanes_max(float v) {
+// The same past the caches' usual order of replacement, for what this kernel does not read again.
+template <typename T>
+__device__ __forceinline__ void store_pack_streamed(T* p, const Pack<T>& v) {
+  typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+  __builtin_nontemporal_store(__builtin_bit_cast(Words, v), reinterpret_cast<Words*>(p));
+}
+
+// The 16 bytes as four registers.  kept() hides where they came from, so that what was unpacked from them
+// before (twice the registers for 16-bit types) is not kept alive for later use instead.
+struct Raw {
+  uint32_t w[4];
+};
+template <typename T>
+__device__ __forceinline__ Raw raw_of(const Pack<T>& p) {
+  return __builtin_bit_cast(Raw, p);
+}
+template <typename T>
+__device__ __forceinline__ Pack<T> pack_of(const Raw& r) {
+  return __builtin_bit_cast(Pack<T>, r);
+}
+__device__ __forceinline__ void kept(Raw& r) {
 #pragma unroll
-  for (int d = 1; d < WIDTH; d <<= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
+  for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(r.w[i]));
+}
+
+// A 32-bit word of the lane whose number differs by MASK: quad permutations and mirrors within the register
+// file for the masks that have one, the LDS crossbar for the rest.
+template <int MASK>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  if constexpr (MASK == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true);
+  else if constexpr (MASK == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true);
+  else if constexpr (MASK == 3) return __builtin_amdgcn_mov_dpp(v, 0x1B, 0xF, 0xF, true);
+  else if constexpr (MASK == 7) return __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, true);
+  else if constexpr (MASK == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, true);
+  else if constexpr (MASK == 15) return __builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, true);
+  else return (uint32_t)__shfl_xor((int)v, MASK, 64);
+}
+template <int MASK>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
+  return ((uint64_t)lane_xor<MASK>((uint32_t)(v >> 32)) << 32) | lane_xor<MASK>((uint32_t)v);
+}
+template <int MASK>
+__device__ __forceinline__ float lane_xor(float v) {
+  return __uint_as_float(lane_xor<MASK>(__float_as_uint(v)));
+}
+template <int MASK>
+__device__ __forceinline__ double lane_xor(double v) {
+  return __longlong_as_double((long long)lane_xor<MASK>((uint64_t)__double_as_longlong(v)));
+}
+
+// Reductions over groups of WIDTH lanes, the same result in every lane, taken in the same tree.  Once four
+// lanes agree, mirroring eight of them is as good as exchanging the fours.
+template <int WIDTH, typename W, typename Combine>
+__device__ __forceinline__ W lanes_all(W v, Combine combine) {
+  if constexpr (WIDTH >= 2) v = combine(v, lane_xor<1>(v));
+  if constexpr (WIDTH >= 4) v = combine(v, lane_xor<2>(v));
+  if constexpr (WIDTH >= 8) v = combine(v, lane_xor<7>(v));
+  if constexpr (WIDTH >= 16) v = combine(v, lane_xor<15>(v));
+  if constexpr (WIDTH >= 32) v = combine(v, lane_xor<16>(v));
+  if constexpr (WIDTH >= 64) v = combine(v, lane_xor<32>(v));
   return v;
 }
-template <int WIDTH>
-__device__ __forceinline__ double lanes_max(double v) {
-#pragma unroll
-  for (int d = 1; d < WIDTH; d <<= 1) v = fmax(v, __shfl_xor(v, d, 64));
-  return v;
+template <int WIDTH, typename W>
+__device__ __forceinline__ W lanes_max(W v) {
+  return lanes_all<WIDTH>(v, [](W p, W q) { return fmax(p, q); });
 }
-// every lane of the group ends with the same sum, taken in the same tree
 template <int WIDTH, typename W>
 __device__ __forceinline__ W lanes_sum(W v) {
-#pragma unroll
-  for (int d = 1; d < WIDTH; d <<= 1) v += __shfl_xor(v, d, 64);
-  return v;
+  return lanes_all<WIDTH>(v, [](W p, W q) { return p + q; });
 }
 
 }  // namespace bn_rows

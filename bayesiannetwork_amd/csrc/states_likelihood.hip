@@ -72,31 +72,29 @@ struct Total {
   __device__ __forceinline__ W reference() const { return isinf(best) && best < 0 ? (W)0 : best; }
 };
 
-// ll of the row, in double: the difference to the largest logit is not rounded together with the
-// logarithm, so a row whose state is nearly certain keeps its small value's digits
+// ll of a row, in double: the difference to the largest logit is not rounded together with the
+// logarithm, so a row whose state is nearly certain keeps its small value's digits.  `target` is the
+// state's logit.
 template <typename T, typename W>
-__device__ __forceinline__ void finish_row(const Rows& a, int64_t r, const T* x, int64_t state, const Total<W>& total) {
-  using Out = typename Value<T>::Wide;
+__device__ __forceinline__ void finish_row(const Rows& a, int64_t r, bool observed, W target, const Total<W>& total) {
   double ll = 0.0;
-  if (state >= 0) {
-    const double target = (double)Value<T>::widen(x[state]);
-    ll = total.sum == (W)0 ? -INFINITY : (target - (double)total.reference()) - log((double)total.sum);
-  }
-  if (a.ll) static_cast<Out*>(a.ll)[r] = (Out)ll;
+  if (observed)
+    ll = total.sum == (W)0 ? -INFINITY : ((double)target - (double)total.reference()) - log((double)total.sum);
+  if (a.ll) static_cast<W*>(a.ll)[r] = (W)ll;
   if (a.totals) {
     a.totals[2 * r] = (double)total.best;
     a.totals[2 * r + 1] = (double)total.sum;
   }
 }
 
-// Gradient of a row: weight * ([i = state] - exp(x_i - best) / sum).
+// Gradient of a row: weight * ([i = state] - exp(x_i - best) / sum), 0 for a row that was not observed.
 template <typename W>
 struct Slope {
   W reference, scale, weight;
-  int64_t state;
-  __device__ __forceinline__ W at(W x, int64_t i) const {
+  bool observed;
+  __device__ __forceinline__ W at(W x, bool is_state) const {
     const W p = exp_wide(x - reference) * scale;
-    return weight * ((i == state ? (W)1 : (W)0) - p);
+    return weight * ((is_state ? (W)1 : (W)0) - p);
   }
 };
 
@@ -106,71 +104,142 @@ __device__ __forceinline__ typename Value<T>::Wide row_weight(const Rows& a, int
   return a.weights ? static_cast<const W*>(a.weights)[r * a.weights_stride] : (W)1;
 }
 
+template <typename W>
+__device__ __forceinline__ Slope<W> slope_from_total(W weight, bool observed, const Total<W>& total) {
+  // sum 0: no possible state, no gradient
+  const bool none = total.sum == (W)0;
+  return {total.reference(), none ? (W)0 : (W)1 / total.sum, none ? (W)0 : weight, observed};
+}
+
+// The gradient at the V states from i on, of which the row has n (x: their logits); the row's state is `at`
+// places behind i.  0 beyond the row.
 template <typename T, typename W>
-__device__ __forceinline__ Slope<W> slope_from_total(const Rows& a, int64_t r, int64_t state, const Total<W>& total) {
-  // sum 0 (no possible state): scale 0 and weight 0 below
-  const W weight = total.sum == (W)0 ? (W)0 : row_weight<T>(a, r);
-  const W scale = total.sum == (W)0 ? (W)0 : (W)1 / total.sum;
-  return {total.reference(), scale, weight, state};
+__device__ __forceinline__ Pack<T> gradient_pack(const Slope<W>& slope, Pack<T> x, int64_t at, int64_t inside) {
+  constexpr int V = Value<T>::kVec;
+  const int place = (uint64_t)at < (uint64_t)V ? (int)at : -1;
+  if (!slope.observed) inside = 0;
+  if (inside >= V) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) x.v[j] = Value<T>::round(slope.at(Value<T>::widen(x.v[j]), place == j));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      x.v[j] = Value<T>::round(j < inside ? slope.at(Value<T>::widen(x.v[j]), place == j) : (W)0);
+  }
+  return x;
+}
+
+// Stores the part of a pack that lies inside a row of `width` states.
+template <typename T, typename Index>
+__device__ __forceinline__ void store_row_pack(T* out, Index i, Index width, const Pack<T>& p) {
+  constexpr int V = Value<T>::kVec;
+  if (i + V <= width) {
+    store_pack(out + i, p);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (i + j < width) out[i + j] = p.v[j];
+  }
+}
+
+// The V logits from i on, -inf where the row's n states have ended.
+template <typename T, typename Index>
+__device__ __forceinline__ Pack<T> row_pack(const T* x, Index i, Index n) {
+  constexpr int V = Value<T>::kVec;
+  Pack<T> p;
+  if (i + V <= n) {
+    p = load_pack(x + i);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) p.v[j] = i + j < n ? x[i + j] : Value<T>::round(-INFINITY);
+  }
+  return p;
+}
+
+// The same as registers that stay packed.
+template <typename T, typename Index>
+__device__ __forceinline__ Raw row_raw(const T* x, Index i, Index n) {
+  Raw raw;
+  if (i + Value<T>::kVec <= n) {
+    raw = raw_of(load_pack(x + i));
+  } else {
+    raw = raw_of(row_pack(x, i, n));
+  }
+  return raw;
 }
 
 // ---- short rows: LANES lanes hold a row as PACKS packs each -----------------------------------
 
-template <typename T, int LANES, int PACKS, int MODE>
+// A group takes KEEP rows, all loaded before the first is worked on; the logarithms of their sums (a hundred
+// double instructions, whatever the number of lanes that need one) are left to the end, where lane k has
+// row k's.
+template <typename T, int LANES, int PACKS, int KEEP, int MODE>
 __global__ void __launch_bounds__(256) rows_in_lanes(const Rows a) {
   using W = typename Value<T>::Wide;
   constexpr int V = Value<T>::kVec;
-  constexpr int kRowsPerBlock = 256 / LANES;
-  const int lane = threadIdx.x % LANES;
+  constexpr int kRowsPerBlock = 256 / LANES * KEEP;
+  static_assert(KEEP <= LANES, "one lane per kept row");
+  const int lane = threadIdx.x % LANES, width = (int)a.width;
   for (int64_t r0 = (int64_t)blockIdx.x * kRowsPerBlock; r0 < a.rows; r0 += (int64_t)gridDim.x * kRowsPerBlock) {
-    const int64_t r = r0 + threadIdx.x / LANES;
-    if (r >= a.rows) continue;  // whole groups leave together: the shuffles below stay within a group
-    const T* x = static_cast<const T*>(a.logits) + r * a.stride;
-    const int64_t n = row_count(a, r);
-    const int64_t state = row_state(a, r, n);
-    W v[PACKS * V];
-    W best = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < PACKS; ++k) {
-      const int64_t i = (int64_t)(k * LANES + lane) * V;
-      if (i + V <= n) {
-        const Pack<T> p = load_pack(x + i);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[k * V + j] = Value<T>::widen(p.v[j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[k * V + j] = i + j < n ? Value<T>::widen(x[i + j]) : (W)-INFINITY;
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) best = fmax(best, v[k * V + j]);
+    const int64_t base = r0 + (int64_t)(threadIdx.x / LANES) * KEEP;
+    if (base >= a.rows) continue;  // whole groups leave together: the exchanges below stay within a group
+    // lane k < KEEP knows row base + k
+    const int64_t own = base + lane;
+    const bool owner = lane < KEEP && own < a.rows;
+    int own_count = 0, own_state = -1;
+    W own_target = 0, own_weight = 0;
+    if (owner) {
+      own_count = (int)row_count(a, own);
+      own_state = (int)row_state(a, own, own_count);
+      if (own_state >= 0) own_target = Value<T>::widen(static_cast<const T*>(a.logits)[own * a.stride + own_state]);
+      if (MODE == kBoth) own_weight = row_weight<T>(a, own);
     }
-    Total<W> total;
-    total.best = lanes_max<LANES>(best);
-    const W reference = total.reference();
-    W sum = 0;
+    Raw raw[KEEP][PACKS];
 #pragma unroll
-    for (int k = 0; k < PACKS * V; ++k) sum += exp_wide(v[k] - reference);
-    total.sum = lanes_sum<LANES>(sum);
-    if (lane == 0) finish_row<T>(a, r, x, state, total);
-    if constexpr (MODE == kBoth) {
-      const Slope<W> slope = slope_from_total<T>(a, r, state, total);
-      T* out = static_cast<T*>(a.gradient) + r * a.gradient_stride;
+    for (int q = 0; q < KEEP; ++q) {
+      const T* x = static_cast<const T*>(a.logits) + (base + q) * a.stride;
+      const int n = __shfl(own_count, q, LANES);
+#pragma unroll
+      for (int k = 0; k < PACKS; ++k) raw[q][k] = row_raw(x, (k * LANES + lane) * V, n);
+    }
+    Total<W> own_total{(W)-INFINITY, (W)0};
+#pragma unroll
+    for (int q = 0; q < KEEP; ++q) {
+      W best = -INFINITY;
 #pragma unroll
       for (int k = 0; k < PACKS; ++k) {
-        const int64_t i = (int64_t)(k * LANES + lane) * V;
-        Pack<T> p;
+        kept(raw[q][k]);
+        const Pack<T> p = pack_of<T>(raw[q][k]);
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          p.v[j] = Value<T>::round(state >= 0 && i + j < n ? slope.at(v[k * V + j], i + j) : (W)0);
-        if (i + V <= a.width) {
-          store_pack(out + i, p);
-        } else {
+        for (int j = 0; j < V; ++j) best = fmax(best, Value<T>::widen(p.v[j]));
+      }
+      Total<W> total;
+      total.best = lanes_max<LANES>(best);
+      const W reference = total.reference();
+      W sum = 0;
 #pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (i + j < a.width) out[i + j] = p.v[j];
+      for (int k = 0; k < PACKS; ++k) {
+        kept(raw[q][k]);
+        const Pack<T> p = pack_of<T>(raw[q][k]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum += exp_wide(Value<T>::widen(p.v[j]) - reference);
+      }
+      total.sum = lanes_sum<LANES>(sum);
+      if (lane == q) own_total = total;
+      if constexpr (MODE == kBoth) {
+        if (base + q >= a.rows) continue;
+        const int n = __shfl(own_count, q, LANES), state = __shfl(own_state, q, LANES);
+        const Slope<W> slope = slope_from_total(__shfl(own_weight, q, LANES), state >= 0, total);
+        T* out = static_cast<T*>(a.gradient) + (base + q) * a.gradient_stride;
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k) {
+          const int i = (k * LANES + lane) * V;
+          kept(raw[q][k]);
+          if (i < width) store_row_pack(out, i, width, gradient_pack(slope, pack_of<T>(raw[q][k]), state - i, n - i));
         }
       }
     }
+    if (owner) finish_row<T>(a, own, own_state >= 0, own_target, own_total);
   }
 }
 
@@ -184,7 +253,6 @@ __device__ __forceinline__ W block_max(W v, W* lds) {
   W m = lds[0];
 #pragma unroll
   for (int w = 1; w < THREADS / 64; ++w) m = fmax(m, lds[w]);
-  __syncthreads();
   return m;
 }
 
@@ -196,100 +264,208 @@ __device__ __forceinline__ W block_sum(W v, W* lds) {
   W s = 0;
 #pragma unroll
   for (int w = 0; w < THREADS / 64; ++w) s += lds[w];
-  __syncthreads();
   return s;
 }
 
-// Two or three passes over the row in memory: maximum, sum and (both) the gradient.
+// Log-likelihood and gradient of rows that a block's registers hold.  A thread takes its logits' exponentials
+// relative to its own largest one and keeps them; once the block has agreed on the row's maximum and sum, one
+// factor per thread turns them into the gradient.  So every logit costs one exponential, and its register is
+// free again before the block has met: the next row's logits are requested then and arrive while this row is
+// reduced and written.  4096 rows of 64000 bfloat16 states, 1.05 GB, take 190 us, 5.5 TB/s; loading, reducing
+// and storing one after the other took 353 us (a CU holds one such row, and its memory pipe idled in
+// between), reading the row twice instead 318 us.
+// The gradient is stored past the caches' order: 190 us against 203 there, 8.7 against 10.3 at 1000 rows of
+// 5003 float32, where what reads it next is no slower for it (18.7 against 20.7 us together); between about
+// 100 and 256 MB the next reader loses more than is won here (4096 x 16000: 44 against 46 us alone, 99
+// against 92 together).
+//
+// A row is up to PACKS rounds of THREADS whole packs, by uniform addresses and without checks, and a rest of
+// less than a round with them (checks in the unrolled rounds cost more registers than the row itself).
+template <typename T, int THREADS, int PACKS>
+__global__ void __launch_bounds__(THREADS) rows_in_block(const Rows a) {
+  using W = typename Value<T>::Wide;
+  constexpr int V = Value<T>::kVec;
+  constexpr int kWaves = THREADS / 64;
+  constexpr int kRound = THREADS * V;  // states
+  __shared__ W maxima[2][kWaves], sums[2][kWaves];  // by turns: one barrier per row is enough
+  const int width = (int)a.width;
+  const uint32_t place = threadIdx.x * V;  // of this thread's pack in every round
+  const auto load = [&](const T* x, int k, int n) {
+    Raw raw;
+    if ((k + 1) * kRound <= n) {
+      raw = raw_of(load_pack((x + k * kRound) + place));
+    } else {
+      Pack<T> none;
+#pragma unroll
+      for (int j = 0; j < V; ++j) none.v[j] = Value<T>::round(-INFINITY);
+      raw = raw_of(none);
+    }
+    return raw;
+  };
+  int64_t r = blockIdx.x;
+  if (r >= a.rows) return;
+  int n = (int)row_count(a, r);
+  Raw raw[PACKS], rest;
+  {
+    const T* x = static_cast<const T*>(a.logits) + r * a.stride;
+#pragma unroll
+    for (int k = 0; k < PACKS; ++k) raw[k] = load(x, k, n);
+    rest = row_raw(x, n / kRound * kRound + (int)place, n);
+  }
+  for (int turn = 0;; turn ^= 1) {
+    const int64_t next = r + gridDim.x;
+    const bool more = next < a.rows;
+    const int next_n = more ? (int)row_count(a, next) : 0;
+    const int state = (int)row_state(a, r, n);
+    const W weight = row_weight<T>(a, r);
+    // the thread whose pack holds the row's state also writes its gradient, after the pack
+    const bool owner = (int)threadIdx.x == (state >= 0 ? state / V % THREADS : 0);
+    W target = 0;
+    if (owner && state >= 0) target = Value<T>::widen(static_cast<const T*>(a.logits)[r * a.stride + state]);
+    W own = -INFINITY;
+    const auto raise = [&](Raw& from) {
+      kept(from);
+      const Pack<T> p = pack_of<T>(from);
+#pragma unroll
+      for (int j = 0; j < V; ++j) own = fmax(own, Value<T>::widen(p.v[j]));
+    };
+#pragma unroll
+    for (int k = 0; k < PACKS; ++k) raise(raw[k]);
+    raise(rest);
+    const W reference = own == (W)-INFINITY ? (W)0 : own;
+    W e[PACKS + 1][V], sum = 0;
+    const auto add = [&](Raw& from, W (&to)[V]) {
+      kept(from);
+      const Pack<T> p = pack_of<T>(from);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        to[j] = exp_wide(Value<T>::widen(p.v[j]) - reference);
+        sum += to[j];
+      }
+    };
+    const T* next_x = static_cast<const T*>(a.logits) + next * a.stride;
+#pragma unroll
+    for (int k = 0; k < PACKS; ++k) {
+      add(raw[k], e[k]);
+      raw[k] = load(next_x, k, next_n);  // nothing if there is no next row
+    }
+    add(rest, e[PACKS]);
+    rest = row_raw(next_x, next_n / kRound * kRound + (int)place, next_n);
+    // (a thread or wave without possible states has sum 0 and stays out through the factor 0; NaN stays in)
+    const W wave_best = lanes_max<64>(own);
+    const W wave_sum = lanes_sum<64>(sum * (own == (W)-INFINITY ? (W)0 : exp_wide(own - wave_best)));
+    if ((threadIdx.x & 63) == 0) {
+      maxima[turn][threadIdx.x >> 6] = wave_best;
+      sums[turn][threadIdx.x >> 6] = wave_sum;
+    }
+    __syncthreads();  // every thread has read its logits, the owner the state's: the gradient may replace them
+    Total<W> total{(W)-INFINITY, (W)0};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) total.best = fmax(total.best, maxima[turn][w]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+      total.sum += sums[turn][w] * (maxima[turn][w] == (W)-INFINITY ? (W)0 : exp_wide(maxima[turn][w] - total.best));
+    const Slope<W> slope = slope_from_total(weight, state >= 0, total);
+    const W factor = (own == (W)-INFINITY ? (W)0 : exp_wide(own - total.best)) * slope.scale * -slope.weight;
+    T* out = static_cast<T*>(a.gradient) + r * a.gradient_stride;
+    int written = 0;  // states behind which the gradient is 0
+    if (state >= 0) {
+#pragma unroll
+      for (int k = 0; k < PACKS; ++k) {
+        if ((k + 1) * kRound <= n) {
+          Pack<T> g;
+#pragma unroll
+          for (int j = 0; j < V; ++j) g.v[j] = Value<T>::round(e[k][j] * factor);
+          store_pack_streamed((out + k * kRound) + place, g);
+        }
+      }
+      const int i = n / kRound * kRound + (int)place;
+      Pack<T> g;
+#pragma unroll
+      for (int j = 0; j < V; ++j) g.v[j] = Value<T>::round(e[PACKS][j] * factor);
+      if (i < n) store_row_pack(out, i, n, g);
+      written = n;
+    }
+    for (int i = written + (int)threadIdx.x; i < width; i += THREADS) out[i] = Value<T>::round((W)0);
+    if (owner) {
+      if (state >= 0) out[state] = Value<T>::round(slope.at(target, true));
+      finish_row<T>(a, r, state >= 0, target, total);
+    }
+    if (!more) return;
+    r = next;
+    n = next_n;
+  }
+}
+
+// Longer rows, or rows that only need their sum: one pass with a running maximum, whose change rescales the
+// sum, and (both) a second one over the row in memory.
 template <typename T, int THREADS, int MODE>
 __global__ void __launch_bounds__(THREADS) rows_streamed(const Rows a) {
   using W = typename Value<T>::Wide;
   constexpr int V = Value<T>::kVec;
-  __shared__ W lds[THREADS / 64];
+  __shared__ W maxima[THREADS / 64], sums[THREADS / 64];
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T* x = static_cast<const T*>(a.logits) + r * a.stride;
     const int64_t n = row_count(a, r);
     const int64_t state = row_state(a, r, n);
-    const int64_t packs = n / V;
-    W best = -INFINITY;
-    for (int64_t k = threadIdx.x; k < packs; k += THREADS) {
-      const Pack<T> p = load_pack(x + k * V);
+    W target = 0;
+    if (threadIdx.x == 0 && state >= 0) target = Value<T>::widen(x[state]);
+    Total<W> own{(W)-INFINITY, (W)0};
+#pragma unroll 2
+    for (int64_t i = (int64_t)threadIdx.x * V; i < n; i += THREADS * V) {
+      const Pack<T> p = row_pack(x, i, n);
+      W best = own.best;
 #pragma unroll
       for (int j = 0; j < V; ++j) best = fmax(best, Value<T>::widen(p.v[j]));
-    }
-    const int64_t tail = packs * V + threadIdx.x;
-    if (tail < n) best = fmax(best, Value<T>::widen(x[tail]));
-    Total<W> total;
-    total.best = block_max<THREADS>(best, lds);
-    const W reference = total.reference();
-    W sum = 0;
-    for (int64_t k = threadIdx.x; k < packs; k += THREADS) {
-      const Pack<T> p = load_pack(x + k * V);
-#pragma unroll
-      for (int j = 0; j < V; ++j) sum += exp_wide(Value<T>::widen(p.v[j]) - reference);
-    }
-    if (tail < n) sum += exp_wide(Value<T>::widen(x[tail]) - reference);
-    total.sum = block_sum<THREADS>(sum, lds);
-    if (threadIdx.x == 0) finish_row<T>(a, r, x, state, total);
-    if constexpr (MODE == kBoth) {
-      __syncthreads();  // finish_row reads the state's logit, which the gradient may overwrite
-      const Slope<W> slope = slope_from_total<T>(a, r, state, total);
-      T* out = static_cast<T*>(a.gradient) + r * a.gradient_stride;
-      const int64_t out_packs = a.width / V;
-      for (int64_t k = threadIdx.x; k < out_packs; k += THREADS) {
-        const int64_t i = k * V;
-        Pack<T> p;
-        if (k < packs) p = load_pack(x + i);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          W g = 0;
-          if (state >= 0 && i + j < n) g = slope.at(Value<T>::widen(k < packs ? p.v[j] : x[i + j]), i + j);
-          p.v[j] = Value<T>::round(g);
-        }
-        store_pack(out + i, p);
+      if (best > own.best) {
+        if (own.sum != (W)0) own.sum *= exp_wide(own.best - best);  // 0 stays 0 while best was -inf
+        own.best = best;
       }
-      const int64_t i = out_packs * V + threadIdx.x;
-      if (i < a.width) out[i] = Value<T>::round(state >= 0 && i < n ? slope.at(Value<T>::widen(x[i]), i) : (W)0);
+      const W reference = own.reference();
+#pragma unroll
+      for (int j = 0; j < V; ++j) own.sum += exp_wide(Value<T>::widen(p.v[j]) - reference);
     }
+    Total<W> total;
+    total.best = block_max<THREADS>(own.best, maxima);
+    if (own.sum != (W)0) own.sum *= exp_wide(own.reference() - total.reference());
+    total.sum = block_sum<THREADS>(own.sum, sums);
+    if constexpr (MODE == kBoth) {
+      const Slope<W> slope = slope_from_total(row_weight<T>(a, r), state >= 0, total);
+      T* out = static_cast<T*>(a.gradient) + r * a.gradient_stride;
+#pragma unroll 2
+      for (int64_t i = (int64_t)threadIdx.x * V; i < a.width; i += THREADS * V)
+        store_row_pack(out, i, a.width, gradient_pack(slope, row_pack(x, i, n), state - i, n - i));
+    }
+    if (threadIdx.x == 0) finish_row<T>(a, r, state >= 0, target, total);
+    __syncthreads();  // the next row writes maxima and sums
   }
 }
 
-// ---- the backward pass on its own: elementwise, from the rows' totals ----------------------
+// ---- the backward pass on its own: elementwise, from the rows' totals --------------------------
 
-// A block takes kPacksPerBlock packs of the output, row after row.
 constexpr int kBackwardThreads = 256;
 
-template <typename T>
-__global__ void __launch_bounds__(kBackwardThreads) rows_backward(const Rows a, int64_t packs_per_row) {
+// Index: uint32_t where all packs can be counted in 32 bits, whose division is five times cheaper.
+template <typename T, typename Index>
+__global__ void __launch_bounds__(kBackwardThreads) rows_backward(const Rows a, Index packs_per_row, Index packs) {
   using W = typename Value<T>::Wide;
   constexpr int V = Value<T>::kVec;
-  const int64_t total_packs = a.rows * packs_per_row;
-  for (int64_t q = (int64_t)blockIdx.x * kBackwardThreads + threadIdx.x; q < total_packs;
-       q += (int64_t)gridDim.x * kBackwardThreads) {
+  const Index step = (Index)gridDim.x * kBackwardThreads;
+  Index q = (Index)blockIdx.x * kBackwardThreads + threadIdx.x;
+  if (q >= packs) return;
+  while (true) {
     const int64_t r = q / packs_per_row;
-    const int64_t i = (q - r * packs_per_row) * V;
+    const int64_t i = (int64_t)(q - (Index)r * packs_per_row) * V;
     const T* x = static_cast<const T*>(a.logits) + r * a.stride;
-    T* out = static_cast<T*>(a.gradient) + r * a.gradient_stride;
     const int64_t n = row_count(a, r);
-    const int64_t state = row_state(a, r, n);
+    const Pack<T> p = row_pack(x, i, n);
     const Total<W> total{(W)a.totals[2 * r], (W)a.totals[2 * r + 1]};
-    const Slope<W> slope = slope_from_total<T>(a, r, state, total);
-    Pack<T> p;
-    const bool whole = i + V <= n;
-    if (whole) p = load_pack(x + i);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      W g = 0;
-      if (state >= 0 && i + j < n) g = slope.at(Value<T>::widen(whole ? p.v[j] : x[i + j]), i + j);
-      p.v[j] = Value<T>::round(g);
-    }
-    if (i + V <= a.width) {
-      store_pack(out + i, p);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (i + j < a.width) out[i + j] = p.v[j];
-    }
+    const int64_t state = row_state(a, r, n);
+    const Slope<W> slope = slope_from_total(row_weight<T>(a, r), state >= 0, total);
+    store_row_pack(static_cast<T*>(a.gradient) + r * a.gradient_stride, i, a.width,
+                   gradient_pack(slope, p, state - i, n - i));
+    if (packs - q <= step) return;
+    q += step;
   }
 }
 
@@ -306,26 +482,48 @@ using bn::fail;
 
 constexpr int64_t kMaxBlocks = 1 << 20;
 
-template <typename T, int LANES, int PACKS, int MODE>
+template <typename T, int LANES, int PACKS, int KEEP, int MODE>
 void launch_lanes(const Rows& a, hipStream_t s) {
-  const int64_t per_block = 256 / LANES;
+  const int64_t per_block = 256 / LANES * KEEP;
   const int64_t blocks = std::min((a.rows + per_block - 1) / per_block, kMaxBlocks);
-  hipLaunchKernelGGL((rows_in_lanes<T, LANES, PACKS, MODE>), dim3((uint32_t)blocks), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((rows_in_lanes<T, LANES, PACKS, KEEP, MODE>), dim3((uint32_t)blocks), dim3(256), 0, s, a);
+}
+
+template <typename T, int LANES, int PACKS, int MODE>
+void launch_short(const Rows& a, hipStream_t s) {
+  constexpr int kKeep = std::min(LANES, PACKS == 1 ? 8 : PACKS == 2 ? 4 : 2);
+  // several rows per group once that leaves every SIMD (1024) four waves
+  if (kKeep > 1 && a.rows * LANES >= (int64_t)64 * 4096 * kKeep)
+    launch_lanes<T, LANES, PACKS, kKeep, MODE>(a, s);
+  else
+    launch_lanes<T, LANES, PACKS, 1, MODE>(a, s);
+}
+
+template <typename T, int THREADS, int PACKS>
+void launch_block(const Rows& a, hipStream_t s) {
+  // as many blocks as the 256 CUs' registers hold at a time
+  constexpr int64_t kPerCu = PACKS == 16 ? 1 : PACKS == 8 ? 768 / THREADS : 1024 / THREADS;
+  hipLaunchKernelGGL((rows_in_block<T, THREADS, PACKS>), dim3((uint32_t)std::min<int64_t>(a.rows, 256 * kPerCu)),
+                     dim3(THREADS), 0, s, a);
 }
 
 template <typename T, int MODE>
 int launch_forward(const Rows& a, hipStream_t s) {
   constexpr int64_t V = Value<T>::kVec;
   const int64_t packs = (a.width + V - 1) / V;
-  if (packs <= 1) launch_lanes<T, 1, 1, MODE>(a, s);
-  else if (packs <= 2) launch_lanes<T, 2, 1, MODE>(a, s);
-  else if (packs <= 4) launch_lanes<T, 4, 1, MODE>(a, s);
-  else if (packs <= 8) launch_lanes<T, 8, 1, MODE>(a, s);
-  else if (packs <= 16) launch_lanes<T, 16, 1, MODE>(a, s);
-  else if (packs <= 32) launch_lanes<T, 32, 1, MODE>(a, s);
-  else if (packs <= 64) launch_lanes<T, 64, 1, MODE>(a, s);
-  else if (packs <= 128) launch_lanes<T, 64, 2, MODE>(a, s);
-  else if (packs <= 256) launch_lanes<T, 64, 4, MODE>(a, s);
+  if (packs <= 1) launch_short<T, 1, 1, MODE>(a, s);
+  else if (packs <= 2) launch_short<T, 2, 1, MODE>(a, s);
+  else if (packs <= 4) launch_short<T, 4, 1, MODE>(a, s);
+  else if (packs <= 8) launch_short<T, 8, 1, MODE>(a, s);
+  else if (packs <= 16) launch_short<T, 16, 1, MODE>(a, s);
+  else if (packs <= 32) launch_short<T, 32, 1, MODE>(a, s);
+  else if (packs <= 64) launch_short<T, 64, 1, MODE>(a, s);
+  else if (packs <= 128) launch_short<T, 64, 2, MODE>(a, s);
+  else if (packs <= 256) launch_short<T, 64, 4, MODE>(a, s);
+  else if (MODE == kBoth && packs <= 256 * 4) launch_block<T, 256, 4>(a, s);
+  else if (MODE == kBoth && packs <= 256 * 8) launch_block<T, 256, 8>(a, s);
+  else if (MODE == kBoth && packs <= 512 * 8) launch_block<T, 512, 8>(a, s);
+  else if (MODE == kBoth && packs <= 512 * 16) launch_block<T, 512, 16>(a, s);
   else
     hipLaunchKernelGGL((rows_streamed<T, 512, MODE>), dim3((uint32_t)std::min(a.rows, kMaxBlocks)), dim3(512), 0, s, a);
   BN_HIP_CHECK(hipGetLastError());
@@ -335,9 +533,14 @@ int launch_forward(const Rows& a, hipStream_t s) {
 template <typename T>
 int launch_backward(const Rows& a, hipStream_t s) {
   constexpr int64_t V = Value<T>::kVec;
-  const int64_t packs = (a.width + V - 1) / V;
-  const int64_t blocks = std::min((a.rows * packs + kBackwardThreads - 1) / kBackwardThreads, kMaxBlocks);
-  hipLaunchKernelGGL(rows_backward<T>, dim3((uint32_t)blocks), dim3(kBackwardThreads), 0, s, a, packs);
+  const int64_t per_row = (a.width + V - 1) / V, packs = a.rows * per_row;
+  const dim3 grid((uint32_t)std::min((packs + kBackwardThreads - 1) / kBackwardThreads, kMaxBlocks));
+  if (packs < (int64_t)1 << 32)
+    hipLaunchKernelGGL((rows_backward<T, uint32_t>), grid, dim3(kBackwardThreads), 0, s, a, (uint32_t)per_row,
+                       (uint32_t)packs);
+  else
+    hipLaunchKernelGGL((rows_backward<T, uint64_t>), grid, dim3(kBackwardThreads), 0, s, a, (uint64_t)per_row,
+                       (uint64_t)packs);
   BN_HIP_CHECK(hipGetLastError());
   return BN_OK;
 }

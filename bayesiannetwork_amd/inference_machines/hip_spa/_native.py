@@ -237,12 +237,21 @@ DTYPE_CODES = {torch.float32: 0, torch.float64: 1, torch.float16: 2, torch.bfloa
 
 def pointer(tensor):
     """The tensor's device address; None stays a null pointer."""
-    return None if tensor is None else c_void_p(tensor.data_ptr())
+    return None if tensor is None else tensor.data_ptr()
 
 
-def stream_of(device):
-    """The stream torch enqueues on at this moment, as the library takes it."""
-    return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def launch(device: torch.device, entry, *args):
+    """``entry(*args, stream)`` with the device current and on the stream torch enqueues on at this
+    moment.  (The raw stream handle and the skipped device switch are most of a small call's host time.)"""
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
+        rc = entry(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = entry(*args, stream)
+    if rc != 0:
+        check(rc)
 
 
 def i32_array(values):

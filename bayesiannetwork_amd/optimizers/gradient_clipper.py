@@ -80,11 +80,9 @@ class HipGradientClipper:
             self._handle = None
 
     def _call(self, entry, *args) -> torch.Tensor:
-        with torch.cuda.device(self._device):
-            norm = torch.empty((), device=self._device, dtype=torch.float64)
-            workspace = torch.empty((self._workspace_bytes,), device=self._device, dtype=torch.uint8)
-            _native.check(entry(self._handle, *args, _native.pointer(workspace), _native.pointer(norm),
-                                _native.stream_of(self._device)))
+        norm = torch.empty((), device=self._device, dtype=torch.float64)
+        workspace = torch.empty((self._workspace_bytes,), device=self._device, dtype=torch.uint8)
+        _native.launch(self._device, entry, self._handle, *args, workspace.data_ptr(), norm.data_ptr())
         return norm
 
     def norm(self) -> torch.Tensor:
@@ -97,4 +95,4 @@ class HipGradientClipper:
         max_norm = float(max_norm)
         if not 0.0 < max_norm < float("inf"):
             raise ValueError(f"max_norm must be positive and finite, not {max_norm}")
-        return self._call(self._lib.bn_gradient_set_clip, ctypes.c_double(max_norm))
+        return self._call(self._lib.bn_gradient_set_clip, max_norm)

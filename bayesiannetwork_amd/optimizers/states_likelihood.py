@@ -24,26 +24,23 @@ def _ll_dtype(logits: torch.Tensor) -> torch.dtype:
 
 
 def _row_arguments(logits, counts, states):
-    return (_native.DTYPE_CODES[logits.dtype], _native.pointer(logits), logits.shape[0], logits.shape[1],
-            logits.stride(0), _native.pointer(counts), _native.pointer(states), _STATE_BYTES[states.dtype])
+    return (_native.DTYPE_CODES[logits.dtype], logits.data_ptr(), logits.size(0), logits.size(1), logits.stride(0),
+            _native.pointer(counts), states.data_ptr(), _STATE_BYTES[states.dtype])
 
 
 def _forward(logits, states, counts, with_totals):
-    ll = torch.empty((logits.shape[0],), device=logits.device, dtype=_ll_dtype(logits))
-    totals = torch.empty((logits.shape[0], 2), device=logits.device, dtype=torch.float64) if with_totals else None
-    with torch.cuda.device(logits.device):
-        _native.check(_native.load().bn_states_log_likelihood(
-            *_row_arguments(logits, counts, states), _native.pointer(ll), _native.pointer(totals),
-            _native.stream_of(logits.device)))
+    rows, device = logits.size(0), logits.device
+    ll = torch.empty((rows,), device=device, dtype=_ll_dtype(logits))
+    totals = torch.empty((rows, 2), device=device, dtype=torch.float64) if with_totals else None
+    _native.launch(device, _native.load().bn_states_log_likelihood, *_row_arguments(logits, counts, states),
+                   ll.data_ptr(), _native.pointer(totals))
     return ll, totals
 
 
 def _gradient(logits, states, counts, totals, weights, ll, out):
-    with torch.cuda.device(logits.device):
-        _native.check(_native.load().bn_states_log_likelihood_gradient(
-            *_row_arguments(logits, counts, states), _native.pointer(totals), _native.pointer(weights),
-            0 if weights is None else weights.stride(0), _native.pointer(ll), _native.pointer(out), out.stride(0),
-            _native.stream_of(logits.device)))
+    _native.launch(logits.device, _native.load().bn_states_log_likelihood_gradient,
+                   *_row_arguments(logits, counts, states), _native.pointer(totals), _native.pointer(weights),
+                   0 if weights is None else weights.stride(0), _native.pointer(ll), out.data_ptr(), out.stride(0))
 
 
 class _StatesLogLikelihood(torch.autograd.Function):
@@ -97,10 +94,8 @@ def states_log_likelihood_and_gradient(logits: torch.Tensor, states: torch.Tenso
     and type; it may be ``logits`` itself, whose values the gradient then replaces.
     """
     states, counts = _check(logits, states, num_states)
-    logits = logits.detach()
     if weights is not None:
         _rows.check_per_row(weights, logits, (_ll_dtype(logits),), "weights")
-        weights = weights.detach()
     if out is None:
         out = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
     else:

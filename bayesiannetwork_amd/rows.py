@@ -17,11 +17,12 @@ def check_logits(logits: torch.Tensor, name: str = "logits") -> None:
         raise TypeError(f"{name} must be float32, float64, float16 or bfloat16, not {logits.dtype}")
     if logits.dim() != 2:
         raise ValueError(f"{name} must be [rows, states], not of shape {tuple(logits.shape)}")
-    if logits.shape[1] < 1:
+    width = logits.size(1)
+    if width < 1:
         raise ValueError(f"{name} must have at least one state per row")
-    if logits.device.type != "cuda":
+    if not logits.is_cuda:
         raise ValueError(f"{name} must be on an AMD GPU (there is no CPU path)")
-    if logits.shape[1] > 1 and logits.stride(1) != 1:
+    if width > 1 and logits.stride(1) != 1:
         raise ValueError(f"the states of a row of {name} must lie side by side (call .contiguous())")
 
 
@@ -30,8 +31,8 @@ def check_per_row(tensor: torch.Tensor, logits: torch.Tensor, dtypes, name: str)
         raise TypeError(f"{name} must be a tensor")
     if tensor.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, not {tensor.dtype}")
-    if tuple(tensor.shape) != (logits.shape[0],):
-        raise ValueError(f"{name} must have one entry per row: shape {(logits.shape[0],)}, not {tuple(tensor.shape)}")
+    if tensor.dim() != 1 or tensor.size(0) != logits.size(0):
+        raise ValueError(f"{name} must have one entry per row: shape {(logits.size(0),)}, not {tuple(tensor.shape)}")
     if tensor.device != logits.device:
         raise ValueError(f"{name} is on {tensor.device}, the logits are on {logits.device}")
 

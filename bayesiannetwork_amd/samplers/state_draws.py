@@ -68,22 +68,20 @@ def draw_states(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: Se
     if not 0.0 <= filters.min_p <= 1.0:
         raise ValueError(f"min_p must be in [0, 1], not {min_p}")
 
-    logits = logits.detach()
     uniforms = uniforms.contiguous()
     counts = _rows.row_states(num_states, logits)
     lib = _native.load()
+    rows, states = logits.shape
     dtype = _native.DTYPE_CODES[logits.dtype]
-    with torch.cuda.device(logits.device):
-        out = torch.empty((logits.shape[0],), device=logits.device, dtype=torch.int32)
-        if logits.shape[0] == 0:
-            return out
-        need = lib.bn_draw_states_workspace_bytes(dtype, logits.shape[0], logits.shape[1])
-        if need < 0:
-            raise ValueError(f"draw_states takes at most 2^24 states per row, not {logits.shape[1]}")
-        workspace = torch.empty((need,), device=logits.device, dtype=torch.uint8)
-        _native.check(lib.bn_draw_states(
-            dtype, _native.pointer(logits), logits.shape[0], logits.shape[1], logits.stride(0),
-            _native.pointer(counts), _native.DTYPE_CODES[uniforms.dtype], _native.pointer(uniforms),
-            ctypes.byref(filters), _native.pointer(workspace), _native.pointer(out),
-            _native.stream_of(logits.device)))
+    device = logits.device
+    out = torch.empty((rows,), device=device, dtype=torch.int32)
+    if rows == 0:
+        return out
+    need = lib.bn_draw_states_workspace_bytes(dtype, rows, states)
+    if need < 0:
+        raise ValueError(f"draw_states takes at most 2^24 states per row, not {states}")
+    workspace = torch.empty((need,), device=device, dtype=torch.uint8) if need else None
+    _native.launch(device, lib.bn_draw_states, dtype, logits.data_ptr(), rows, states, logits.stride(0),
+                   _native.pointer(counts), _native.DTYPE_CODES[uniforms.dtype], uniforms.data_ptr(),
+                   ctypes.byref(filters), _native.pointer(workspace), out.data_ptr())
     return out

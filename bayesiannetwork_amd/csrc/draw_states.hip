@@ -36,7 +36,7 @@ int check_draws(int dtype, const Draws& a) {
   return BN_OK;
 }
 
-// Workspace of long rows: block sums of all rows, then block keys.
+// Workspace of long rows: block sums, row states and block keys of all rows.
 int64_t blocks_per_row(int64_t num_states) { return num_states <= kShortStates ? 0 : (num_states + kBlock - 1) / kBlock; }
 
 }  // namespace
@@ -46,7 +46,9 @@ extern "C" {
 int64_t bn_draw_states_workspace_bytes(int dtype, int64_t rows, int64_t num_states) {
   if (dtype_bytes(dtype) == 0 || rows < 0 || rows > (int64_t)1 << 40 || num_states < 1 || num_states > kMaxStates) return -1;
   const int64_t key_bytes = dtype == BN_F64 ? 8 : 4;
-  return rows * blocks_per_row(num_states) * (8 + key_bytes);
+  const int64_t blocks = blocks_per_row(num_states);
+  if (blocks == 0) return 0;
+  return rows * ((blocks + 2) * (int64_t)sizeof(double) + (int64_t)sizeof(RowState) + blocks * key_bytes);
 }
 
 int bn_draw_states(int dtype, const void* logits_dev, int64_t rows, int64_t num_states, int64_t row_stride,
@@ -74,8 +76,10 @@ int bn_draw_states(int dtype, const void* logits_dev, int64_t rows, int64_t num_
     return fail(BN_ERR_INVALID, "row address not aligned to its type");
   if (reinterpret_cast<uintptr_t>(workspace_dev) % 8) return fail(BN_ERR_INVALID, "workspace not aligned to 8 bytes");
   if (a.blocks_per_row > 0) {
+    a.sums_per_row = a.blocks_per_row + 2;
     a.block_sums = static_cast<double*>(workspace_dev);
-    a.block_keys = a.block_sums + rows * a.blocks_per_row;
+    a.row_states = reinterpret_cast<RowState*>(a.block_sums + rows * a.sums_per_row);
+    a.block_keys = a.row_states + rows;
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {

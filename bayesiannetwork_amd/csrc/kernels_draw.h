@@ -24,6 +24,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cstdint>
 #include <type_traits>
 
 #include "row_values.h"
@@ -69,6 +70,8 @@ __device__ __forceinline__ KeyType<T> key_at(const T* x, int64_t i) {
 __device__ __forceinline__ bool undrawable(float x) { return !(x < INFINITY); }
 __device__ __forceinline__ bool undrawable(double x) { return !(x < (double)INFINITY); }
 
+struct RowState;
+
 struct Draws {
   const void* logits;
   int64_t rows;
@@ -78,9 +81,12 @@ struct Draws {
   const void* uniforms;
   int32_t uniform_dtype;
   bn_draw_filters filters;
-  void* block_keys;     // [rows][blocks_per_row], long rows
-  double* block_sums;   // [rows][blocks_per_row]
+  // long rows: the workspace
+  double* block_sums;     // [rows][sums_per_row]
+  RowState* row_states;   // [rows]
+  void* block_keys;       // [rows][blocks_per_row]
   int64_t blocks_per_row;
+  int64_t sums_per_row;   // two more: draw_wide's segments, of 128 states at least, take two entries each
   int32_t* out;
 };
 
@@ -121,31 +127,34 @@ __device__ __forceinline__ Setting row_setting(const Draws& a, int64_t r) {
   return s;
 }
 
-// exp((x - best) / T) for x <= best, as 2^t with t = (x - best) log2(e) / T: 2^t = 2^round(t) * 2^f with a
-// polynomial of degree 10 in f (interpolating (2^f - 1) / f at the Chebyshev nodes of [-1/2, 1/2]: 6e-16
-// relative, exactly 1 at f = 0).  17 double instructions, which run beside the loads that feed them; the
-// library's exp took twice that.
+// exp((x - best) / T) for x <= best, as 2^t with t = (x - best) log2(e) / T: 2^t = 2^k * 2^f, k = round(t), with
+// a polynomial of degree 9 in f (interpolating (2^f - 1) / f at the Chebyshev nodes of [-1/2, 1/2]: 4e-14
+// relative, exactly 1 at f = 0).  k comes from adding 1.5 * 2^52, whose sum carries it in its low bits, and goes
+// into an exponent by shifting: 17 instructions of the full double rate, none of the conversions and
+// scalings that take four times as long (256 x 131072 bfloat16: block_summaries 36 -> 20 us with it).
 struct Weight {
   double best;
-  double rate;  // log2(e) / T; a T below 1e-290 acts like one (0 for what is below the maximum)
+  double rate;    // log2(e) / T; T is taken within 1e-290 .. 1e290
+  double lowest;  // x - best from which on the weight is 0: t = -1023, whose exponent field is 0
   __device__ __forceinline__ Weight(double best_, double temperature)
-      : best(best_), rate(1.4426950408889634074 / fmax(temperature, 1e-290)) {}
+      : best(best_), rate(1.4426950408889634074 / fmin(fmax(temperature, 1e-290), 1e290)), lowest(-1023.0 / rate) {}
   __device__ __forceinline__ double operator()(double x) const {
-    const double t = fmax((x - best) * rate, -2200.0);  // 2^-2200 is 0, and -inf stays out of the polynomial
-    const double whole = rint(t);
-    const double f = t - whole;
-    double p = 7.070977866508138e-09;
-    p = fma(p, f, 1.0205905413765595e-07);
-    p = fma(p, f, 1.3215451633221434e-06);
-    p = fma(p, f, 1.5252672924850737e-05);
-    p = fma(p, f, 0.00015403530424776529);
-    p = fma(p, f, 0.0013333558200794592);
-    p = fma(p, f, 0.009618129107618665);
-    p = fma(p, f, 0.05550410866465167);
-    p = fma(p, f, 0.24022650695910075);
-    p = fma(p, f, 0.6931471805599462);
+    constexpr double kShift = 6755399441055744.0;
+    const double d = fmax(x - best, lowest);
+    const double shifted = fma(d, rate, kShift);
+    const double f = fma(d, rate, kShift - shifted);
+    double p = 1.0203121063391729e-07;
+    p = fma(p, f, 1.3255224878668817e-06);
+    p = fma(p, f, 1.525268684626772e-05);
+    p = fma(p, f, 0.00015403455852453838);
+    p = fma(p, f, 0.0013333558179043112);
+    p = fma(p, f, 0.009618129159402558);
+    p = fma(p, f, 0.055504108664760424);
+    p = fma(p, f, 0.2402265069581299);
+    p = fma(p, f, 0.6931471805599453);
     p = fma(p, f, 1.0);
-    return ldexp(p, (int)whole);
+    const uint32_t k = (uint32_t)(uint64_t)__double_as_longlong(shifted);
+    return p * __hiloint2double((int)((k + 1023u) << 20), 0);
   }
   template <typename Key>
   __device__ __forceinline__ double of_key(Key k) const;
@@ -236,12 +245,16 @@ struct Sorted<uint64_t> { using Type = Wide64; };
 
 template <int MASK, int E, bool MIRROR, typename C>
 __device__ __forceinline__ void exchange_lanes(C (&c)[E], bool lower) {
-  C o[E];
+  // no two are equal: the slots differ.  Two at a time, since a mirrored pair reads each other's place.
+  static_assert(!MIRROR || E == 1 || E % 2 == 0, "mirrored in pairs");
 #pragma unroll
-  for (int j = 0; j < E; ++j) o[j] = c[MIRROR ? E - 1 - j : j].template other<MASK>();
-#pragma unroll
-  for (int j = 0; j < E; ++j)
-    if (o[j].above(c[j]) == lower) c[j] = o[j];  // no two are equal: the slots differ
+  for (int j = 0; j < (E + 1) / 2; ++j) {
+    const int k = E - 1 - j;
+    const C at_j = c[MIRROR ? k : j].template other<MASK>();
+    const C at_k = c[MIRROR ? j : k].template other<MASK>();
+    if (at_j.above(c[j]) == lower) c[j] = at_j;
+    if (k != j && at_k.above(c[k]) == lower) c[k] = at_k;
+  }
 }
 
 template <int STRIDE, int E, typename C>
@@ -278,14 +291,14 @@ __device__ __forceinline__ void sort_group(C (&c)[E], int lane) {
 // The draw among states held by a group of lanes, key[j] of slot lane * E + j, 0 where there is none; slots
 // ascend with the states' indices.  `total`: the weight that top-p is a share of, when top-k is off and
 // states outside the group hold some of it; negative: the group's.  Returns the slot, the same in every lane.
-template <int G, int E, typename Key>
+template <bool FILTER, int G, int E, typename Key>
 __device__ int draw_in_group(const Key (&key)[E], const Setting& s, const Weight& weight, double row_total) {
   using C = typename Sorted<Key>::Type;
   const int lane = threadIdx.x % G;
   const bool filtered = s.has_top_k() || s.has_top_p();
   C floor = C::make(0, 0);
   // rows of one wave differ in their settings: the wave sorts if any of them has to
-  if (__any(filtered)) {
+  if (FILTER && __any(filtered)) {
     C c[E];
 #pragma unroll
     for (int j = 0; j < E; ++j) c[j] = C::make(key[j], lane * E + j);
@@ -359,56 +372,55 @@ __device__ __forceinline__ int first_in_group(const Key (&key)[E], Key best) {
 constexpr int kShortThreads = 256;
 
 // Rows of up to G * E states.
-template <typename T, int G, int E>
-__global__ void __launch_bounds__(kShortThreads) draw_short(const Draws a) {
+// FILTER: some row may have a top-k or top-p (without them the sort's registers are not claimed either).
+template <typename T, bool FILTER, int G, int E>
+__global__ void __launch_bounds__(kShortThreads, FILTER ? 4 : 6) draw_short(const Draws a, int64_t first_row) {
   using W = typename Value<T>::Wide;
   using Key = KeyType<T>;
   constexpr int V = Value<T>::kVec;
   constexpr int kRows = kShortThreads / G;
   const int lane = threadIdx.x % G;
-  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < a.rows; r0 += (int64_t)gridDim.x * kRows) {
-    const int64_t r = r0 + threadIdx.x / G;
-    if (r >= a.rows) continue;  // whole groups leave together
-    const T* x = static_cast<const T*>(a.logits) + r * a.stride;
-    const Setting s = row_setting(a, r);
-    const int n = (int)s.n, first = lane * E;
-    Key key[E];
-    bool bad = false;
-    Key best = 0;
-    const auto take = [&](int j, T v) {
-      const W wide = Value<T>::widen(v);
-      bad |= undrawable(wide);
-      key[j] = KeyOf<W>::key(wide);
-      best = best > key[j] ? best : key[j];
-    };
-    if (E >= V && first + E <= n) {
+  const int64_t r = first_row + (int64_t)blockIdx.x * kRows + threadIdx.x / G;
+  if (r >= a.rows) return;  // whole groups leave together
+  const T* x = static_cast<const T*>(a.logits) + r * a.stride;
+  const Setting s = row_setting(a, r);
+  const int n = (int)s.n, first = lane * E;
+  Key key[E];
+  bool bad = false;
+  Key best = 0;
+  const auto take = [&](int j, T v) {
+    const W wide = Value<T>::widen(v);
+    bad |= undrawable(wide);
+    key[j] = KeyOf<W>::key(wide);
+    best = best > key[j] ? best : key[j];
+  };
+  if (E >= V && first + E <= n) {
 #pragma unroll
-      for (int k = 0; k + V <= E; k += V) {
-        const Pack<T> p = load_pack(x + first + k);
+    for (int k = 0; k + V <= E; k += V) {
+      const Pack<T> p = load_pack(x + first + k);
 #pragma unroll
-        for (int j = 0; j < V; ++j) take(k + j, p.v[j]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        key[j] = 0;
-        if (first + j < n) take(j, x[first + j]);
-      }
+      for (int j = 0; j < V; ++j) take(k + j, p.v[j]);
     }
+  } else {
 #pragma unroll
-    for (int d = 1; d < G; d <<= 1) {
-      const Key o = (Key)__shfl_xor((typename std::conditional<sizeof(Key) == 8, unsigned long long, unsigned>::type)best, d, 64);
-      best = best > o ? best : o;
+    for (int j = 0; j < E; ++j) {
+      key[j] = 0;
+      if (first + j < n) take(j, x[first + j]);
     }
-    bad = group_all<G>((int)bad, [](int p, int q) { return p | q; }) != 0;
-    const double largest = (double)KeyOf<W>::value(best);
-    const bool valid = s.valid && !bad && !isinf(largest);
-    const bool greedy = s.temperature == 0.0;
-    const Weight weight(valid ? largest : 0.0, greedy ? 1.0 : s.temperature);
-    int pick = draw_in_group<G, E>(key, s, weight, -1.0);
-    if (greedy) pick = first_in_group<G, E>(key, best);
-    if (lane == 0) a.out[r] = valid ? pick : -1;
   }
+#pragma unroll
+  for (int d = 1; d < G; d <<= 1) {
+    const Key o = (Key)__shfl_xor((typename std::conditional<sizeof(Key) == 8, unsigned long long, unsigned>::type)best, d, 64);
+    best = best > o ? best : o;
+  }
+  bad = group_all<G>((int)bad, [](int p, int q) { return p | q; }) != 0;
+  const double largest = (double)KeyOf<W>::value(best);
+  const bool valid = s.valid && !bad && !isinf(largest);
+  const bool greedy = s.temperature == 0.0;
+  const Weight weight(valid ? largest : 0.0, greedy ? 1.0 : s.temperature);
+  int pick = draw_in_group<FILTER, G, E>(key, s, weight, -1.0);
+  if (greedy) pick = first_in_group<G, E>(key, best);
+  if (lane == 0) a.out[r] = valid ? pick : -1;
 }
 
 // ---- long rows: summaries of 64 states -----------------------------------------------------------
@@ -474,7 +486,7 @@ __global__ void __launch_bounds__(kSummaryThreads) block_summaries(const Draws a
       if (lane % kLanes == 0 && i < n) {
         // the largest key there is marks a block that makes its row undrawable
         keys[i / kBlock] = bad ? (Key)~(Key)0 : KeyOf<W>::key(best);
-        if (sums) a.block_sums[r * a.blocks_per_row + i / kBlock] = sum;
+        if (sums) a.block_sums[r * a.sums_per_row + i / kBlock] = sum;
       }
     }
   }
@@ -482,18 +494,22 @@ __global__ void __launch_bounds__(kSummaryThreads) block_summaries(const Draws a
 
 // ---- long rows: the draw ----------------------------------------------------------------------------
 
-constexpr int kCandidates = 1024;  // states that one wave draws among
-constexpr int kListed = 512;       // blocks they may come from
+// What draw_long found out about a row that draw_wide has to finish.
+struct RowState {
+  unsigned long long best, floor;  // keys: the largest, and one below which nothing is kept
+  double total;                    // weight of the whole row, where top-k is off
+  long long pending;               // 0: the row is drawn
+};
 
-template <typename Key, int THREADS>
-struct Shared {
+constexpr int kCandidates = 512;  // states that one wave draws among
+constexpr int kListed = 512;      // blocks they may come from
+constexpr int kLongThreads = 256;
+
+template <int THREADS>
+struct Bins {
   static constexpr int kBins = 4 * THREADS;
   unsigned long long mass[kBins];
   uint32_t count[kBins];
-  Key candidate[kCandidates];
-  int32_t candidate_index[kCandidates];
-  int32_t listed[kListed];
-  double sums[THREADS / 64];
   unsigned long long words[THREADS / 64];
   long long answer[4];
 };
@@ -513,7 +529,6 @@ __device__ __forceinline__ U block_all(U v, unsigned long long* lds, Combine com
 }
 constexpr auto kMax = [](unsigned long long p, unsigned long long q) { return p > q ? p : q; };
 constexpr auto kMin = [](unsigned long long p, unsigned long long q) { return p < q ? p : q; };
-constexpr auto kSum = [](unsigned long long p, unsigned long long q) { return p + q; };
 
 // Exclusive prefix sum of one value per thread, and the block's total.
 template <int THREADS, typename U>
@@ -541,30 +556,14 @@ __device__ __forceinline__ U block_scan(U v, unsigned long long* lds, U* total) 
   return base + before;
 }
 
-// Calls fn(index, key) for all n states of a row in memory.
-template <typename T, int THREADS, typename Fn>
-__device__ __forceinline__ void for_each_state(const T* x, int64_t n, Fn fn) {
-  using W = typename Value<T>::Wide;
-  constexpr int V = Value<T>::kVec;
-  const int64_t packs = n / V;
-#pragma unroll 2
-  for (int64_t k = threadIdx.x; k < packs; k += THREADS) {
-    const Pack<T> p = load_pack(x + k * V);
-#pragma unroll
-    for (int j = 0; j < V; ++j) fn(k * V + j, KeyOf<W>::key(Value<T>::widen(p.v[j])));
-  }
-  const int64_t i = packs * V + threadIdx.x;
-  if (i < n) fn(i, KeyOf<W>::key(Value<T>::widen(x[i])));
+// A weight as an integer: times a power of two that lets n of them add up within 62 bits and one be rounded
+// by adding 2^52.
+__device__ __forceinline__ double mass_scale(int n) {
+  const int room = 62 - (32 - __clz(n));
+  return ldexp(1.0, room < 50 ? room : 50);
 }
-
-// A weight as an integer: times 2^scale_bits, which lets n of them add up within 62 bits and one be
-// rounded by adding 2^52.
-__device__ __forceinline__ int mass_bits(int64_t n) {
-  const int room = 62 - (64 - __clzll((unsigned long long)n));
-  return room < 50 ? room : 50;
-}
-__device__ __forceinline__ unsigned long long mass_of(double w, int bits) {
-  const double shifted = ldexp(w, bits) + 4503599627370496.0;
+__device__ __forceinline__ unsigned long long mass_of(double w, double scale) {
+  const double shifted = w * scale + 4503599627370496.0;
   return (unsigned long long)__double_as_longlong(shifted) & 0xFFFFFFFFFFFFFull;
 }
 
@@ -576,33 +575,41 @@ struct Bin {
   bool reached;               // the target is reached in it or above; else it is the lowest that holds a state
 };
 
+// How keys of [low, high] fall into the bins.
+template <int THREADS, typename Key>
+__device__ __forceinline__ int bin_shift(Key low, Key high) {
+  constexpr int kLog = THREADS == 1024 ? 12 : THREADS == 512 ? 11 : 10;
+  static_assert((1 << kLog) == Bins<THREADS>::kBins, "four bins per thread");
+  const Key range = high - low;
+  const int bits = sizeof(Key) == 8 ? 64 - __clzll((long long)range) : 32 - __clz((int)(uint32_t)range);
+  return bits > kLog ? bits - kLog : 0;
+}
+template <typename Key>
+__device__ __forceinline__ Key bin_high(Key bin_low, int shift, Key high) {
+  const Key top = bin_low + (((Key)1 << shift) - 1);
+  return top > high || top < bin_low ? high : top;
+}
+
 // The bin of keys in [low, high] in which the count (BY_MASS: the mass) from the top, `above` included,
 // reaches `target`.  each(fn) calls fn(key) for every key there is; keys outside the range are passed over.
-// States on `floor` (nothing lies below it) have mass floor_mass together.
 template <bool BY_MASS, int THREADS, typename Key, typename Each, typename Mass>
-__device__ Bin<Key> find_bin(Shared<Key, THREADS>& lds, Each each, Mass mass, Key low, Key high,
-                             unsigned long long above, double target, Key floor, unsigned long long floor_mass) {
-  constexpr int kBins = Shared<Key, THREADS>::kBins;
-  constexpr int kLog = THREADS == 1024 ? 12 : THREADS == 512 ? 11 : 10;
-  static_assert((1 << kLog) == kBins, "four bins per thread");
-  const Key range = high - low;
-  const int bits = range == 0 ? 0 : (sizeof(Key) == 8 ? 64 - __clzll((unsigned long long)range) : 32 - __clz((int)(uint32_t)range));
-  const int shift = bits > kLog ? bits - kLog : 0;
+__device__ Bin<Key> find_bin(Bins<THREADS>& lds, Each each, Mass mass, Key low, Key high, unsigned long long above,
+                             double target) {
+  constexpr int kBins = Bins<THREADS>::kBins;
+  const int shift = bin_shift<THREADS>(low, high);
   __syncthreads();
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
     lds.count[b * THREADS + threadIdx.x] = 0;
-    lds.mass[b * THREADS + threadIdx.x] = 0;
+    if (BY_MASS) lds.mass[b * THREADS + threadIdx.x] = 0;
   }
   __syncthreads();
   each([&](Key k) {
     if (k < low || k > high) return;
     const int bin = (int)((k - low) >> shift);
     atomicAdd(&lds.count[bin], 1u);
-    if (BY_MASS && k != floor) atomicAdd(&lds.mass[bin], mass(k));
+    if (BY_MASS) atomicAdd(&lds.mass[bin], mass(k));
   });
-  __syncthreads();
-  if (BY_MASS && threadIdx.x == 0 && floor >= low && floor <= high) lds.mass[(int)((floor - low) >> shift)] += floor_mass;
   __syncthreads();
   // thread t holds bins kBins - 1 - 4 t downwards
   unsigned long long own[4], sum = 0, total;
@@ -613,33 +620,40 @@ __device__ Bin<Key> find_bin(Shared<Key, THREADS>& lds, Each each, Mass mass, Ke
     sum += own[b];
   }
   unsigned long long before = above + block_scan<THREADS>(sum, lds.words, &total);
-  unsigned long long found = ~0ull, lowest = 0, found_above = 0, lowest_above = 0;
+  // the first bin that reaches the target in the high word, the last one that holds a state (counted from the
+  // other end) in the low one
+  unsigned int found = ~0u, lowest = ~0u;
+  unsigned long long found_above = 0, lowest_above = 0;
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
-    const int at = 4 * (int)threadIdx.x + b;
+    const unsigned int at = 4 * threadIdx.x + b;
     if (lds.count[kBins - 1 - at] != 0) {
-      if (found == ~0ull && (double)(before + own[b]) >= target) {
-        found = (unsigned long long)at;
+      if (found == ~0u && (double)(before + own[b]) >= target) {
+        found = at;
         found_above = before;
       }
-      lowest = (unsigned long long)at + 1;
+      lowest = kBins - 1 - at;
       lowest_above = before;
     }
     before += own[b];
   }
-  const unsigned long long first = block_all<THREADS>(found, lds.words, kMin);
-  const unsigned long long last = block_all<THREADS>(lowest, lds.words, kMax);
-  const unsigned long long at = first != ~0ull ? first : last - 1;
-  if (threadIdx.x == (unsigned)(at / 4)) lds.answer[0] = (long long)(first != ~0ull ? found_above : lowest_above);
+  const unsigned long long both = block_all<THREADS>(((unsigned long long)found << 32) | lowest, lds.words,
+                                                     [](unsigned long long p, unsigned long long q) {
+                                                       const unsigned long long hi = (p >> 32) < (q >> 32) ? p >> 32 : q >> 32;
+                                                       const uint32_t lo = std::min((uint32_t)p, (uint32_t)q);
+                                                       return (hi << 32) | lo;
+                                                     });
+  const bool reached = (uint32_t)(both >> 32) != ~0u;
+  const int at = reached ? (int)(both >> 32) : kBins - 1 - (int)(uint32_t)both;
+  if (threadIdx.x == (unsigned)(at / 4)) lds.answer[0] = (long long)(reached ? found_above : lowest_above);
   __syncthreads();
-  const int bin = kBins - 1 - (int)at;
+  const int bin = kBins - 1 - at;
   Bin<Key> out;
   out.low = low + ((Key)bin << shift);
-  const Key top = out.low + (((Key)1 << shift) - 1);
-  out.high = top > high || top < out.low ? high : top;
+  out.high = bin_high(out.low, shift, high);
   out.above = (unsigned long long)lds.answer[0];
   out.states = lds.count[bin];
-  out.reached = first != ~0ull;
+  out.reached = reached;
   return out;
 }
 
@@ -647,47 +661,48 @@ __device__ Bin<Key> find_bin(Shared<Key, THREADS>& lds, Each each, Mass mass, Ke
 // 64 * PER states of one segment by one wave.  sum_of(segment) is the segment's weight, weight_at(index) a
 // state's (0: not kept).
 template <int THREADS, int PER, typename Lds, typename SumOf, typename WeightAt>
-__device__ int64_t locate(Lds& lds, int64_t segments, double uniform, SumOf sum_of, WeightAt weight_at) {
-  const int64_t each = (segments + THREADS - 1) / THREADS;
-  const int64_t begin = std::min<int64_t>((int64_t)threadIdx.x * each, segments);
-  const int64_t end = std::min<int64_t>(begin + each, segments);
+__device__ int locate(Lds& lds, int segments, double uniform, SumOf sum_of, WeightAt weight_at) {
+  const int each = (segments + THREADS - 1) / THREADS;
+  const int begin = std::min((int)threadIdx.x * each, segments);
+  const int end = std::min(begin + each, segments);
   double here = 0.0, total;
-  int64_t last_filled = -1;
-  for (int64_t q = begin; q < end; ++q) {
+  int last_filled = -1;
+  for (int q = begin; q < end; ++q) {
     const double s = sum_of(q);
     here += s;
     if (s > 0.0) last_filled = q;
   }
   const double left = block_scan<THREADS>(here, lds.words, &total);
   const double target = uniform * total;
-  // u = 1, or the sums' rounding: the last segment that holds anything
-  const bool mine = here > 0.0 && left + here > target;
-  unsigned long long owner = block_all<THREADS>(mine ? (unsigned long long)threadIdx.x : ~0ull, lds.words, kMin);
-  const bool none = owner == ~0ull;
-  if (none) owner = block_all<THREADS>(here > 0.0 ? (unsigned long long)threadIdx.x + 1 : 0ull, lds.words, kMax) - 1;
-  if (threadIdx.x == (unsigned)owner) {
-    double upto = left;
-    int64_t segment = last_filled;
+  // the first thread whose segments exceed the target; u = 1, or the sums' rounding: the last that holds anything
+  const uint32_t over = here > 0.0 && left + here > target ? threadIdx.x : ~0u;
+  const uint32_t filled = here > 0.0 ? THREADS - 1 - threadIdx.x : ~0u;
+  const unsigned long long both = block_all<THREADS>(((unsigned long long)over << 32) | filled, lds.words,
+                                                     [](unsigned long long p, unsigned long long q) {
+                                                       const unsigned long long hi = (p >> 32) < (q >> 32) ? p >> 32 : q >> 32;
+                                                       const uint32_t lo = std::min((uint32_t)p, (uint32_t)q);
+                                                       return (hi << 32) | lo;
+                                                     });
+  const bool none = (uint32_t)(both >> 32) == ~0u;
+  const uint32_t owner = none ? THREADS - 1 - (uint32_t)both : (uint32_t)(both >> 32);
+  if (threadIdx.x == owner) {
     double before = left;
-    for (int64_t q = begin; q < end; ++q) {
-      const double s = sum_of(q);
-      if (s > 0.0 && (q == last_filled || (!none && upto + s > target))) {
-        segment = q;
-        before = upto;
-        break;
-      }
-      upto += s;
+    int segment = begin;
+    for (; segment < last_filled; ++segment) {
+      const double s = sum_of(segment);
+      if (!none && before + s > target) break;
+      before += s;
     }
     lds.answer[1] = segment;
     lds.answer[2] = __double_as_longlong(before);
   }
   __syncthreads();
-  const int64_t start = lds.answer[1] * (64 * PER);
+  const int start = (int)lds.answer[1] * (64 * PER);
   if (threadIdx.x < 64) {
     double w[PER], sum = 0.0, all;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      w[j] = weight_at(start + (int64_t)threadIdx.x * PER + j);
+      w[j] = weight_at(start + (int)threadIdx.x * PER + j);
       sum += w[j];
     }
     double upto = __longlong_as_double(lds.answer[2]) + group_scan<64>(sum, &all);
@@ -705,40 +720,46 @@ __device__ int64_t locate(Lds& lds, int64_t segments, double uniform, SumOf sum_
     if (threadIdx.x == 0) lds.answer[3] = start + (pick == INT32_MAX ? last : pick);
   }
   __syncthreads();
-  return lds.answer[3];
+  return (int)lds.answer[3];
 }
 
-template <int E, typename Key, int THREADS>
-__device__ __forceinline__ int draw_among_candidates(const Shared<Key, THREADS>& lds, int count, const Setting& s,
-                                                     const Weight& weight, double row_total) {
+template <typename Key>
+struct Candidates {
+  Key key[kCandidates];
+  int32_t index[kCandidates];
+  int32_t listed[kListed];
+};
+
+template <int E, typename Key>
+__device__ __forceinline__ int draw_among(const Candidates<Key>& from, int count, const Setting& s, const Weight& weight,
+                                          double row_total) {
   Key key[E];
 #pragma unroll
   for (int j = 0; j < E; ++j) {
     const int at = (int)(threadIdx.x & 63) * E + j;
-    key[j] = at < count ? lds.candidate[at] : (Key)0;
+    key[j] = at < count ? from.key[at] : (Key)0;
   }
-  return draw_in_group<64, E>(key, s, weight, row_total);
+  return draw_in_group<true, 64, E>(key, s, weight, row_total);
 }
 
-// One row, by the whole block; the same answer in every thread.
-template <typename T, int THREADS>
-__device__ int64_t draw_row(const Draws& a, int64_t r, Shared<KeyType<T>, THREADS>& lds) {
+// One row, by the whole block, from its summaries; the same answer in every thread: the state, -1, or -2 for
+// a row that is left to draw_wide, with what it needs in `state`.
+template <typename T>
+__device__ int draw_row(const Draws& a, int64_t r, Bins<kLongThreads>& lds, Candidates<KeyType<T>>& from, RowState& state) {
   using W = typename Value<T>::Wide;
   using Key = KeyType<T>;
-  constexpr int V = Value<T>::kVec;
+  constexpr int THREADS = kLongThreads;
   const T* x = static_cast<const T*>(a.logits) + r * a.stride;
-  Setting s = row_setting(a, r);
+  const Setting s = row_setting(a, r);
   if (!s.valid) return -1;
-  const int64_t n = s.n;
-  const int64_t blocks = (n + kBlock - 1) / kBlock;
+  const int n = (int)s.n;
+  const int blocks = (n + kBlock - 1) / kBlock;
   const Key* keys = static_cast<const Key*>(a.block_keys) + r * a.blocks_per_row;
-  double* sums = a.block_sums + r * a.blocks_per_row;
+  const double* sums = a.block_sums + r * a.sums_per_row;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 
-  unsigned long long best = 0, least = ~0ull;
-  for (int64_t b = threadIdx.x; b < blocks; b += THREADS) {
-    best = kMax(best, (unsigned long long)keys[b]);
-    least = kMin(least, (unsigned long long)keys[b]);
-  }
+  unsigned long long best = 0;
+  for (int b = threadIdx.x; b < blocks; b += THREADS) best = kMax(best, (unsigned long long)keys[b]);
   best = block_all<THREADS>(best, lds.words, kMax);
   if ((Key)best == (Key)~(Key)0) return -1;
   const double largest = (double)KeyOf<W>::value((Key)best);
@@ -746,28 +767,30 @@ __device__ int64_t draw_row(const Draws& a, int64_t r, Shared<KeyType<T>, THREAD
 
   if (s.temperature == 0.0) {
     unsigned long long block = ~0ull;
-    for (int64_t b = threadIdx.x; b < blocks && block == ~0ull; b += THREADS)
+    for (int b = threadIdx.x; b < blocks && block == ~0ull; b += THREADS)
       if ((unsigned long long)keys[b] == best) block = (unsigned long long)b;
     block = block_all<THREADS>(block, lds.words, kMin);
-    const int64_t i = (int64_t)block * kBlock + (threadIdx.x & 63);
+    const int i = (int)block * kBlock + lane;
     const uint64_t hits = __ballot(i < n && key_at(x, std::min(i, n - 1)) == (Key)best);
-    return (int64_t)block * kBlock + __ffsll((unsigned long long)hits) - 1;
+    return (int)block * kBlock + __ffsll((unsigned long long)hits) - 1;
   }
 
   const Weight weight(largest, s.temperature);
-  const auto block_sum_of = [&](int64_t b) { return sums[b] * weight.of_key(keys[b]); };
+  const auto block_sum_of = [&](int b) { return sums[b] * weight.of_key(keys[b]); };
   if (!s.has_top_k() && !s.has_top_p() && s.min_p == 0.0)
-    return locate<THREADS, 1>(lds, blocks, s.uniform, block_sum_of, [&](int64_t i) {
+    return locate<THREADS, 1>(lds, blocks, s.uniform, block_sum_of, [&](int i) {
       return i < n ? weight.of_key(key_at(x, std::min(i, n - 1))) : 0.0;
     });
 
   // ---- a floor below which nothing is kept
-  least = block_all<THREADS>(least, lds.words, kMin);
-  const int bits = mass_bits(n);
-  const auto mass = [&](Key k) { return mass_of(weight.of_key(k), bits); };
+  const double scale = mass_scale(n);
+  const auto mass = [&](Key k) { return mass_of(weight.of_key(k), scale); };
   const auto each_block = [&](auto fn) {
-    for (int64_t b = threadIdx.x; b < blocks; b += THREADS) fn(keys[b]);
+    for (int b = threadIdx.x; b < blocks; b += THREADS) fn(keys[b]);
   };
+  unsigned long long least = ~0ull;
+  for (int b = threadIdx.x; b < blocks; b += THREADS) least = kMin(least, (unsigned long long)keys[b]);
+  least = block_all<THREADS>(least, lds.words, kMin);
   Key floor = 1;
   const auto raise_floor = [&](double least_weight) {  // only states of at least this weight are kept
     const double step = s.temperature * log(least_weight);
@@ -779,194 +802,390 @@ __device__ int64_t draw_row(const Draws& a, int64_t r, Shared<KeyType<T>, THREAD
   if (s.has_top_k()) {
     // the largest keys of k blocks are k states: the k-th state's key is not below the k-th of them
     if (s.top_k < blocks)
-      floor = find_bin<false>(lds, each_block, mass, (Key)least, (Key)best, 0ull, (double)s.top_k, (Key)0, 0ull).low;
+      floor = find_bin<false>(lds, each_block, mass, (Key)least, (Key)best, 0ull, (double)s.top_k).low;
   } else if (s.has_top_p()) {
     double here = 0.0;
-    const int64_t each = (blocks + THREADS - 1) / THREADS;
-    for (int64_t b = (int64_t)threadIdx.x * each; b < std::min<int64_t>((int64_t)(threadIdx.x + 1) * each, blocks); ++b)
-      here += block_sum_of(b);
+    const int each = (blocks + THREADS - 1) / THREADS;
+    for (int b = (int)threadIdx.x * each; b < std::min((int)(threadIdx.x + 1) * each, blocks); ++b) here += block_sum_of(b);
     (void)block_scan<THREADS>(here, lds.words, &row_total);
     // the states below (1 - p) W / n hold less than the share that is left out
-    const double lowest = largest + s.temperature * log(fmax((1.0 - s.top_p) * row_total / (double)n, 1e-300)) -
-                          1e-6 * (fabs(largest) + 1.0);
-    const W bound = (W)fmax(lowest, -(double)INFINITY);
-    if (bound < (W)largest && !isinf(bound)) floor = std::max(floor, KeyOf<W>::key(bound));
-    // and blocks' largest states that hold the share by themselves do too
-    const Bin<Key> bin = find_bin<true>(lds, each_block, mass, (Key)least, (Key)best, 0ull,
-                                        s.top_p * ldexp(row_total, bits) * (1.0 + 1e-9), (Key)0, 0ull);
+    raise_floor((1.0 - s.top_p) * row_total / (double)n);
+    // and where blocks' largest states hold the share by themselves, nothing below those is kept
+    const Bin<Key> bin = find_bin<true>(lds, each_block, mass, std::max(floor, (Key)least), (Key)best, 0ull,
+                                        s.top_p * row_total * scale * (1.0 + 1e-9));
     if (bin.reached) floor = std::max(floor, bin.low);
   }
   // (with top-k and top-p together W is the weight of all top-k states, those that min-p drops among them)
   if (s.min_p > 0.0 && !(s.has_top_k() && s.has_top_p())) raise_floor(s.min_p);
 
   // ---- few states at or above it: one wave draws among them
-  {
-    const int64_t each = (blocks + THREADS - 1) / THREADS;
-    const int64_t begin = std::min<int64_t>((int64_t)threadIdx.x * each, blocks), end = std::min<int64_t>(begin + each, blocks);
-    unsigned long long passing = 0, listed;
-    for (int64_t b = begin; b < end; ++b) passing += keys[b] >= floor;
-    unsigned long long at = block_scan<THREADS>(passing, lds.words, &listed);
-    if (listed <= kListed) {
-      for (int64_t b = begin; b < end; ++b)
-        if (keys[b] >= floor) lds.listed[at++] = (int32_t)b;
-      __syncthreads();
-      // counts per listed block, their prefix sums, then the states in order of their index
-      const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-      for (int q = wave; q < (int)listed; q += THREADS / 64) {
-        const int64_t i = (int64_t)lds.listed[q] * kBlock + lane;
-        const uint64_t hits = __ballot(i < n && key_at(x, std::min(i, n - 1)) >= floor);
-        if (lane == 0) lds.count[q] = (uint32_t)__popcll(hits);
-      }
-      __syncthreads();
-      unsigned long long mine = 0, candidates;
-      constexpr int kPer = (kListed + THREADS - 1) / THREADS;
+  const int each = (blocks + THREADS - 1) / THREADS;
+  const int begin = std::min((int)threadIdx.x * each, blocks), end = std::min(begin + each, blocks);
+  unsigned long long passing = 0, listed;
+  for (int b = begin; b < end; ++b) passing += keys[b] >= floor;
+  unsigned long long at = block_scan<THREADS>(passing, lds.words, &listed);
+  if (listed <= kListed) {
+    for (int b = begin; b < end; ++b)
+      if (keys[b] >= floor) from.listed[at++] = b;
+    __syncthreads();
+    // counts per listed block, their prefix sums, then the states in order of their index
+    for (int q = wave; q < (int)listed; q += THREADS / 64) {
+      const int i = from.listed[q] * kBlock + lane;
+      const uint64_t hits = __ballot(i < n && key_at(x, std::min(i, n - 1)) >= floor);
+      if (lane == 0) lds.count[q] = (uint32_t)__popcll(hits);
+    }
+    __syncthreads();
+    constexpr int kPer = kListed / THREADS;
+    unsigned long long mine = 0, candidates;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int q = (int)threadIdx.x * kPer + j;
+      if (q < (int)listed) mine += lds.count[q];
+    }
+    unsigned long long before = block_scan<THREADS>(mine, lds.words, &candidates);
+    if (candidates <= kCandidates) {
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         const int q = (int)threadIdx.x * kPer + j;
-        if (q < (int)listed) mine += lds.count[q];
+        if (q < (int)listed) {
+          const uint32_t c = lds.count[q];
+          lds.count[q] = (uint32_t)before;
+          before += c;
+        }
       }
-      unsigned long long before = block_scan<THREADS>(mine, lds.words, &candidates);
-      if (candidates <= kCandidates) {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const int q = (int)threadIdx.x * kPer + j;
-          if (q < (int)listed) {
-            const uint32_t c = lds.count[q];
-            lds.count[q] = (uint32_t)before;
-            before += c;
-          }
+      __syncthreads();
+      for (int q = wave; q < (int)listed; q += THREADS / 64) {
+        const int i = from.listed[q] * kBlock + lane;
+        const Key k = key_at(x, std::min(i, n - 1));
+        const bool hit = i < n && k >= floor;
+        const uint64_t hits = __ballot(hit);
+        if (hit) {
+          const int to = (int)lds.count[q] + __popcll(hits & ((1ull << lane) - 1));
+          from.key[to] = k;
+          from.index[to] = i;
         }
-        __syncthreads();
-        for (int q = wave; q < (int)listed; q += THREADS / 64) {
-          const int64_t i = (int64_t)lds.listed[q] * kBlock + lane;
-          const Key k = key_at(x, std::min(i, n - 1));
-          const bool hit = i < n && k >= floor;
-          const uint64_t hits = __ballot(hit);
-          if (hit) {
-            const int to = (int)lds.count[q] + __popcll(hits & ((1ull << lane) - 1));
-            lds.candidate[to] = k;
-            lds.candidate_index[to] = (int32_t)i;
-          }
-        }
-        __syncthreads();
-        if (threadIdx.x < 64) {
-          const int count = (int)candidates;
-          int slot;
-          if (count <= 64)
-            slot = draw_among_candidates<1>(lds, count, s, weight, row_total);
-          else if (count <= 256)
-            slot = draw_among_candidates<4>(lds, count, s, weight, row_total);
-          else
-            slot = draw_among_candidates<16>(lds, count, s, weight, row_total);
-          if (threadIdx.x == 0) lds.answer[3] = lds.candidate_index[slot];
-        }
-        __syncthreads();
-        return lds.answer[3];
       }
+      __syncthreads();
+      if (wave == 0) {
+        const int count = (int)candidates;
+        int slot;
+        if (count <= 64)
+          slot = draw_among<1>(from, count, s, weight, row_total);
+        else if (count <= 256)
+          slot = draw_among<4>(from, count, s, weight, row_total);
+        else
+          slot = draw_among<8>(from, count, s, weight, row_total);
+        if (lane == 0) lds.answer[3] = from.index[slot];
+      }
+      __syncthreads();
+      return (int)lds.answer[3];
     }
+  }
+  state = {best, (unsigned long long)floor, row_total, 1};
+  return -2;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLongThreads, 4) draw_long(const Draws a, int64_t first_row) {
+  __shared__ Bins<kLongThreads> lds;
+  __shared__ Candidates<KeyType<T>> from;
+  const int64_t r = first_row + blockIdx.x;
+  RowState state{};
+  const int drawn = draw_row<T>(a, r, lds, from, state);
+  if (threadIdx.x == 0) {
+    if (drawn >= -1) a.out[r] = drawn;
+    a.row_states[r] = state;
+  }
+}
+
+// ---- long rows that keep many states ----------------------------------------------------------------
+
+// Calls fn(index, key) for all n states of a row in memory.
+template <typename T, int THREADS, typename Fn>
+__device__ __forceinline__ void for_each_state(const T* x, int n, Fn fn) {
+  using W = typename Value<T>::Wide;
+  constexpr int V = Value<T>::kVec;
+  const int packs = n / V;
+#pragma unroll 2
+  for (int k = threadIdx.x; k < packs; k += THREADS) {
+    const Pack<T> p = load_pack(x + k * V);
+#pragma unroll
+    for (int j = 0; j < V; ++j) fn(k * V + j, KeyOf<W>::key(Value<T>::widen(p.v[j])));
+  }
+  const int i = packs * V + (int)threadIdx.x;
+  if (i < n) fn(i, KeyOf<W>::key(Value<T>::widen(x[i])));
+}
+
+template <typename Key, int THREADS>
+struct Listed {
+  static constexpr int kRoom = 4 * THREADS;
+  Key key[kRoom];
+  int32_t index[kRoom];
+  uint32_t count;
+};
+
+// The states of a prefix of the order: keys above `key`, and those on it up to an index.
+template <typename Key>
+struct Prefix {
+  Key key;
+  int last;
+  __device__ __forceinline__ bool has(int i, Key k) const { return k > key || (k == key && i <= last); }
+};
+
+// The index of the `kept`-th state, in ascending index, on a key; all of them are in the list if `in_list`.
+template <typename T, int THREADS>
+__device__ int last_kept(const T* x, int n, KeyType<T> key, unsigned long long kept, Bins<THREADS>& lds,
+                         const Listed<KeyType<T>, THREADS>& list, bool in_list) {
+  constexpr int V = Value<T>::kVec;
+  if (in_list) {
+    const uint32_t count = list.count;
+    const auto each = [&](auto fn) {
+      for (uint32_t q = threadIdx.x; q < count; q += THREADS)
+        if (list.key[q] == key) fn(~(uint32_t)list.index[q]);
+    };
+    Bin<uint32_t> bin{~(uint32_t)n, ~0u, 0ull, 0ull, true};
+    do {
+      bin = find_bin<false>(lds, each, [](uint32_t) { return 0ull; }, bin.low, bin.high, bin.above, (double)kept);
+    } while (bin.low != bin.high);
+    return (int)~bin.low;
+  }
+  unsigned long long seen = 0;
+  for (int base = 0; base < n && seen < kept; base += THREADS * V) {
+    const int i = base + (int)threadIdx.x * V;
+    unsigned long long mine = 0, all;
+    uint32_t on = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (i + j < n && key_at(x, i + j) == key) {
+        on |= 1u << j;
+        ++mine;
+      }
+    unsigned long long before = seen + block_scan<THREADS>(mine, lds.words, &all);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (on >> j & 1) {
+        if (++before == kept) lds.answer[0] = i + j;
+      }
+    seen += all;
+  }
+  __syncthreads();
+  return (int)lds.answer[0];
+}
+
+// One row by the whole block, over the row in memory: one pass counts its states by key, a second one adds up
+// what is certainly kept, and the few thousand states around the threshold are settled in LDS.
+template <typename T, int THREADS>
+__device__ int draw_wide_row(const Draws& a, int64_t r, const RowState& state, Bins<THREADS>& lds,
+                             Listed<KeyType<T>, THREADS>& list) {
+  using W = typename Value<T>::Wide;
+  using Key = KeyType<T>;
+  using Sum = unsigned long long;
+  constexpr int V = Value<T>::kVec;
+  constexpr int kBins = Bins<THREADS>::kBins;
+  constexpr uint32_t kRoom = Listed<Key, THREADS>::kRoom;
+  const T* x = static_cast<const T*>(a.logits) + r * a.stride;
+  const Setting s = row_setting(a, r);
+  const int n = (int)s.n;
+  const Key best = (Key)state.best, floor = (Key)state.floor;
+  const Weight weight((double)KeyOf<W>::value(best), s.temperature);
+  const double scale = mass_scale(n);
+  const auto mass = [&](Key k) { return mass_of(weight.of_key(k), scale); };
+  const auto no_mass = [](Key) { return 0ull; };
+
+  const auto fill_list = [&](const Prefix<Key>& in, Key low, Key high) {
+    __syncthreads();
+    if (threadIdx.x == 0) list.count = 0;
+    __syncthreads();
+    for_each_state<T, THREADS>(x, n, [&](int i, Key k) {
+      if (k < low || k > high || !in.has(i, k)) return;
+      const uint32_t at = atomicAdd(&list.count, 1u);
+      list.key[at] = k;
+      list.index[at] = i;
+    });
+    __syncthreads();
+  };
+  const auto each_listed = [&](auto fn) {
+    const uint32_t count = list.count;
+    for (uint32_t q = threadIdx.x; q < count; q += THREADS) fn(list.key[q]);
+  };
+
+  // ---- top-k: the k-th key by counting
+  Prefix<Key> kept{floor, n};
+  if (s.has_top_k()) {
+    const auto each_state = [&](auto fn) {
+      for_each_state<T, THREADS>(x, n, [&](int, Key k) { fn(k); });
+    };
+    Bin<Key> bin{floor, best, 0ull, 0ull, true};
+    do {
+      bin = find_bin<false>(lds, each_state, no_mass, bin.low, bin.high, bin.above, (double)s.top_k);
+    } while (bin.low != bin.high && bin.states > kRoom);
+    const bool in_list = bin.states <= kRoom;
+    if (in_list) {
+      fill_list(kept, bin.low, bin.high);
+      while (bin.low != bin.high)
+        bin = find_bin<false>(lds, each_listed, no_mass, bin.low, bin.high, bin.above, (double)s.top_k);
+    }
+    kept.key = bin.low;
+    const Sum ties = (Sum)s.top_k - bin.above;
+    if (ties < bin.states) kept.last = last_kept<T, THREADS>(x, n, bin.low, ties, lds, list, in_list);
   }
 
-  // ---- many: the threshold by counts and masses over the whole row
-  const auto each_state = [&](auto fn) {
-    for_each_state<T, THREADS>(x, n, [&](int64_t, Key k) { fn(k); });
+  const int segments = (n + 64 * V - 1) / (64 * V);
+  double* sums = a.block_sums + r * a.sums_per_row;  // the block sums have served: one entry per segment,
+  Sum* extra = reinterpret_cast<Sum*>(sums + segments);  // and what the list adds to it
+  // Weights of the states of a prefix above a key: their sum, and by segments those that min-p leaves.
+  const auto add_up = [&](const Prefix<Key>& in, Key above) {
+    double all = 0.0;
+    for (int q = threadIdx.x >> 6; q < segments; q += THREADS / 64) {
+      const int i = (q * 64 + (int)(threadIdx.x & 63)) * V;
+      double drawn = 0.0;
+      const auto add = [&](int at, Key k) {
+        if (k <= above || !in.has(at, k)) return;
+        const double w = weight.of_key(k);
+        all += w;
+        drawn += w >= s.min_p ? w : 0.0;
+      };
+      if (i + V <= n) {
+        const Pack<T> p = load_pack(x + i);
+#pragma unroll
+        for (int j = 0; j < V; ++j) add(i + j, KeyOf<W>::key(Value<T>::widen(p.v[j])));
+      } else {
+        for (int j = 0; j < V; ++j)
+          if (i + j < n) add(i + j, key_at(x, i + j));
+      }
+      drawn = lanes_sum<64>(drawn);
+      if ((threadIdx.x & 63) == 0) {
+        sums[q] = drawn;
+        extra[q] = 0;
+      }
+    }
+    double total;
+    (void)block_scan<THREADS>(all, lds.words, &total);  // (its barriers also publish the segments' sums)
+    return total;
   };
-  Key threshold = floor;
-  unsigned long long kept_ties = 0, ties = 0;  // of the states on `threshold`; equal: all of them
-  if (s.has_top_k()) {
-    Bin<Key> bin{floor, (Key)best, 0ull, 0ull, true};
-    do {
-      bin = find_bin<false>(lds, each_state, mass, bin.low, bin.high, bin.above, (double)s.top_k, (Key)0, 0ull);
-    } while (bin.low != bin.high);
-    threshold = bin.low;
-    ties = bin.states;
-    kept_ties = (unsigned long long)s.top_k - bin.above;
-  }
+
+  constexpr double kListScale = 1125899906842624.0;  // 2^50: at most 4096 weights add up
+  bool added = false;
   if (s.has_top_p()) {
-    const Key lowest = s.has_top_k() ? threshold : (Key)0;  // the key whose states are not all in A
-    const unsigned long long lowest_mass = s.has_top_k() ? kept_ties * mass(threshold) : 0ull;
-    double target = s.top_p * ldexp(row_total, bits);
-    if (s.has_top_k()) {
-      unsigned long long all = 0;
-      for_each_state<T, THREADS>(x, n, [&](int64_t, Key k) {
-        if (k > threshold) all += mass(k);
-      });
-      target = s.top_p * (double)(block_all<THREADS>(all, lds.words, kSum) + lowest_mass);
-    }
-    Bin<Key> bin{threshold, (Key)best, 0ull, 0ull, true};
-    do {
-      bin = find_bin<true>(lds, each_state, mass, bin.low, bin.high, bin.above, target, lowest, lowest_mass);
-    } while (bin.low != bin.high);
-    const unsigned long long in_a = bin.low == lowest && s.has_top_k() ? kept_ties : bin.states;
-    const double each = (double)mass(bin.low), above = (double)bin.above;
-    unsigned long long keep = in_a;
-    if (each > 0.0) keep = (unsigned long long)fmin(fmax(ceil((target - above) / each), 1.0), (double)in_a);
-    while (keep > 1 && above + (double)(keep - 1) * each >= target) --keep;
-    while (keep < in_a && above + (double)keep * each < target) ++keep;
-    threshold = bin.low;
-    ties = bin.states;
-    kept_ties = keep;
-  }
-  int64_t last_tie = n;
-  if (kept_ties < ties) {  // the index of the last kept state on the threshold
-    constexpr int64_t kStep = (int64_t)THREADS * V;
-    unsigned long long seen = 0;
-    for (int64_t base = 0; base < n && seen < kept_ties; base += kStep) {
-      const int64_t i = base + (int64_t)threadIdx.x * V;
-      unsigned long long mine = 0, all;
-      uint32_t on = 0;
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (i + j < n && key_at(x, i + j) == threshold) {
-          on |= 1u << j;
-          ++mine;
-        }
-      unsigned long long before = seen + block_scan<THREADS>(mine, lds.words, &all);
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (on >> j & 1) {
-          if (++before == kept_ties) lds.answer[0] = i + j;
-        }
-      seen += all;
-    }
+    const double w_all = s.has_top_k() ? add_up(kept, (Key)0) : state.total;
+    const double target = s.top_p * w_all;
+    // counts by key bound the mass from the top: what lies above `high` is kept, what lies below `low` is not
+    const int shift = bin_shift<THREADS>(kept.key, best);
     __syncthreads();
-    last_tie = lds.answer[0];
-  }
-  // ---- the draw: sums of 64 V kept states in index order (they take the place of the block sums)
-  const auto kept_weight = [&](int64_t i, Key k) {
-    if (k < threshold || (k == threshold && i > last_tie)) return 0.0;
-    const double w = weight.of_key(k);
-    return w >= s.min_p ? w : 0.0;
-  };
-  const int64_t segments = (n + 64 * V - 1) / (64 * V);
-  __syncthreads();
-  for (int64_t q = threadIdx.x >> 6; q < segments; q += THREADS / 64) {
-    const int64_t i = q * 64 * V + (int64_t)(threadIdx.x & 63) * V;
-    double sum = 0.0;
-    if (i + V <= n) {
-      const Pack<T> p = load_pack(x + i);
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum += kept_weight(i + j, KeyOf<W>::key(Value<T>::widen(p.v[j])));
-    } else {
-      for (int j = 0; j < V; ++j)
-        if (i + j < n) sum += kept_weight(i + j, key_at(x, i + j));
+    for (int b = 0; b < 4; ++b) lds.count[b * THREADS + threadIdx.x] = 0;
+    __syncthreads();
+    for_each_state<T, THREADS>(x, n, [&](int i, Key k) {
+      if (kept.has(i, k)) atomicAdd(&lds.count[(int)((k - kept.key) >> shift)], 1u);
+    });
+    __syncthreads();
+    double least[4], most[4], least_sum = 0.0, most_sum = 0.0, ignored;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int bin = kBins - 1 - 4 * (int)threadIdx.x - b;
+      const double count = (double)lds.count[bin];
+      least[b] = most[b] = 0.0;
+      if (count > 0.0) {
+        const Key low = kept.key + ((Key)bin << shift);
+        least[b] = count * weight.of_key(low);
+        most[b] = count * weight.of_key(bin_high(low, shift, best));
+      }
+      least_sum += least[b];
+      most_sum += most[b];
     }
-    sum = lanes_sum<64>(sum);
-    if ((threadIdx.x & 63) == 0) sums[q] = sum;
+    double at_least = block_scan<THREADS>(least_sum, lds.words, &ignored);
+    double at_most = block_scan<THREADS>(most_sum, lds.words, &ignored);
+    unsigned int first = ~0u, last = ~0u, lowest = ~0u;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const unsigned int at = 4 * threadIdx.x + b;
+      at_least += least[b];
+      at_most += most[b];
+      if (lds.count[kBins - 1 - at] != 0) {
+        if (first == ~0u && at_most >= target * (1.0 - 1e-9)) first = at;
+        if (last == ~0u && at_least >= target * (1.0 + 1e-9)) last = at;
+        lowest = kBins - 1 - at;
+      }
+    }
+    first = (unsigned int)block_all<THREADS>((Sum)first, lds.words, kMin);
+    last = (unsigned int)block_all<THREADS>((Sum)last, lds.words, kMin);
+    lowest = kBins - 1 - (unsigned int)block_all<THREADS>((Sum)lowest, lds.words, kMin);
+    if (last > lowest) last = lowest;
+    if (first > last) first = last;
+    Sum around = 0;
+    for (unsigned int at = first + threadIdx.x; at <= last; at += THREADS) around += lds.count[kBins - 1 - at];
+    around = block_all<THREADS>(around, lds.words, [](Sum p, Sum q) { return p + q; });
+    Bin<Key> bin;
+    bin.low = kept.key + ((Key)(kBins - 1 - last) << shift);
+    const Key top = kept.key + ((Key)(kBins - 1 - first) << shift);
+    bin.high = bin_high(top, shift, best);
+    bin.states = around;
+    const double certain = add_up(kept, bin.high);
+    bin.above = (Sum)llrint(certain * scale);
+    const double reach = target * scale;
+    const auto each_in = [&](auto fn) {
+      for_each_state<T, THREADS>(x, n, [&](int i, Key k) {
+        if (kept.has(i, k)) fn(k);
+      });
+    };
+    while (bin.low != bin.high && bin.states > kRoom)
+      bin = find_bin<true>(lds, each_in, mass, bin.low, bin.high, bin.above, reach);
+    const bool in_list = bin.states <= kRoom;
+    const Key list_high = bin.high;
+    if (in_list) {
+      fill_list(kept, bin.low, bin.high);
+      do {
+        bin = find_bin<true>(lds, each_listed, mass, bin.low, bin.high, bin.above, reach);
+      } while (bin.low != bin.high);
+    }
+    // of the states on the key: those with less than the target before them, one at least
+    const double each = (double)mass(bin.low), above = (double)bin.above;
+    Sum ties = bin.states;
+    if (each > 0.0) ties = (Sum)fmin(fmax(ceil((reach - above) / each), 1.0), (double)bin.states);
+    while (ties > 1 && above + (double)(ties - 1) * each >= reach) --ties;
+    while (ties < bin.states && above + (double)ties * each < reach) ++ties;
+    const int bound = bin.low == kept.key ? kept.last : n;
+    kept.key = bin.low;
+    kept.last = ties < bin.states ? last_kept<T, THREADS>(x, n, bin.low, ties, lds, list, in_list) : bound;
+    if (in_list) {
+      // the segments hold what lies above the first bounds; the list holds the rest, if it begins there
+      added = list_high == bin_high(top, shift, best);
+      if (added) {
+        const uint32_t count = list.count;
+        for (uint32_t q = threadIdx.x; q < count; q += THREADS)
+          if (kept.has(list.index[q], list.key[q])) {
+            const double w = weight.of_key(list.key[q]);
+            if (w >= s.min_p) atomicAdd(&extra[list.index[q] / (64 * V)], mass_of(w, kListScale));
+          }
+        __threadfence();
+      }
+    }
   }
+  if (!added) (void)add_up(kept, (Key)0);
   __syncthreads();
-  return locate<THREADS, V>(lds, segments, s.uniform, [&](int64_t q) { return sums[q]; }, [&](int64_t i) {
-    return i < n ? kept_weight(i, key_at(x, std::min(i, n - 1))) : 0.0;
-  });
+  return locate<THREADS, V>(
+      lds, segments, s.uniform,
+      [&](int q) {
+        const Sum more = __hip_atomic_load(&extra[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return sums[q] + (double)more / kListScale;
+      },
+      [&](int i) {
+        if (i >= n) return 0.0;
+        const Key k = key_at(x, std::min(i, n - 1));
+        const double w = kept.has(i, k) ? weight.of_key(k) : 0.0;
+        return w >= s.min_p ? w : 0.0;
+      });
 }
 
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS) draw_long(const Draws a) {
-  __shared__ Shared<KeyType<T>, THREADS> lds;
-  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const int64_t state = draw_row<T, THREADS>(a, r, lds);
-    if (threadIdx.x == 0) a.out[r] = (int32_t)state;
-    __syncthreads();
-  }
+__global__ void __launch_bounds__(THREADS) draw_wide(const Draws a, int64_t first_row) {
+  __shared__ Bins<THREADS> lds;
+  __shared__ Listed<KeyType<T>, THREADS> list;
+  const int64_t r = first_row + blockIdx.x;
+  const RowState state = a.row_states[r];
+  if (!state.pending) return;
+  const int drawn = draw_wide_row<T, THREADS>(a, r, state, lds, list);
+  if (threadIdx.x == 0) a.out[r] = drawn;
 }
 
 constexpr int64_t kMaxStates = 1 << 24;
@@ -975,8 +1194,15 @@ constexpr int64_t kMaxBlocks = 1 << 20;
 template <typename T, int G, int E>
 void launch_short(const Draws& a, hipStream_t s) {
   const int64_t per_block = kShortThreads / G;
-  hipLaunchKernelGGL((draw_short<T, G, E>), dim3((uint32_t)std::min((a.rows + per_block - 1) / per_block, kMaxBlocks)),
-                     dim3(kShortThreads), 0, s, a);
+  const bn_draw_filters& f = a.filters;
+  const bool filter = f.top_k_dev || f.top_p_dev || (f.top_k > 0 && f.top_k < a.width) || f.top_p < 1.0;
+  for (int64_t r = 0; r < a.rows; r += kMaxBlocks * per_block) {
+    const dim3 grid((uint32_t)std::min((a.rows - r + per_block - 1) / per_block, kMaxBlocks));
+    if (filter)
+      hipLaunchKernelGGL((draw_short<T, true, G, E>), grid, dim3(kShortThreads), 0, s, a, r);
+    else
+      hipLaunchKernelGGL((draw_short<T, false, G, E>), grid, dim3(kShortThreads), 0, s, a, r);
+  }
 }
 
 template <typename T>
@@ -984,13 +1210,19 @@ void launch_long(const Draws& a, hipStream_t s) {
   constexpr int kPacks = 4;
   constexpr int64_t kTile = (int64_t)64 * Value<T>::kVec * kPacks * (kSummaryThreads / 64);
   const int64_t tiles = (a.width + kTile - 1) / kTile;
+  const bn_draw_filters& f = a.filters;
+  const bool filter = f.top_k_dev || f.top_p_dev || f.min_p_dev || f.top_k > 0 || f.top_p < 1.0 || f.min_p > 0.0;
   hipLaunchKernelGGL((block_summaries<T, kPacks>), dim3((uint32_t)std::min(a.rows * tiles, kMaxBlocks)),
                      dim3(kSummaryThreads), 0, s, a, tiles);
-  const dim3 grid((uint32_t)std::min(a.rows, kMaxBlocks));
-  if (a.width <= 16384)
-    hipLaunchKernelGGL((draw_long<T, 256>), grid, dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((draw_long<T, 512>), grid, dim3(512), 0, s, a);
+  for (int64_t r = 0; r < a.rows; r += kMaxBlocks) {
+    const dim3 grid((uint32_t)std::min(a.rows - r, kMaxBlocks));
+    hipLaunchKernelGGL(draw_long<T>, grid, dim3(kLongThreads), 0, s, a, r);
+    if (!filter) continue;
+    if (a.width <= 16384)
+      hipLaunchKernelGGL((draw_wide<T, 256>), grid, dim3(256), 0, s, a, r);
+    else
+      hipLaunchKernelGGL((draw_wide<T, 1024>), grid, dim3(1024), 0, s, a, r);
+  }
 }
 
 template <typename T>

@@ -3,8 +3,8 @@ hands, with ties, masks, padding and every filter.
 
 The states have to be equal.  Both sides sum in double (the kept set's borders partly in integers
 of 2^-38 of a weight or finer), so they can only differ where a border lies within 1e-10 of the target;
-the oracle says how far its borders are, and no test row here is nearer than that unless all its sums are
-exact (equal weights)."""
+the oracle says how far its borders are.  A row that is nearer than that (among a million states some
+weights are below 1e-10 of the sum) is not compared, unless all its sums are exact (equal weights)."""
 
 import numpy as np
 import pytest
@@ -48,11 +48,15 @@ def _oracle(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
 
 def _check(got, rows, uniforms, settings, exact_sums=False):
     got = got.cpu().numpy()
+    undecided = 0
     for r, x in enumerate(rows):
         want, margin = _oracle(x, float(uniforms[r]), **{k: v[r] if hasattr(v, "__len__") else v
                                                          for k, v in settings.items()})
-        assert exact_sums or margin > 1e-10, (r, margin)
+        if margin <= 1e-10 and not exact_sums:
+            undecided += 1
+            continue
         assert got[r] == want, (r, got[r], want, margin)
+    assert undecided <= len(rows) // 4
 
 
 SETTINGS = {
@@ -220,6 +224,28 @@ def test_long_rows_of_flat_and_peaked_distributions():
         u = torch.rand((6,), generator=gen, dtype=torch.float64)
         for settings in (dict(), dict(top_p=0.97), dict(top_k=5000), dict(top_k=20000, top_p=0.5, min_p=1e-4)):
             _check(draw_states(x.cuda(), u.cuda(), **settings), x.double().numpy(), u.numpy(), settings)
+
+
+@pytest.mark.parametrize("states,dtype", [(2000, torch.float32), (3001, torch.float16), (9000, torch.bfloat16),
+                                          (60001, torch.float64), (300007, torch.float16), (1200001, torch.float32)],
+                         ids=str)
+def test_rows_that_keep_many_states(states, dtype):
+    """Filters that leave most of a flat row: the threshold lies among thousands of states, on keys that many
+    share (float16, bfloat16) or that are nearly all different; some rows end inside their ties."""
+    from bayesiannetwork_amd.samplers import draw_states
+
+    gen = torch.Generator().manual_seed(states)
+    rows = 4
+    x = torch.randn((rows, states), generator=gen)
+    x[0] = torch.round(x[0] * 2) / 2  # a dozen keys
+    x[1] *= 0.05
+    x[2] *= 3
+    x = x.to(dtype)
+    u = torch.rand((rows,), generator=gen, dtype=torch.float64)
+    for settings in (dict(top_p=0.93), dict(top_k=states // 3), dict(top_k=states - 7, temperature=0.8),
+                     dict(top_k=states // 2, top_p=0.6), dict(min_p=0.01), dict(top_p=0.9, min_p=0.05),
+                     dict(top_k=states // 2, top_p=0.7, min_p=0.02), dict(top_p=0.999999)):
+        _check(draw_states(x.cuda(), u.cuda(), **settings), x.double().numpy(), u.numpy(), settings)
 
 
 def test_frequencies_of_a_posterior():

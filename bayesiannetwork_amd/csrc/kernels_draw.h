@@ -184,102 +184,66 @@ __device__ __forceinline__ double group_scan(double v, double* total) {
   const double before = __shfl_up(upto, 1, G);
   return lane == 0 ? 0.0 : before;
 }
-template <int G, typename U, typename Combine>
-__device__ __forceinline__ U group_all(U v, Combine combine) {
-#pragma unroll
-  for (int d = 1; d < G; d <<= 1) v = combine(v, (U)__shfl_xor(v, d, 64));
-  return v;
-}
-
 // ---- a row in registers: E states in each of G lanes --------------------------------------------
 
-// What is sorted: (key, slot) with larger keys and, on one key, lower slots first.  A 32-bit key and a
-// slot below 1024 are 42 bits: as the mantissa of a double they are exchanged by one v_max_f64 and one
-// v_min_f64.
-struct Packed {
-  double v;
-  static __device__ __forceinline__ Packed make(uint32_t key, int slot) {
-    const uint32_t low = (key << 10) | (uint32_t)(1023 - slot);
-    return {__longlong_as_double((long long)(((uint64_t)(0x43300000u | (key >> 22)) << 32) | low))};
-  }
-  __device__ __forceinline__ uint32_t key() const {
-    const uint64_t b = (uint64_t)__double_as_longlong(v);
-    return (uint32_t)(b >> 10);
-  }
-  __device__ __forceinline__ bool above(const Packed& o) const { return v > o.v; }
-  static __device__ __forceinline__ void order(Packed& hi, Packed& lo) {
-    double big, small;  // never NaN: no canonicalisation needed, which fmax would bring
-    asm("v_max_f64 %0, %1, %2" : "=v"(big) : "v"(hi.v), "v"(lo.v));
-    asm("v_min_f64 %0, %1, %2" : "=v"(small) : "v"(hi.v), "v"(lo.v));
-    hi.v = big;
-    lo.v = small;
-  }
-  template <int MASK>
-  __device__ __forceinline__ Packed other() const { return {lane_xor<MASK>(v)}; }
-  __device__ __forceinline__ Packed shuffled(int mask) const { return {__shfl_xor(v, mask, 64)}; }
-};
-struct Wide64 {
-  uint64_t k;
-  uint32_t slot;
-  static __device__ __forceinline__ Wide64 make(uint64_t key, int slot) { return {key, (uint32_t)slot}; }
-  __device__ __forceinline__ uint64_t key() const { return k; }
-  __device__ __forceinline__ bool above(const Wide64& o) const { return k > o.k || (k == o.k && slot < o.slot); }
-  static __device__ __forceinline__ void order(Wide64& hi, Wide64& lo) {
-    const Wide64 a = hi, b = lo;
-    const bool swap = b.above(a);
-    hi = swap ? b : a;
-    lo = swap ? a : b;
-  }
-  template <int MASK>
-  __device__ __forceinline__ Wide64 other() const { return {lane_xor<MASK>(k), lane_xor<MASK>(slot)}; }
-  __device__ __forceinline__ Wide64 shuffled(int mask) const {
-    return {(uint64_t)__shfl_xor((unsigned long long)k, mask, 64), (uint32_t)__shfl_xor((int)slot, mask, 64)};
-  }
-};
-template <typename Key>
-struct Sorted;
-template <>
-struct Sorted<uint32_t> { using Type = Packed; };
-template <>
-struct Sorted<uint64_t> { using Type = Wide64; };
+// a and b in descending order.  (Plain v_max / v_min: fmax would first make NaNs of signalling ones quiet,
+// and a row with a NaN is not drawn anyway.)
+__device__ __forceinline__ void order(float& a, float& b) {
+  float hi, lo;
+  asm("v_max_f32 %0, %1, %2" : "=v"(hi) : "v"(a), "v"(b));
+  asm("v_min_f32 %0, %1, %2" : "=v"(lo) : "v"(a), "v"(b));
+  a = hi;
+  b = lo;
+}
+__device__ __forceinline__ void order(double& a, double& b) {
+  double hi, lo;
+  asm("v_max_f64 %0, %1, %2" : "=v"(hi) : "v"(a), "v"(b));
+  asm("v_min_f64 %0, %1, %2" : "=v"(lo) : "v"(a), "v"(b));
+  a = hi;
+  b = lo;
+}
 
-template <int MASK, int E, bool MIRROR, typename C>
-__device__ __forceinline__ void exchange_lanes(C (&c)[E], bool lower) {
-  // no two are equal: the slots differ.  Two at a time, since a mirrored pair reads each other's place.
+template <int MASK, int E, bool MIRROR, typename W>
+__device__ __forceinline__ void exchange_lanes(W (&c)[E], bool lower) {
+  // two at a time, since a mirrored pair reads each other's place
   static_assert(!MIRROR || E == 1 || E % 2 == 0, "mirrored in pairs");
 #pragma unroll
   for (int j = 0; j < (E + 1) / 2; ++j) {
     const int k = E - 1 - j;
-    const C at_j = c[MIRROR ? k : j].template other<MASK>();
-    const C at_k = c[MIRROR ? j : k].template other<MASK>();
-    if (at_j.above(c[j]) == lower) c[j] = at_j;
-    if (k != j && at_k.above(c[k]) == lower) c[k] = at_k;
+    W at_j = lane_xor<MASK>(c[MIRROR ? k : j]), at_k = lane_xor<MASK>(c[MIRROR ? j : k]);
+    order(c[j], at_j);
+    if (!lower) c[j] = at_j;
+    if (k != j) {
+      order(c[k], at_k);
+      if (!lower) c[k] = at_k;
+    }
   }
 }
 
-template <int STRIDE, int E, typename C>
-__device__ __forceinline__ void half_cleaners(C (&c)[E], int lane) {
+template <int STRIDE, int E, typename W>
+__device__ __forceinline__ void half_cleaners(W (&c)[E], int lane) {
   if constexpr (STRIDE >= 1) {
     if constexpr (STRIDE >= E) {
       exchange_lanes<STRIDE / E, E, false>(c, (lane & (STRIDE / E)) == 0);
     } else {
 #pragma unroll
       for (int j = 0; j < E; ++j)
-        if ((j & STRIDE) == 0) C::order(c[j], c[j | STRIDE]);
+        if ((j & STRIDE) == 0) order(c[j], c[j | STRIDE]);
     }
     half_cleaners<STRIDE / 2, E>(c, lane);
   }
 }
 
-// Bitonic sort of G * E entries, the largest first (position lane * E + j); every merge starts by comparing
-// mirrored positions, so that all exchanges point the same way.
-template <int K, int G, int E, typename C>
-__device__ __forceinline__ void sort_group(C (&c)[E], int lane) {
+// Bitonic sort of G * E logits, the largest first (position lane * E + j); every merge starts by comparing
+// mirrored positions, so that all exchanges point the same way.  Logits alone: which of the equal ones are
+// kept is told by counting them afterwards, and an exchange costs two instructions of the full rate.
+template <int K, int G, int E, typename W>
+__device__ __forceinline__ void sort_group(W (&c)[E], int lane) {
   if constexpr (K <= G * E) {
     if constexpr (K <= E) {
 #pragma unroll
       for (int j = 0; j < E; ++j)
-        if ((j ^ (K - 1)) > j) C::order(c[j], c[j ^ (K - 1)]);
+        if ((j ^ (K - 1)) > j) order(c[j], c[j ^ (K - 1)]);
     } else {
       exchange_lanes<K / E - 1, E, true>(c, (lane & (K / E / 2)) == 0);
     }
@@ -288,59 +252,88 @@ __device__ __forceinline__ void sort_group(C (&c)[E], int lane) {
   }
 }
 
-// The draw among states held by a group of lanes, key[j] of slot lane * E + j, 0 where there is none; slots
-// ascend with the states' indices.  `total`: the weight that top-p is a share of, when top-k is off and
-// states outside the group hold some of it; negative: the group's.  Returns the slot, the same in every lane.
-template <bool FILTER, int G, int E, typename Key>
-__device__ int draw_in_group(const Key (&key)[E], const Setting& s, const Weight& weight, double row_total) {
-  using C = typename Sorted<Key>::Type;
+// The draw among `count` states held by a group of lanes, x[j] of slot lane * E + j (-inf beyond the count);
+// slots ascend with the states' indices.  `row_total`: the weight that top-p is a share of, when top-k is off
+// and states outside the group hold some of it; negative: the group's.  Returns the slot, the same in every
+// lane.  FILTER: some row may have a top-k or top-p.
+template <bool FILTER, int G, int E, typename W>
+__device__ int draw_in_group(const W (&x)[E], int count, const Setting& s, const Weight& weight, double row_total) {
   const int lane = threadIdx.x % G;
-  const bool filtered = s.has_top_k() || s.has_top_p();
-  C floor = C::make(0, 0);
+  const auto least = [](W p, W q) { return fmin(p, q); };
+  const auto add = [](int p, int q) { return p + q; };
+  W threshold = -INFINITY;
+  int ties = INT32_MAX;  // states on the threshold that are kept
   // rows of one wave differ in their settings: the wave sorts if any of them has to
+  const bool filtered = s.has_top_k() || s.has_top_p();
   if (FILTER && __any(filtered)) {
-    C c[E];
+    W c[E];
 #pragma unroll
-    for (int j = 0; j < E; ++j) c[j] = C::make(key[j], lane * E + j);
+    for (int j = 0; j < E; ++j) c[j] = x[j];
     sort_group<2, G, E>(c, lane);
-    double w[E], here = 0.0, all;
+    // the kept ones are a prefix of the order: its length, and the last one's logit
+    const int top = (int)(s.top_k < count ? s.top_k : count);
+    int length = 0;
+    W last = INFINITY;
+    if (__any(s.has_top_p())) {
+      double w[E], here = 0.0, all;
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      w[j] = lane * E + j < s.top_k && c[j].key() != 0 ? weight.of_key(c[j].key()) : 0.0;
-      here += w[j];
-    }
-    double before = group_scan<G>(here, &all);
-    const double target = s.top_p * (row_total >= 0.0 ? row_total : all);
-    // the last kept entry: the first one, and those with less than the target before them
-    C last = C::make(0, 0);
-    bool any = false;
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const int at = lane * E + j;
-      if (at < s.top_k && c[j].key() != 0 && (at == 0 || before < target)) {
-        last = c[j];
-        any = true;
+      for (int j = 0; j < E; ++j) {
+        w[j] = lane * E + j < top ? weight((double)c[j]) : 0.0;
+        here += w[j];
       }
-      before += w[j];
+      double before = group_scan<G>(here, &all);
+      const double target = s.top_p * (row_total >= 0.0 ? row_total : all);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int at = lane * E + j;
+        // those with less than the target before them, and the first one in any case
+        const bool kept = at < top && (at == 0 || before < target);
+        length += kept;
+        last = kept ? c[j] : last;
+        before += w[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const bool kept = lane * E + j < top;
+        length += kept;
+        last = kept ? c[j] : last;
+      }
     }
-    // kept entries are a prefix of the order: of the lanes' last ones the lowest is the threshold
-    if (!any) last = C::make((Key)~(Key)0, 0);
+    length = lanes_all<G>(length, add);
+    last = lanes_all<G>(last, least);
+    int above = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) above += c[j] > last;
+    above = lanes_all<G>(above, add);
+    if (filtered) {
+      threshold = last;
+      ties = length - above;
+    }
+  }
+  int on_threshold = 0;
+  if (FILTER) {  // ties are kept in the order of their slots
+#pragma unroll
+    for (int j = 0; j < E; ++j) on_threshold += x[j] == threshold;
+    int upto = on_threshold;
 #pragma unroll
     for (int d = 1; d < G; d <<= 1) {
-      const C o = last.shuffled(d);
-      if (last.above(o)) last = o;
+      const int left = __shfl_up(upto, d, G);
+      if (lane >= d) upto += left;
     }
-    if (filtered) floor = last;
+    on_threshold = upto - on_threshold;  // in the lanes before
   }
   double w[E], here = 0.0, all;
 #pragma unroll
   for (int j = 0; j < E; ++j) {
-    const C c = C::make(key[j], lane * E + j);
-    w[j] = 0.0;
-    if (key[j] != 0 && !floor.above(c)) {
-      w[j] = weight.of_key(key[j]);
-      if (w[j] < s.min_p) w[j] = 0.0;
+    w[j] = weight((double)x[j]);
+    bool kept = w[j] >= s.min_p;
+    if (FILTER) {
+      const bool tie = x[j] == threshold;
+      kept = kept && (x[j] > threshold || (tie && on_threshold < ties));
+      on_threshold += tie;
     }
+    if (!kept) w[j] = 0.0;
     here += w[j];
   }
   double upto = group_scan<G>(here, &all);
@@ -354,72 +347,61 @@ __device__ int draw_in_group(const Key (&key)[E], const Setting& s, const Weight
       if (upto > target && pick == INT32_MAX) pick = last;
     }
   }
-  pick = group_all<G>(pick, [](int p, int q) { return p < q ? p : q; });
-  last = group_all<G>(last, [](int p, int q) { return p > q ? p : q; });
+  pick = lanes_all<G>(pick, [](int p, int q) { return p < q ? p : q; });
+  last = lanes_all<G>(last, [](int p, int q) { return p > q ? p : q; });
   return pick == INT32_MAX ? last : pick;  // u = 1, or the sums' rounding: the last kept state
 }
 
 // The lowest slot that holds `best`.
-template <int G, int E, typename Key>
-__device__ __forceinline__ int first_in_group(const Key (&key)[E], Key best) {
+template <int G, int E, typename W>
+__device__ __forceinline__ int first_in_group(const W (&x)[E], W best) {
   int first = INT32_MAX;
 #pragma unroll
   for (int j = E - 1; j >= 0; --j)
-    if (key[j] == best) first = (int)(threadIdx.x % G) * E + j;
-  return group_all<G>(first, [](int p, int q) { return p < q ? p : q; });
+    if (x[j] == best) first = (int)(threadIdx.x % G) * E + j;
+  return lanes_all<G>(first, [](int p, int q) { return p < q ? p : q; });
 }
 
 constexpr int kShortThreads = 256;
 
 // Rows of up to G * E states.
-// FILTER: some row may have a top-k or top-p (without them the sort's registers are not claimed either).
 template <typename T, bool FILTER, int G, int E>
-__global__ void __launch_bounds__(kShortThreads, FILTER ? 4 : 6) draw_short(const Draws a, int64_t first_row) {
+__global__ void __launch_bounds__(kShortThreads) draw_short(const Draws a, int64_t first_row) {
   using W = typename Value<T>::Wide;
-  using Key = KeyType<T>;
   constexpr int V = Value<T>::kVec;
   constexpr int kRows = kShortThreads / G;
   const int lane = threadIdx.x % G;
   const int64_t r = first_row + (int64_t)blockIdx.x * kRows + threadIdx.x / G;
   if (r >= a.rows) return;  // whole groups leave together
-  const T* x = static_cast<const T*>(a.logits) + r * a.stride;
+  const T* row = static_cast<const T*>(a.logits) + r * a.stride;
   const Setting s = row_setting(a, r);
   const int n = (int)s.n, first = lane * E;
-  Key key[E];
-  bool bad = false;
-  Key best = 0;
-  const auto take = [&](int j, T v) {
-    const W wide = Value<T>::widen(v);
-    bad |= undrawable(wide);
-    key[j] = KeyOf<W>::key(wide);
-    best = best > key[j] ? best : key[j];
-  };
+  W x[E];
   if (E >= V && first + E <= n) {
 #pragma unroll
     for (int k = 0; k + V <= E; k += V) {
-      const Pack<T> p = load_pack(x + first + k);
+      const Pack<T> p = load_pack(row + first + k);
 #pragma unroll
-      for (int j = 0; j < V; ++j) take(k + j, p.v[j]);
+      for (int j = 0; j < V; ++j) x[k + j] = Value<T>::widen(p.v[j]);
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      key[j] = 0;
-      if (first + j < n) take(j, x[first + j]);
-    }
+    for (int j = 0; j < E; ++j) x[j] = first + j < n ? Value<T>::widen(row[first + j]) : (W)-INFINITY;
   }
+  bool bad = false;
+  W best = -INFINITY;
 #pragma unroll
-  for (int d = 1; d < G; d <<= 1) {
-    const Key o = (Key)__shfl_xor((typename std::conditional<sizeof(Key) == 8, unsigned long long, unsigned>::type)best, d, 64);
-    best = best > o ? best : o;
+  for (int j = 0; j < E; ++j) {
+    bad |= undrawable(x[j]);
+    best = fmax(best, x[j]);
   }
-  bad = group_all<G>((int)bad, [](int p, int q) { return p | q; }) != 0;
-  const double largest = (double)KeyOf<W>::value(best);
-  const bool valid = s.valid && !bad && !isinf(largest);
+  best = lanes_max<G>(best);
+  bad = lanes_all<G>((int)bad, [](int p, int q) { return p | q; }) != 0;
+  const bool valid = s.valid && !bad && !isinf(best);
   const bool greedy = s.temperature == 0.0;
-  const Weight weight(valid ? largest : 0.0, greedy ? 1.0 : s.temperature);
-  int pick = draw_in_group<FILTER, G, E>(key, s, weight, -1.0);
-  if (greedy) pick = first_in_group<G, E>(key, best);
+  const Weight weight(valid ? (double)best : 0.0, greedy ? 1.0 : s.temperature);
+  int pick = draw_in_group<FILTER, G, E>(x, n, s, weight, -1.0);
+  if (greedy) pick = first_in_group<G, E>(x, best);
   if (lane == 0) a.out[r] = valid ? pick : -1;
 }
 
@@ -507,11 +489,12 @@ constexpr int kLongThreads = 256;
 
 template <int THREADS>
 struct Bins {
+  static constexpr int kThreads = THREADS;
   static constexpr int kBins = 4 * THREADS;
-  unsigned long long mass[kBins];
-  uint32_t count[kBins];
   unsigned long long words[THREADS / 64];
   long long answer[4];
+  unsigned long long mass[kBins];
+  uint32_t count[kBins];
 };
 
 template <int THREADS, typename U, typename Combine>
@@ -529,6 +512,12 @@ __device__ __forceinline__ U block_all(U v, unsigned long long* lds, Combine com
 }
 constexpr auto kMax = [](unsigned long long p, unsigned long long q) { return p > q ? p : q; };
 constexpr auto kMin = [](unsigned long long p, unsigned long long q) { return p < q ? p : q; };
+// two 32-bit minima at once
+constexpr auto kMinOfHalves = [](unsigned long long p, unsigned long long q) {
+  const uint32_t hi = (uint32_t)(p >> 32) < (uint32_t)(q >> 32) ? (uint32_t)(p >> 32) : (uint32_t)(q >> 32);
+  const uint32_t lo = (uint32_t)p < (uint32_t)q ? (uint32_t)p : (uint32_t)q;
+  return ((unsigned long long)hi << 32) | lo;
+};
 
 // Exclusive prefix sum of one value per thread, and the block's total.
 template <int THREADS, typename U>
@@ -567,36 +556,19 @@ __device__ __forceinline__ unsigned long long mass_of(double w, double scale) {
   return (unsigned long long)__double_as_longlong(shifted) & 0xFFFFFFFFFFFFFull;
 }
 
-template <typename Key>
-struct Bin {
-  Key low, high;              // keys of the bin
-  unsigned long long above;   // count or mass of the bins above it
-  unsigned long long states;  // in it
-  bool reached;               // the target is reached in it or above; else it is the lowest that holds a state
+// A bin, and what lies above it.
+struct Found {
+  int bin;
+  unsigned long long above;   // count or mass of the bins above
+  unsigned long long states;  // in the bin
+  bool reached;               // the target is reached in it; else it is the lowest that holds a state
 };
 
-// How keys of [low, high] fall into the bins.
-template <int THREADS, typename Key>
-__device__ __forceinline__ int bin_shift(Key low, Key high) {
-  constexpr int kLog = THREADS == 1024 ? 12 : THREADS == 512 ? 11 : 10;
-  static_assert((1 << kLog) == Bins<THREADS>::kBins, "four bins per thread");
-  const Key range = high - low;
-  const int bits = sizeof(Key) == 8 ? 64 - __clzll((long long)range) : 32 - __clz((int)(uint32_t)range);
-  return bits > kLog ? bits - kLog : 0;
-}
-template <typename Key>
-__device__ __forceinline__ Key bin_high(Key bin_low, int shift, Key high) {
-  const Key top = bin_low + (((Key)1 << shift) - 1);
-  return top > high || top < bin_low ? high : top;
-}
-
-// The bin of keys in [low, high] in which the count (BY_MASS: the mass) from the top, `above` included,
-// reaches `target`.  each(fn) calls fn(key) for every key there is; keys outside the range are passed over.
-template <bool BY_MASS, int THREADS, typename Key, typename Each, typename Mass>
-__device__ Bin<Key> find_bin(Bins<THREADS>& lds, Each each, Mass mass, Key low, Key high, unsigned long long above,
-                             double target) {
-  constexpr int kBins = Bins<THREADS>::kBins;
-  const int shift = bin_shift<THREADS>(low, high);
+// The bin in which the count (BY_MASS: the mass) from the top, `above` included, reaches `target`.  each(fn)
+// calls fn(key) for every key there is; bin_of(key) is its bin, ascending with the key, or negative.
+template <bool BY_MASS, typename Lds, typename Each, typename BinOf, typename Mass>
+__device__ Found find_bin(Lds& lds, Each each, BinOf bin_of, Mass mass, unsigned long long above, double target) {
+  constexpr int THREADS = Lds::kThreads, kBins = Lds::kBins;
   __syncthreads();
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
@@ -604,9 +576,9 @@ __device__ Bin<Key> find_bin(Bins<THREADS>& lds, Each each, Mass mass, Key low, 
     if (BY_MASS) lds.mass[b * THREADS + threadIdx.x] = 0;
   }
   __syncthreads();
-  each([&](Key k) {
-    if (k < low || k > high) return;
-    const int bin = (int)((k - low) >> shift);
+  each([&](auto k) {
+    const int bin = bin_of(k);
+    if (bin < 0) return;
     atomicAdd(&lds.count[bin], 1u);
     if (BY_MASS) atomicAdd(&lds.mass[bin], mass(k));
   });
@@ -620,13 +592,12 @@ __device__ Bin<Key> find_bin(Bins<THREADS>& lds, Each each, Mass mass, Key low, 
     sum += own[b];
   }
   unsigned long long before = above + block_scan<THREADS>(sum, lds.words, &total);
-  // the first bin that reaches the target in the high word, the last one that holds a state (counted from the
-  // other end) in the low one
-  unsigned int found = ~0u, lowest = ~0u;
+  // the first bin that reaches the target and, counted from the other end, the last one that holds a state
+  uint32_t found = ~0u, lowest = ~0u;
   unsigned long long found_above = 0, lowest_above = 0;
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
-    const unsigned int at = 4 * threadIdx.x + b;
+    const uint32_t at = 4 * threadIdx.x + b;
     if (lds.count[kBins - 1 - at] != 0) {
       if (found == ~0u && (double)(before + own[b]) >= target) {
         found = at;
@@ -637,31 +608,46 @@ __device__ Bin<Key> find_bin(Bins<THREADS>& lds, Each each, Mass mass, Key low, 
     }
     before += own[b];
   }
-  const unsigned long long both = block_all<THREADS>(((unsigned long long)found << 32) | lowest, lds.words,
-                                                     [](unsigned long long p, unsigned long long q) {
-                                                       const unsigned long long hi = (p >> 32) < (q >> 32) ? p >> 32 : q >> 32;
-                                                       const uint32_t lo = std::min((uint32_t)p, (uint32_t)q);
-                                                       return (hi << 32) | lo;
-                                                     });
+  const unsigned long long both = block_all<THREADS>(((unsigned long long)found << 32) | lowest, lds.words, kMinOfHalves);
   const bool reached = (uint32_t)(both >> 32) != ~0u;
   const int at = reached ? (int)(both >> 32) : kBins - 1 - (int)(uint32_t)both;
   if (threadIdx.x == (unsigned)(at / 4)) lds.answer[0] = (long long)(reached ? found_above : lowest_above);
   __syncthreads();
-  const int bin = kBins - 1 - at;
-  Bin<Key> out;
-  out.low = low + ((Key)bin << shift);
-  out.high = bin_high(out.low, shift, high);
-  out.above = (unsigned long long)lds.answer[0];
-  out.states = lds.count[bin];
-  out.reached = reached;
-  return out;
+  return {kBins - 1 - at, (unsigned long long)lds.answer[0], lds.count[kBins - 1 - at], reached};
+}
+
+// A range of keys, what lies above it and how many states it holds.
+template <typename Key>
+struct KeyRange {
+  Key low, high;
+  unsigned long long above, states;
+  bool reached;
+};
+
+// find_bin with as many bins of equal width as there are for the keys of a range; narrows it to the one found.
+template <bool BY_MASS, typename Lds, typename Key, typename Each, typename Mass>
+__device__ void narrow(Lds& lds, KeyRange<Key>& range, Each each, Mass mass, double target) {
+  constexpr int kLog = Lds::kThreads == 1024 ? 12 : 10;
+  static_assert((1 << kLog) == Lds::kBins, "four bins per thread");
+  const Key low = range.low, high = range.high, span = high - low;
+  const int bits = sizeof(Key) == 8 ? 64 - __clzll((long long)span) : 32 - __clz((int)(uint32_t)span);
+  const int shift = bits > kLog ? bits - kLog : 0;
+  const Found f = find_bin<BY_MASS>(
+      lds, each, [&](Key k) { return k < low || k > high ? -1 : (int)((k - low) >> shift); }, mass, range.above, target);
+  range.low = low + ((Key)f.bin << shift);
+  const Key top = range.low + (((Key)1 << shift) - 1);
+  range.high = top > high || top < range.low ? high : top;
+  range.above = f.above;
+  range.states = f.states;
+  range.reached = f.reached;
 }
 
 // Finds the state at which a cumulative sum exceeds its target: segment sums in index order first, then the
 // 64 * PER states of one segment by one wave.  sum_of(segment) is the segment's weight, weight_at(index) a
 // state's (0: not kept).
-template <int THREADS, int PER, typename Lds, typename SumOf, typename WeightAt>
+template <int PER, typename Lds, typename SumOf, typename WeightAt>
 __device__ int locate(Lds& lds, int segments, double uniform, SumOf sum_of, WeightAt weight_at) {
+  constexpr int THREADS = Lds::kThreads;
   const int each = (segments + THREADS - 1) / THREADS;
   const int begin = std::min((int)threadIdx.x * each, segments);
   const int end = std::min(begin + each, segments);
@@ -677,12 +663,7 @@ __device__ int locate(Lds& lds, int segments, double uniform, SumOf sum_of, Weig
   // the first thread whose segments exceed the target; u = 1, or the sums' rounding: the last that holds anything
   const uint32_t over = here > 0.0 && left + here > target ? threadIdx.x : ~0u;
   const uint32_t filled = here > 0.0 ? THREADS - 1 - threadIdx.x : ~0u;
-  const unsigned long long both = block_all<THREADS>(((unsigned long long)over << 32) | filled, lds.words,
-                                                     [](unsigned long long p, unsigned long long q) {
-                                                       const unsigned long long hi = (p >> 32) < (q >> 32) ? p >> 32 : q >> 32;
-                                                       const uint32_t lo = std::min((uint32_t)p, (uint32_t)q);
-                                                       return (hi << 32) | lo;
-                                                     });
+  const unsigned long long both = block_all<THREADS>(((unsigned long long)over << 32) | filled, lds.words, kMinOfHalves);
   const bool none = (uint32_t)(both >> 32) == ~0u;
   const uint32_t owner = none ? THREADS - 1 - (uint32_t)both : (uint32_t)(both >> 32);
   if (threadIdx.x == owner) {
@@ -715,37 +696,52 @@ __device__ int locate(Lds& lds, int segments, double uniform, SumOf sum_of, Weig
         if (!none && upto > target && pick == INT32_MAX) pick = last;
       }
     }
-    pick = group_all<64>(pick, [](int p, int q) { return p < q ? p : q; });
-    last = group_all<64>(last, [](int p, int q) { return p > q ? p : q; });
+    pick = lanes_all<64>(pick, [](int p, int q) { return p < q ? p : q; });
+    last = lanes_all<64>(last, [](int p, int q) { return p > q ? p : q; });
     if (threadIdx.x == 0) lds.answer[3] = start + (pick == INT32_MAX ? last : pick);
   }
   __syncthreads();
   return (int)lds.answer[3];
 }
 
+constexpr int kStaged = 2048;  // summaries kept in LDS: rows of up to 131072 states
+
 template <typename Key>
-struct Candidates {
-  Key key[kCandidates];
-  int32_t index[kCandidates];
-  int32_t listed[kListed];
+struct LongShared {
+  static constexpr int kThreads = kLongThreads;
+  static constexpr int kBins = 4 * kLongThreads;
+  unsigned long long words[kLongThreads / 64];
+  long long answer[4];
+  Key block_key[kStaged];
+  union {
+    double block_sum[kStaged];  // done with before the others are written
+    struct {
+      unsigned long long mass[kBins];
+      uint32_t count[kBins];
+      Key key[kCandidates];
+      int32_t index[kCandidates];
+      int32_t listed[kListed];
+    };
+  };
 };
 
 template <int E, typename Key>
-__device__ __forceinline__ int draw_among(const Candidates<Key>& from, int count, const Setting& s, const Weight& weight,
+__device__ __forceinline__ int draw_among(const LongShared<Key>& lds, int count, const Setting& s, const Weight& weight,
                                           double row_total) {
-  Key key[E];
+  using W = typename std::conditional<sizeof(Key) == 8, double, float>::type;
+  W x[E];
 #pragma unroll
   for (int j = 0; j < E; ++j) {
     const int at = (int)(threadIdx.x & 63) * E + j;
-    key[j] = at < count ? from.key[at] : (Key)0;
+    x[j] = at < count ? KeyOf<W>::value(lds.key[at]) : (W)-INFINITY;
   }
-  return draw_in_group<true, 64, E>(key, s, weight, row_total);
+  return draw_in_group<true, 64, E>(x, count, s, weight, row_total);
 }
 
 // One row, by the whole block, from its summaries; the same answer in every thread: the state, -1, or -2 for
 // a row that is left to draw_wide, with what it needs in `state`.
 template <typename T>
-__device__ int draw_row(const Draws& a, int64_t r, Bins<kLongThreads>& lds, Candidates<KeyType<T>>& from, RowState& state) {
+__device__ int draw_row(const Draws& a, int64_t r, LongShared<KeyType<T>>& lds, RowState& state) {
   using W = typename Value<T>::Wide;
   using Key = KeyType<T>;
   constexpr int THREADS = kLongThreads;
@@ -757,40 +753,61 @@ __device__ int draw_row(const Draws& a, int64_t r, Bins<kLongThreads>& lds, Cand
   const Key* keys = static_cast<const Key*>(a.block_keys) + r * a.blocks_per_row;
   const double* sums = a.block_sums + r * a.sums_per_row;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const bool staged = blocks <= kStaged;
 
-  unsigned long long best = 0;
-  for (int b = threadIdx.x; b < blocks; b += THREADS) best = kMax(best, (unsigned long long)keys[b]);
+  unsigned long long best = 0, least = ~0ull;
+#pragma unroll 8
+  for (int b = threadIdx.x; b < blocks; b += THREADS) {
+    const Key k = keys[b];
+    best = kMax(best, (unsigned long long)k);
+    least = kMin(least, (unsigned long long)k);
+    if (staged) lds.block_key[b] = k;
+  }
   best = block_all<THREADS>(best, lds.words, kMax);
   if ((Key)best == (Key)~(Key)0) return -1;
   const double largest = (double)KeyOf<W>::value((Key)best);
   if (isinf(largest)) return -1;
+  const auto key_of = [&](int b) { return staged ? lds.block_key[b] : keys[b]; };
 
   if (s.temperature == 0.0) {
     unsigned long long block = ~0ull;
     for (int b = threadIdx.x; b < blocks && block == ~0ull; b += THREADS)
-      if ((unsigned long long)keys[b] == best) block = (unsigned long long)b;
+      if (key_of(b) == (Key)best) block = (unsigned long long)b;
     block = block_all<THREADS>(block, lds.words, kMin);
     const int i = (int)block * kBlock + lane;
     const uint64_t hits = __ballot(i < n && key_at(x, std::min(i, n - 1)) == (Key)best);
     return (int)block * kBlock + __ffsll((unsigned long long)hits) - 1;
   }
 
+  // ---- weights of the blocks, where the whole row's counts
   const Weight weight(largest, s.temperature);
-  const auto block_sum_of = [&](int b) { return sums[b] * weight.of_key(keys[b]); };
-  if (!s.has_top_k() && !s.has_top_p() && s.min_p == 0.0)
-    return locate<THREADS, 1>(lds, blocks, s.uniform, block_sum_of, [&](int i) {
-      return i < n ? weight.of_key(key_at(x, std::min(i, n - 1))) : 0.0;
-    });
+  const bool plain = !s.has_top_k() && !s.has_top_p() && s.min_p == 0.0;
+  const int each = (blocks + THREADS - 1) / THREADS;
+  const int begin = std::min((int)threadIdx.x * each, blocks), end = std::min(begin + each, blocks);
+  const auto block_sum_of = [&](int b) { return staged ? lds.block_sum[b] : sums[b] * weight.of_key(keys[b]); };
+  double row_total = -1.0;  // W, where it is the whole row's
+  if (plain || (s.has_top_p() && !s.has_top_k())) {
+    if (staged) {
+#pragma unroll 8
+      for (int b = threadIdx.x; b < blocks; b += THREADS) lds.block_sum[b] = sums[b] * weight.of_key(lds.block_key[b]);
+      __syncthreads();
+    }
+    if (plain)
+      return locate<1>(lds, blocks, s.uniform, block_sum_of, [&](int i) {
+        return i < n ? weight.of_key(key_at(x, std::min(i, n - 1))) : 0.0;
+      });
+    double here = 0.0;
+    for (int b = begin; b < end; ++b) here += block_sum_of(b);
+    (void)block_scan<THREADS>(here, lds.words, &row_total);
+  }
 
   // ---- a floor below which nothing is kept
+  least = block_all<THREADS>(least, lds.words, kMin);
   const double scale = mass_scale(n);
   const auto mass = [&](Key k) { return mass_of(weight.of_key(k), scale); };
   const auto each_block = [&](auto fn) {
-    for (int b = threadIdx.x; b < blocks; b += THREADS) fn(keys[b]);
+    for (int b = threadIdx.x; b < blocks; b += THREADS) fn(key_of(b));
   };
-  unsigned long long least = ~0ull;
-  for (int b = threadIdx.x; b < blocks; b += THREADS) least = kMin(least, (unsigned long long)keys[b]);
-  least = block_all<THREADS>(least, lds.words, kMin);
   Key floor = 1;
   const auto raise_floor = [&](double least_weight) {  // only states of at least this weight are kept
     const double step = s.temperature * log(least_weight);
@@ -798,39 +815,36 @@ __device__ int draw_row(const Draws& a, int64_t r, Bins<kLongThreads>& lds, Cand
     const W bound = (W)(largest + step - 1e-6 * (fabs(largest) + fabs(step) + 1e-6 * s.temperature));
     if (bound < (W)largest && !isinf(bound)) floor = std::max(floor, KeyOf<W>::key(bound));
   };
-  double row_total = -1.0;  // W, where it is the whole row's
   if (s.has_top_k()) {
     // the largest keys of k blocks are k states: the k-th state's key is not below the k-th of them
-    if (s.top_k < blocks)
-      floor = find_bin<false>(lds, each_block, mass, (Key)least, (Key)best, 0ull, (double)s.top_k).low;
+    if (s.top_k < blocks) {
+      KeyRange<Key> range{(Key)least, (Key)best, 0ull, 0ull, true};
+      narrow<false>(lds, range, each_block, mass, (double)s.top_k);
+      floor = range.low;
+    }
   } else if (s.has_top_p()) {
-    double here = 0.0;
-    const int each = (blocks + THREADS - 1) / THREADS;
-    for (int b = (int)threadIdx.x * each; b < std::min((int)(threadIdx.x + 1) * each, blocks); ++b) here += block_sum_of(b);
-    (void)block_scan<THREADS>(here, lds.words, &row_total);
     // the states below (1 - p) W / n hold less than the share that is left out
     raise_floor((1.0 - s.top_p) * row_total / (double)n);
     // and where blocks' largest states hold the share by themselves, nothing below those is kept
-    const Bin<Key> bin = find_bin<true>(lds, each_block, mass, std::max(floor, (Key)least), (Key)best, 0ull,
-                                        s.top_p * row_total * scale * (1.0 + 1e-9));
-    if (bin.reached) floor = std::max(floor, bin.low);
+    KeyRange<Key> range{std::max(floor, (Key)least), (Key)best, 0ull, 0ull, true};
+    narrow<true>(lds, range, each_block, mass, s.top_p * row_total * scale * (1.0 + 1e-9));
+    if (range.reached) floor = std::max(floor, range.low);
   }
   // (with top-k and top-p together W is the weight of all top-k states, those that min-p drops among them)
   if (s.min_p > 0.0 && !(s.has_top_k() && s.has_top_p())) raise_floor(s.min_p);
 
   // ---- few states at or above it: one wave draws among them
-  const int each = (blocks + THREADS - 1) / THREADS;
-  const int begin = std::min((int)threadIdx.x * each, blocks), end = std::min(begin + each, blocks);
   unsigned long long passing = 0, listed;
-  for (int b = begin; b < end; ++b) passing += keys[b] >= floor;
+  for (int b = begin; b < end; ++b) passing += key_of(b) >= floor;
   unsigned long long at = block_scan<THREADS>(passing, lds.words, &listed);
   if (listed <= kListed) {
     for (int b = begin; b < end; ++b)
-      if (keys[b] >= floor) from.listed[at++] = b;
+      if (key_of(b) >= floor) lds.listed[at++] = b;
     __syncthreads();
     // counts per listed block, their prefix sums, then the states in order of their index
+#pragma unroll 4
     for (int q = wave; q < (int)listed; q += THREADS / 64) {
-      const int i = from.listed[q] * kBlock + lane;
+      const int i = lds.listed[q] * kBlock + lane;
       const uint64_t hits = __ballot(i < n && key_at(x, std::min(i, n - 1)) >= floor);
       if (lane == 0) lds.count[q] = (uint32_t)__popcll(hits);
     }
@@ -854,15 +868,16 @@ __device__ int draw_row(const Draws& a, int64_t r, Bins<kLongThreads>& lds, Cand
         }
       }
       __syncthreads();
+#pragma unroll 4
       for (int q = wave; q < (int)listed; q += THREADS / 64) {
-        const int i = from.listed[q] * kBlock + lane;
+        const int i = lds.listed[q] * kBlock + lane;
         const Key k = key_at(x, std::min(i, n - 1));
         const bool hit = i < n && k >= floor;
         const uint64_t hits = __ballot(hit);
         if (hit) {
           const int to = (int)lds.count[q] + __popcll(hits & ((1ull << lane) - 1));
-          from.key[to] = k;
-          from.index[to] = i;
+          lds.key[to] = k;
+          lds.index[to] = i;
         }
       }
       __syncthreads();
@@ -870,12 +885,12 @@ __device__ int draw_row(const Draws& a, int64_t r, Bins<kLongThreads>& lds, Cand
         const int count = (int)candidates;
         int slot;
         if (count <= 64)
-          slot = draw_among<1>(from, count, s, weight, row_total);
+          slot = draw_among<1>(lds, count, s, weight, row_total);
         else if (count <= 256)
-          slot = draw_among<4>(from, count, s, weight, row_total);
+          slot = draw_among<4>(lds, count, s, weight, row_total);
         else
-          slot = draw_among<8>(from, count, s, weight, row_total);
-        if (lane == 0) lds.answer[3] = from.index[slot];
+          slot = draw_among<8>(lds, count, s, weight, row_total);
+        if (lane == 0) lds.answer[3] = lds.index[slot];
       }
       __syncthreads();
       return (int)lds.answer[3];
@@ -886,12 +901,11 @@ __device__ int draw_row(const Draws& a, int64_t r, Bins<kLongThreads>& lds, Cand
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLongThreads, 4) draw_long(const Draws a, int64_t first_row) {
-  __shared__ Bins<kLongThreads> lds;
-  __shared__ Candidates<KeyType<T>> from;
+__global__ void __launch_bounds__(kLongThreads) draw_long(const Draws a, int64_t first_row) {
+  __shared__ LongShared<KeyType<T>> lds;
   const int64_t r = first_row + blockIdx.x;
   RowState state{};
-  const int drawn = draw_row<T>(a, r, lds, from, state);
+  const int drawn = draw_row<T>(a, r, lds, state);
   if (threadIdx.x == 0) {
     if (drawn >= -1) a.out[r] = drawn;
     a.row_states[r] = state;
@@ -900,21 +914,45 @@ __global__ void __launch_bounds__(kLongThreads, 4) draw_long(const Draws a, int6
 
 // ---- long rows that keep many states ----------------------------------------------------------------
 
-// Calls fn(index, key) for all n states of a row in memory.
+// Calls fn(index, logit) for all n states of a row in memory.
 template <typename T, int THREADS, typename Fn>
 __device__ __forceinline__ void for_each_state(const T* x, int n, Fn fn) {
-  using W = typename Value<T>::Wide;
   constexpr int V = Value<T>::kVec;
   const int packs = n / V;
 #pragma unroll 2
   for (int k = threadIdx.x; k < packs; k += THREADS) {
     const Pack<T> p = load_pack(x + k * V);
 #pragma unroll
-    for (int j = 0; j < V; ++j) fn(k * V + j, KeyOf<W>::key(Value<T>::widen(p.v[j])));
+    for (int j = 0; j < V; ++j) fn(k * V + j, Value<T>::widen(p.v[j]));
   }
   const int i = packs * V + (int)threadIdx.x;
-  if (i < n) fn(i, KeyOf<W>::key(Value<T>::widen(x[i])));
+  if (i < n) fn(i, Value<T>::widen(x[i]));
 }
+
+// Bins of equal width in the logit (in the key they would be wide near the maximum, where the weight is, and
+// narrow around 0).  All that lies at or below `low` is in bin 0.
+template <typename W>
+struct Steps {
+  W low, per_bin_inverse;
+  int last;
+  __device__ __forceinline__ Steps(double floor, double best, double temperature, int bins) : last(bins - 1) {
+    // weights are 0 from 750 T below the maximum on
+    low = (W)fmax(floor, best - 750.0 * temperature);
+    if (!(low > -INFINITY)) low = (W)floor;
+    per_bin_inverse = (W)((double)bins / (best - (double)low));
+    if (!(per_bin_inverse > (W)0) || isinf(per_bin_inverse)) per_bin_inverse = 0;
+  }
+  __device__ __forceinline__ int bin(W x) const {
+    return x > low ? (int)fmin((x - low) * per_bin_inverse, (W)last) : 0;
+  }
+  // bounds of the bin's logits, with room for bin()'s roundings (2^-22 of 4096 bins)
+  __device__ __forceinline__ double from(int bin) const {
+    return bin == 0 || per_bin_inverse == (W)0 ? -INFINITY : (double)low + ((double)bin - 0.01) / (double)per_bin_inverse;
+  }
+  __device__ __forceinline__ double to(int bin) const {
+    return bin == last || per_bin_inverse == (W)0 ? INFINITY : (double)low + ((double)bin + 1.01) / (double)per_bin_inverse;
+  }
+};
 
 template <typename Key, int THREADS>
 struct Listed {
@@ -943,11 +981,11 @@ __device__ int last_kept(const T* x, int n, KeyType<T> key, unsigned long long k
       for (uint32_t q = threadIdx.x; q < count; q += THREADS)
         if (list.key[q] == key) fn(~(uint32_t)list.index[q]);
     };
-    Bin<uint32_t> bin{~(uint32_t)n, ~0u, 0ull, 0ull, true};
+    KeyRange<uint32_t> range{~(uint32_t)n, ~0u, 0ull, 0ull, true};
     do {
-      bin = find_bin<false>(lds, each, [](uint32_t) { return 0ull; }, bin.low, bin.high, bin.above, (double)kept);
-    } while (bin.low != bin.high);
-    return (int)~bin.low;
+      narrow<false>(lds, range, each, [](uint32_t) { return 0ull; }, (double)kept);
+    } while (range.low != range.high);
+    return (int)~range.low;
   }
   unsigned long long seen = 0;
   for (int base = 0; base < n && seen < kept; base += THREADS * V) {
@@ -972,7 +1010,7 @@ __device__ int last_kept(const T* x, int n, KeyType<T> key, unsigned long long k
   return (int)lds.answer[0];
 }
 
-// One row by the whole block, over the row in memory: one pass counts its states by key, a second one adds up
+// One row by the whole block, over the row in memory: one pass counts its states by logit, a second one adds up
 // what is certainly kept, and the few thousand states around the threshold are settled in LDS.
 template <typename T, int THREADS>
 __device__ int draw_wide_row(const Draws& a, int64_t r, const RowState& state, Bins<THREADS>& lds,
@@ -987,17 +1025,29 @@ __device__ int draw_wide_row(const Draws& a, int64_t r, const RowState& state, B
   const Setting s = row_setting(a, r);
   const int n = (int)s.n;
   const Key best = (Key)state.best, floor = (Key)state.floor;
-  const Weight weight((double)KeyOf<W>::value(best), s.temperature);
+  const double largest = (double)KeyOf<W>::value(best);
+  const Weight weight(largest, s.temperature);
   const double scale = mass_scale(n);
   const auto mass = [&](Key k) { return mass_of(weight.of_key(k), scale); };
-  const auto no_mass = [](Key) { return 0ull; };
+  const auto no_mass = [](auto) { return 0ull; };
+  const double floor_value = floor == 1 ? -INFINITY : (double)KeyOf<W>::value(floor);
+  const Steps<W> steps(isnan(floor_value) ? -INFINITY : floor_value, largest, s.temperature, kBins);
 
-  const auto fill_list = [&](const Prefix<Key>& in, Key low, Key high) {
+  // the states of a prefix in bins lowest..highest, by key
+  const auto each_in = [&](const Prefix<Key>& in, int lowest, int highest, auto fn) {
+    for_each_state<T, THREADS>(x, n, [&](int i, W v) {
+      const int bin = steps.bin(v);
+      if (bin < lowest || bin > highest) return;
+      const Key k = KeyOf<W>::key(v);
+      if (in.has(i, k)) fn(i, k);
+    });
+  };
+  const auto fill_list = [&](const Prefix<Key>& in, int lowest, int highest, Key low, Key high) {
     __syncthreads();
     if (threadIdx.x == 0) list.count = 0;
     __syncthreads();
-    for_each_state<T, THREADS>(x, n, [&](int i, Key k) {
-      if (k < low || k > high || !in.has(i, k)) return;
+    each_in(in, lowest, highest, [&](int i, Key k) {
+      if (k < low || k > high) return;
       const uint32_t at = atomicAdd(&list.count, 1u);
       list.key[at] = k;
       list.index[at] = i;
@@ -1012,46 +1062,50 @@ __device__ int draw_wide_row(const Draws& a, int64_t r, const RowState& state, B
   // ---- top-k: the k-th key by counting
   Prefix<Key> kept{floor, n};
   if (s.has_top_k()) {
+    const Prefix<Key> all = kept;
     const auto each_state = [&](auto fn) {
-      for_each_state<T, THREADS>(x, n, [&](int, Key k) { fn(k); });
+      for_each_state<T, THREADS>(x, n, [&](int, W v) {
+        if (KeyOf<W>::key(v) >= floor) fn(v);
+      });
     };
-    Bin<Key> bin{floor, best, 0ull, 0ull, true};
-    do {
-      bin = find_bin<false>(lds, each_state, no_mass, bin.low, bin.high, bin.above, (double)s.top_k);
-    } while (bin.low != bin.high && bin.states > kRoom);
-    const bool in_list = bin.states <= kRoom;
+    const Found f = find_bin<false>(lds, each_state, [&](W v) { return steps.bin(v); }, no_mass, 0ull, (double)s.top_k);
+    KeyRange<Key> range{floor, best, f.above, f.states, true};
+    const auto each_key = [&](auto fn) {
+      each_in(all, f.bin, f.bin, [&](int, Key k) { fn(k); });
+    };
+    while (range.low != range.high && range.states > kRoom) narrow<false>(lds, range, each_key, no_mass, (double)s.top_k);
+    const bool in_list = range.states <= kRoom;
     if (in_list) {
-      fill_list(kept, bin.low, bin.high);
-      while (bin.low != bin.high)
-        bin = find_bin<false>(lds, each_listed, no_mass, bin.low, bin.high, bin.above, (double)s.top_k);
+      fill_list(all, f.bin, f.bin, range.low, range.high);
+      while (range.low != range.high) narrow<false>(lds, range, each_listed, no_mass, (double)s.top_k);
     }
-    kept.key = bin.low;
-    const Sum ties = (Sum)s.top_k - bin.above;
-    if (ties < bin.states) kept.last = last_kept<T, THREADS>(x, n, bin.low, ties, lds, list, in_list);
+    kept.key = range.low;
+    const Sum ties = (Sum)s.top_k - range.above;
+    if (ties < range.states) kept.last = last_kept<T, THREADS>(x, n, range.low, ties, lds, list, in_list);
   }
 
   const int segments = (n + 64 * V - 1) / (64 * V);
   double* sums = a.block_sums + r * a.sums_per_row;  // the block sums have served: one entry per segment,
   Sum* extra = reinterpret_cast<Sum*>(sums + segments);  // and what the list adds to it
-  // Weights of the states of a prefix above a key: their sum, and by segments those that min-p leaves.
-  const auto add_up = [&](const Prefix<Key>& in, Key above) {
+  // Weights of the states of a prefix in the bins above one: their sum, and by segments those that min-p leaves.
+  const auto add_up = [&](const Prefix<Key>& in, int above) {
     double all = 0.0;
     for (int q = threadIdx.x >> 6; q < segments; q += THREADS / 64) {
       const int i = (q * 64 + (int)(threadIdx.x & 63)) * V;
       double drawn = 0.0;
-      const auto add = [&](int at, Key k) {
-        if (k <= above || !in.has(at, k)) return;
-        const double w = weight.of_key(k);
+      const auto add = [&](int at, W v) {
+        if (!in.has(at, KeyOf<W>::key(v)) || steps.bin(v) <= above) return;
+        const double w = weight((double)v);
         all += w;
         drawn += w >= s.min_p ? w : 0.0;
       };
       if (i + V <= n) {
         const Pack<T> p = load_pack(x + i);
 #pragma unroll
-        for (int j = 0; j < V; ++j) add(i + j, KeyOf<W>::key(Value<T>::widen(p.v[j])));
+        for (int j = 0; j < V; ++j) add(i + j, Value<T>::widen(p.v[j]));
       } else {
         for (int j = 0; j < V; ++j)
-          if (i + j < n) add(i + j, key_at(x, i + j));
+          if (i + j < n) add(i + j, Value<T>::widen(x[i + j]));
       }
       drawn = lanes_sum<64>(drawn);
       if ((threadIdx.x & 63) == 0) {
@@ -1067,16 +1121,16 @@ __device__ int draw_wide_row(const Draws& a, int64_t r, const RowState& state, B
   constexpr double kListScale = 1125899906842624.0;  // 2^50: at most 4096 weights add up
   bool added = false;
   if (s.has_top_p()) {
-    const double w_all = s.has_top_k() ? add_up(kept, (Key)0) : state.total;
+    const double w_all = s.has_top_k() ? add_up(kept, -1) : state.total;
     const double target = s.top_p * w_all;
-    // counts by key bound the mass from the top: what lies above `high` is kept, what lies below `low` is not
-    const int shift = bin_shift<THREADS>(kept.key, best);
+    // counts by logit bound the mass from the top: what lies above the bins first..last is kept, what lies
+    // below them is not
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < 4; ++b) lds.count[b * THREADS + threadIdx.x] = 0;
     __syncthreads();
-    for_each_state<T, THREADS>(x, n, [&](int i, Key k) {
-      if (kept.has(i, k)) atomicAdd(&lds.count[(int)((k - kept.key) >> shift)], 1u);
+    for_each_state<T, THREADS>(x, n, [&](int i, W v) {
+      if (kept.has(i, KeyOf<W>::key(v))) atomicAdd(&lds.count[steps.bin(v)], 1u);
     });
     __syncthreads();
     double least[4], most[4], least_sum = 0.0, most_sum = 0.0, ignored;
@@ -1086,19 +1140,18 @@ __device__ int draw_wide_row(const Draws& a, int64_t r, const RowState& state, B
       const double count = (double)lds.count[bin];
       least[b] = most[b] = 0.0;
       if (count > 0.0) {
-        const Key low = kept.key + ((Key)bin << shift);
-        least[b] = count * weight.of_key(low);
-        most[b] = count * weight.of_key(bin_high(low, shift, best));
+        least[b] = count * weight(steps.from(bin));
+        most[b] = count * weight(fmin(steps.to(bin), largest));
       }
       least_sum += least[b];
       most_sum += most[b];
     }
     double at_least = block_scan<THREADS>(least_sum, lds.words, &ignored);
     double at_most = block_scan<THREADS>(most_sum, lds.words, &ignored);
-    unsigned int first = ~0u, last = ~0u, lowest = ~0u;
+    uint32_t first = ~0u, last = ~0u, lowest = ~0u;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const unsigned int at = 4 * threadIdx.x + b;
+      const uint32_t at = 4 * threadIdx.x + b;
       at_least += least[b];
       at_most += most[b];
       if (lds.count[kBins - 1 - at] != 0) {
@@ -1107,63 +1160,53 @@ __device__ int draw_wide_row(const Draws& a, int64_t r, const RowState& state, B
         lowest = kBins - 1 - at;
       }
     }
-    first = (unsigned int)block_all<THREADS>((Sum)first, lds.words, kMin);
-    last = (unsigned int)block_all<THREADS>((Sum)last, lds.words, kMin);
-    lowest = kBins - 1 - (unsigned int)block_all<THREADS>((Sum)lowest, lds.words, kMin);
-    if (last > lowest) last = lowest;
-    if (first > last) first = last;
+    const Sum ends = block_all<THREADS>(((Sum)first << 32) | last, lds.words, kMinOfHalves);
+    lowest = kBins - 1 - (uint32_t)block_all<THREADS>((Sum)lowest, lds.words, kMin);
+    last = std::min((uint32_t)ends, lowest);
+    first = std::min((uint32_t)(ends >> 32), last);
+    const int bin_low = kBins - 1 - (int)last, bin_high = kBins - 1 - (int)first;
     Sum around = 0;
-    for (unsigned int at = first + threadIdx.x; at <= last; at += THREADS) around += lds.count[kBins - 1 - at];
+    for (int b = bin_low + (int)threadIdx.x; b <= bin_high; b += THREADS) around += lds.count[b];
     around = block_all<THREADS>(around, lds.words, [](Sum p, Sum q) { return p + q; });
-    Bin<Key> bin;
-    bin.low = kept.key + ((Key)(kBins - 1 - last) << shift);
-    const Key top = kept.key + ((Key)(kBins - 1 - first) << shift);
-    bin.high = bin_high(top, shift, best);
-    bin.states = around;
-    const double certain = add_up(kept, bin.high);
-    bin.above = (Sum)llrint(certain * scale);
+    const double certain = add_up(kept, bin_high);
     const double reach = target * scale;
-    const auto each_in = [&](auto fn) {
-      for_each_state<T, THREADS>(x, n, [&](int i, Key k) {
-        if (kept.has(i, k)) fn(k);
-      });
+    KeyRange<Key> range{kept.key, best, (Sum)llrint(certain * scale), around, true};
+    const auto each_key = [&](auto fn) {
+      each_in(kept, bin_low, bin_high, [&](int, Key k) { fn(k); });
     };
-    while (bin.low != bin.high && bin.states > kRoom)
-      bin = find_bin<true>(lds, each_in, mass, bin.low, bin.high, bin.above, reach);
-    const bool in_list = bin.states <= kRoom;
-    const Key list_high = bin.high;
+    const bool narrowed = around > kRoom;
+    while (range.low != range.high && range.states > kRoom) narrow<true>(lds, range, each_key, mass, reach);
+    const bool in_list = range.states <= kRoom;
     if (in_list) {
-      fill_list(kept, bin.low, bin.high);
+      fill_list(kept, bin_low, bin_high, range.low, range.high);
       do {
-        bin = find_bin<true>(lds, each_listed, mass, bin.low, bin.high, bin.above, reach);
-      } while (bin.low != bin.high);
+        narrow<true>(lds, range, each_listed, mass, reach);
+      } while (range.low != range.high);
     }
     // of the states on the key: those with less than the target before them, one at least
-    const double each = (double)mass(bin.low), above = (double)bin.above;
-    Sum ties = bin.states;
-    if (each > 0.0) ties = (Sum)fmin(fmax(ceil((reach - above) / each), 1.0), (double)bin.states);
+    const double each = (double)mass(range.low), above = (double)range.above;
+    Sum ties = range.states;
+    if (each > 0.0) ties = (Sum)fmin(fmax(ceil((reach - above) / each), 1.0), (double)range.states);
     while (ties > 1 && above + (double)(ties - 1) * each >= reach) --ties;
-    while (ties < bin.states && above + (double)ties * each < reach) ++ties;
-    const int bound = bin.low == kept.key ? kept.last : n;
-    kept.key = bin.low;
-    kept.last = ties < bin.states ? last_kept<T, THREADS>(x, n, bin.low, ties, lds, list, in_list) : bound;
-    if (in_list) {
-      // the segments hold what lies above the first bounds; the list holds the rest, if it begins there
-      added = list_high == bin_high(top, shift, best);
-      if (added) {
-        const uint32_t count = list.count;
-        for (uint32_t q = threadIdx.x; q < count; q += THREADS)
-          if (kept.has(list.index[q], list.key[q])) {
-            const double w = weight.of_key(list.key[q]);
-            if (w >= s.min_p) atomicAdd(&extra[list.index[q] / (64 * V)], mass_of(w, kListScale));
-          }
-        __threadfence();
-      }
+    while (ties < range.states && above + (double)ties * each < reach) ++ties;
+    const int bound = range.low == kept.key ? kept.last : n;
+    kept.key = range.low;
+    kept.last = ties < range.states ? last_kept<T, THREADS>(x, n, range.low, ties, lds, list, in_list) : bound;
+    if (in_list && !narrowed) {
+      // the segments hold what lies above the bins, the list what lies in them
+      const uint32_t count = list.count;
+      for (uint32_t q = threadIdx.x; q < count; q += THREADS)
+        if (kept.has(list.index[q], list.key[q])) {
+          const double w = weight.of_key(list.key[q]);
+          if (w >= s.min_p) atomicAdd(&extra[list.index[q] / (64 * V)], mass_of(w, kListScale));
+        }
+      __threadfence();
+      added = true;
     }
   }
-  if (!added) (void)add_up(kept, (Key)0);
+  if (!added) (void)add_up(kept, -1);
   __syncthreads();
-  return locate<THREADS, V>(
+  return locate<V>(
       lds, segments, s.uniform,
       [&](int q) {
         const Sum more = __hip_atomic_load(&extra[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -1205,6 +1248,16 @@ void launch_short(const Draws& a, hipStream_t s) {
   }
 }
 
+// 16 states per lane take the fewest instructions per row; where that leaves SIMDs (1024) with less than four
+// waves, 4 states per lane make four times as many.
+template <typename T, int G>
+void launch_short_rows(const Draws& a, hipStream_t s) {
+  if (G * 4 <= 64 && a.rows * G < 64 * 4096)
+    launch_short<T, std::min(G * 4, 64), 4>(a, s);
+  else
+    launch_short<T, G, 16>(a, s);
+}
+
 template <typename T>
 void launch_long(const Draws& a, hipStream_t s) {
   constexpr int kPacks = 4;
@@ -1228,12 +1281,11 @@ void launch_long(const Draws& a, hipStream_t s) {
 template <typename T>
 hipError_t launch(const Draws& a, hipStream_t s) {
   if (a.width <= 4) launch_short<T, 1, 4>(a, s);
-  else if (a.width <= 8) launch_short<T, 1, 8>(a, s);
-  else if (a.width <= 16) launch_short<T, 1, 16>(a, s);
-  else if (a.width <= 32) launch_short<T, 2, 16>(a, s);
-  else if (a.width <= 64) launch_short<T, 4, 16>(a, s);
-  else if (a.width <= 128) launch_short<T, 8, 16>(a, s);
-  else if (a.width <= 256) launch_short<T, 16, 16>(a, s);
+  else if (a.width <= 16) launch_short_rows<T, 1>(a, s);
+  else if (a.width <= 32) launch_short_rows<T, 2>(a, s);
+  else if (a.width <= 64) launch_short_rows<T, 4>(a, s);
+  else if (a.width <= 128) launch_short_rows<T, 8>(a, s);
+  else if (a.width <= 256) launch_short_rows<T, 16>(a, s);
   else if (a.width <= 512) launch_short<T, 32, 16>(a, s);
   else if (a.width <= kShortStates) launch_short<T, 64, 16>(a, s);
   else launch_long<T>(a, s);

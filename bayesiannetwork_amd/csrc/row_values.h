@@ -110,6 +110,10 @@ __device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
   return ((uint64_t)lane_xor<MASK>((uint32_t)(v >> 32)) << 32) | lane_xor<MASK>((uint32_t)v);
 }
 template <int MASK>
+__device__ __forceinline__ int lane_xor(int v) {
+  return (int)lane_xor<MASK>((uint32_t)v);
+}
+template <int MASK>
 __device__ __forceinline__ float lane_xor(float v) {
   return __uint_as_float(lane_xor<MASK>(__float_as_uint(v)));
 }

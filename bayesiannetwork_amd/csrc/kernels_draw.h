@@ -171,19 +171,13 @@ __device__ __forceinline__ double Weight::of_key<uint64_t>(uint64_t k) const {
 // ---- lanes ------------------------------------------------------------------------------------
 
 // Exclusive prefix sum over the G lanes of a group, and the group's total.
-template <int G>
-__device__ __forceinline__ double group_scan(double v, double* total) {
-  const int lane = threadIdx.x % G;
-  double upto = v;
-#pragma unroll
-  for (int d = 1; d < G; d <<= 1) {
-    const double left = __shfl_up(upto, d, G);
-    if (lane >= d) upto += left;
-  }
+template <int G, typename U>
+__device__ __forceinline__ U group_scan(U v, U* total) {
+  const U upto = lanes_scan<G>(v);
   *total = __shfl(upto, G - 1, G);
-  const double before = __shfl_up(upto, 1, G);
-  return lane == 0 ? 0.0 : before;
+  return lane_before<G>(upto);
 }
+
 // ---- a row in registers: E states in each of G lanes --------------------------------------------
 
 // a and b in descending order.  (Plain v_max / v_min: fmax would first make NaNs of signalling ones quiet,
@@ -315,13 +309,7 @@ __device__ int draw_in_group(const W (&x)[E], int count, const Setting& s, const
   if (FILTER) {  // ties are kept in the order of their slots
 #pragma unroll
     for (int j = 0; j < E; ++j) on_threshold += x[j] == threshold;
-    int upto = on_threshold;
-#pragma unroll
-    for (int d = 1; d < G; d <<= 1) {
-      const int left = __shfl_up(upto, d, G);
-      if (lane >= d) upto += left;
-    }
-    on_threshold = upto - on_threshold;  // in the lanes before
+    on_threshold = lanes_scan<G>(on_threshold) - on_threshold;  // in the lanes before
   }
   double w[E], here = 0.0, all;
 #pragma unroll
@@ -500,8 +488,7 @@ struct Bins {
 template <int THREADS, typename U, typename Combine>
 __device__ __forceinline__ U block_all(U v, unsigned long long* lds, Combine combine) {
   static_assert(sizeof(U) == 8, "one word per wave");
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v = combine(v, (U)__shfl_xor(v, d, 64));
+  v = lanes_all<64>(v, combine);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) reinterpret_cast<U*>(lds)[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -524,12 +511,7 @@ template <int THREADS, typename U>
 __device__ __forceinline__ U block_scan(U v, unsigned long long* lds, U* total) {
   static_assert(sizeof(U) == 8, "one word per wave");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  U upto = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const U left = (U)__shfl_up(upto, d, 64);
-    if (lane >= d) upto += left;
-  }
+  const U upto = lanes_scan<64>(v);
   __syncthreads();
   if (lane == 63) reinterpret_cast<U*>(lds)[wave] = upto;
   __syncthreads();
@@ -540,9 +522,7 @@ __device__ __forceinline__ U block_scan(U v, unsigned long long* lds, U* total) 
     sum += reinterpret_cast<U*>(lds)[w];
   }
   *total = sum;
-  U before = (U)__shfl_up(upto, 1, 64);
-  if (lane == 0) before = 0;
-  return base + before;
+  return base + lane_before<64>(upto);
 }
 
 // A weight as an integer: times a power of two that lets n of them add up within 62 bits and one be rounded
@@ -945,13 +925,6 @@ struct Steps {
   __device__ __forceinline__ int bin(W x) const {
     return x > low ? (int)fmin((x - low) * per_bin_inverse, (W)last) : 0;
   }
-  // bounds of the bin's logits, with room for bin()'s roundings (2^-22 of 4096 bins)
-  __device__ __forceinline__ double from(int bin) const {
-    return bin == 0 || per_bin_inverse == (W)0 ? -INFINITY : (double)low + ((double)bin - 0.01) / (double)per_bin_inverse;
-  }
-  __device__ __forceinline__ double to(int bin) const {
-    return bin == last || per_bin_inverse == (W)0 ? INFINITY : (double)low + ((double)bin + 1.01) / (double)per_bin_inverse;
-  }
 };
 
 template <typename Key, int THREADS>
@@ -1090,22 +1063,34 @@ __device__ int draw_wide_row(const Draws& a, int64_t r, const RowState& state, B
   // Weights of the states of a prefix in the bins above one: their sum, and by segments those that min-p leaves.
   const auto add_up = [&](const Prefix<Key>& in, int above) {
     double all = 0.0;
-    for (int q = threadIdx.x >> 6; q < segments; q += THREADS / 64) {
+    const auto load = [&](int q) {
+      const int i = (q * 64 + (int)(threadIdx.x & 63)) * V;
+      Pack<T> p;
+      if (i + V <= n) {
+        p = load_pack(x + i);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) p.v[j] = i + j < n ? x[i + j] : Value<T>::round(-INFINITY);
+      }
+      return raw_of(p);
+    };
+    int q = threadIdx.x >> 6;
+    Raw next = load(q);  // the segment after this one is on its way while this one is worked on
+    for (; q < segments; q += THREADS / 64) {
+      Raw raw = next;
+      next = load(q + THREADS / 64);
+      bn_rows::kept(raw);
+      const Pack<T> p = pack_of<T>(raw);
       const int i = (q * 64 + (int)(threadIdx.x & 63)) * V;
       double drawn = 0.0;
-      const auto add = [&](int at, W v) {
-        if (!in.has(at, KeyOf<W>::key(v)) || steps.bin(v) <= above) return;
-        const double w = weight((double)v);
-        all += w;
-        drawn += w >= s.min_p ? w : 0.0;
-      };
-      if (i + V <= n) {
-        const Pack<T> p = load_pack(x + i);
 #pragma unroll
-        for (int j = 0; j < V; ++j) add(i + j, Value<T>::widen(p.v[j]));
-      } else {
-        for (int j = 0; j < V; ++j)
-          if (i + j < n) add(i + j, Value<T>::widen(x[i + j]));
+      for (int j = 0; j < V; ++j) {
+        const W v = Value<T>::widen(p.v[j]);
+        if (in.has(i + j, KeyOf<W>::key(v)) && steps.bin(v) > above) {
+          const double w = weight((double)v);
+          all += w;
+          drawn += w >= s.min_p ? w : 0.0;
+        }
       }
       drawn = lanes_sum<64>(drawn);
       if ((threadIdx.x & 63) == 0) {
@@ -1123,40 +1108,45 @@ __device__ int draw_wide_row(const Draws& a, int64_t r, const RowState& state, B
   if (s.has_top_p()) {
     const double w_all = s.has_top_k() ? add_up(kept, -1) : state.total;
     const double target = s.top_p * w_all;
-    // counts by logit bound the mass from the top: what lies above the bins first..last is kept, what lies
-    // below them is not
+    // Masses by logit, from weights of single precision, tell the bins around the threshold: what lies above
+    // these is kept, what lies below is not.  Three roundings of the exponent t make a weight wrong by
+    // 3 * 2^-24 * ln 2 * |t|, the exponential itself by 2^-22; a sum that starts with the largest weight, 1, has a
+    // mean |t| of 25 at most (2^24 states of weight 2^-24 double it), so it is off by less than 4e-6 of
+    // itself, a fifth of kSlack, and by the integers' rounding.
     __syncthreads();
-#pragma unroll
-    for (int b = 0; b < 4; ++b) lds.count[b * THREADS + threadIdx.x] = 0;
-    __syncthreads();
-    for_each_state<T, THREADS>(x, n, [&](int i, W v) {
-      if (kept.has(i, KeyOf<W>::key(v))) atomicAdd(&lds.count[steps.bin(v)], 1u);
-    });
-    __syncthreads();
-    double least[4], most[4], least_sum = 0.0, most_sum = 0.0, ignored;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const int bin = kBins - 1 - 4 * (int)threadIdx.x - b;
-      const double count = (double)lds.count[bin];
-      least[b] = most[b] = 0.0;
-      if (count > 0.0) {
-        least[b] = count * weight(steps.from(bin));
-        most[b] = count * weight(fmin(steps.to(bin), largest));
-      }
-      least_sum += least[b];
-      most_sum += most[b];
+      lds.count[b * THREADS + threadIdx.x] = 0;
+      lds.mass[b * THREADS + threadIdx.x] = 0;
     }
-    double at_least = block_scan<THREADS>(least_sum, lds.words, &ignored);
-    double at_most = block_scan<THREADS>(most_sum, lds.words, &ignored);
+    __syncthreads();
+    constexpr double kRoughScale = 274877906944.0;  // 2^38: 2^24 weights add up within 62 bits
+    constexpr double kSlack = 2e-5;
+    const double rough_error = (double)n + 1.0;
+    const float rate = (float)weight.rate;
+    for_each_state<T, THREADS>(x, n, [&](int i, W v) {
+      if (!kept.has(i, KeyOf<W>::key(v))) return;
+      const int bin = steps.bin(v);
+      const float rough = __builtin_amdgcn_exp2f((float)((double)v - largest) * rate);
+      atomicAdd(&lds.count[bin], 1u);
+      atomicAdd(&lds.mass[bin], mass_of((double)rough, kRoughScale));
+    });
+    __syncthreads();
+    Sum own[4], own_sum = 0, ignored;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      own[b] = lds.mass[kBins - 1 - 4 * (int)threadIdx.x - b];
+      own_sum += own[b];
+    }
+    Sum upto = block_scan<THREADS>(own_sum, lds.words, &ignored);
     uint32_t first = ~0u, last = ~0u, lowest = ~0u;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       const uint32_t at = 4 * threadIdx.x + b;
-      at_least += least[b];
-      at_most += most[b];
+      upto += own[b];
       if (lds.count[kBins - 1 - at] != 0) {
-        if (first == ~0u && at_most >= target * (1.0 - 1e-9)) first = at;
-        if (last == ~0u && at_least >= target * (1.0 + 1e-9)) last = at;
+        if (first == ~0u && (double)upto * (1.0 + kSlack) + rough_error >= target * kRoughScale) first = at;
+        if (last == ~0u && (double)upto * (1.0 - kSlack) - rough_error >= target * kRoughScale) last = at;
         lowest = kBins - 1 - at;
       }
     }

@@ -93,17 +93,29 @@ __device__ __forceinline__ void kept(Raw& r) {
   for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(r.w[i]));
 }
 
-// A 32-bit word of the lane whose number differs by MASK: quad permutations and mirrors within the register
-// file for the masks that have one, the LDS crossbar for the rest.
+// A 32-bit word of the lane whose number differs by MASK, by permutations within the register file: quads and
+// mirrors of 8 and 16 lanes, exchanged rows of 16 and halves of 32.  (Through the LDS crossbar each of these
+// waits some hundred cycles, and sorts and reductions are chains of them.)
 template <int MASK>
 __device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
   if constexpr (MASK == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true);
   else if constexpr (MASK == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true);
   else if constexpr (MASK == 3) return __builtin_amdgcn_mov_dpp(v, 0x1B, 0xF, 0xF, true);
   else if constexpr (MASK == 7) return __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, true);
+  else if constexpr (MASK == 4) return lane_xor<3>(lane_xor<7>(v));
   else if constexpr (MASK == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, true);
   else if constexpr (MASK == 15) return __builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, true);
-  else return (uint32_t)__shfl_xor((int)v, MASK, 64);
+  else if constexpr (MASK == 16) {
+    const auto both = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return (threadIdx.x & 16) ? both[0] : both[1];
+  } else if constexpr (MASK == 31) return lane_xor<16>(lane_xor<15>(v));
+  else if constexpr (MASK == 32) {
+    const auto both = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return (threadIdx.x & 32) ? both[0] : both[1];
+  } else {
+    static_assert(MASK == 63, "a permutation that the sorts and reductions use");
+    return lane_xor<32>(lane_xor<31>(v));
+  }
 }
 template <int MASK>
 __device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
@@ -116,6 +128,10 @@ __device__ __forceinline__ int lane_xor(int v) {
 template <int MASK>
 __device__ __forceinline__ float lane_xor(float v) {
   return __uint_as_float(lane_xor<MASK>(__float_as_uint(v)));
+}
+template <int MASK>
+__device__ __forceinline__ unsigned long long lane_xor(unsigned long long v) {
+  return (unsigned long long)lane_xor<MASK>((uint64_t)v);
 }
 template <int MASK>
 __device__ __forceinline__ double lane_xor(double v) {
@@ -141,6 +157,46 @@ __device__ __forceinline__ W lanes_max(W v) {
 template <int WIDTH, typename W>
 __device__ __forceinline__ W lanes_sum(W v) {
   return lanes_all<WIDTH>(v, [](W p, W q) { return p + q; });
+}
+
+// Inclusive prefix sums over groups of WIDTH lanes: within rows of 16 lanes by shifts, then each row's last
+// lane to the rows behind it.
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ uint32_t lanes_shifted(uint32_t v) {
+  return __builtin_amdgcn_update_dpp(0u, v, CONTROL, ROWS, 0xF, false);  // 0 where no lane is shifted in
+}
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ int lanes_shifted(int v) {
+  return (int)lanes_shifted<CONTROL, ROWS>((uint32_t)v);
+}
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ unsigned long long lanes_shifted(unsigned long long v) {
+  return ((unsigned long long)lanes_shifted<CONTROL, ROWS>((uint32_t)(v >> 32)) << 32) |
+         lanes_shifted<CONTROL, ROWS>((uint32_t)v);
+}
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ double lanes_shifted(double v) {
+  return __longlong_as_double((long long)lanes_shifted<CONTROL, ROWS>((unsigned long long)__double_as_longlong(v)));
+}
+template <int WIDTH, typename U>
+__device__ __forceinline__ U lanes_scan(U v) {
+  const int lane = threadIdx.x % WIDTH;
+  const auto add = [&](U left, int distance) {
+    if (WIDTH >= 16 || lane >= distance) v += left;  // narrower groups do not end with their row
+  };
+  if constexpr (WIDTH >= 2) add(lanes_shifted<0x111, 0xF>(v), 1);
+  if constexpr (WIDTH >= 4) add(lanes_shifted<0x112, 0xF>(v), 2);
+  if constexpr (WIDTH >= 8) add(lanes_shifted<0x114, 0xF>(v), 4);
+  if constexpr (WIDTH >= 16) add(lanes_shifted<0x118, 0xF>(v), 8);
+  if constexpr (WIDTH >= 32) add(lanes_shifted<0x142, 0xA>(v), 16);
+  if constexpr (WIDTH >= 64) add(lanes_shifted<0x143, 0xC>(v), 32);
+  return v;
+}
+// The value of the lane before, 0 in a group's first.
+template <int WIDTH, typename U>
+__device__ __forceinline__ U lane_before(U v) {
+  const U left = lanes_shifted<0x138, 0xF>(v);
+  return threadIdx.x % WIDTH == 0 ? (U)0 : left;
 }
 
 }  // namespace bn_rows

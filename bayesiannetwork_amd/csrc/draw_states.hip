@@ -36,8 +36,12 @@ int check_draws(int dtype, const Draws& a) {
   return BN_OK;
 }
 
-// Workspace of long rows: block sums, row states and block keys of all rows.
+// Workspace of long rows: block sums, row states and piece keys of all rows.
 int64_t blocks_per_row(int64_t num_states) { return num_states <= kShortStates ? 0 : (num_states + kBlock - 1) / kBlock; }
+int64_t pieces_per_row(int64_t num_states) {
+  const int64_t piece = piece_states(num_states);
+  return num_states <= kShortStates ? 0 : (num_states + piece - 1) / piece;
+}
 
 }  // namespace
 
@@ -48,7 +52,7 @@ int64_t bn_draw_states_workspace_bytes(int dtype, int64_t rows, int64_t num_stat
   const int64_t key_bytes = dtype == BN_F64 ? 8 : 4;
   const int64_t blocks = blocks_per_row(num_states);
   if (blocks == 0) return 0;
-  return rows * ((blocks + 2) * (int64_t)sizeof(double) + (int64_t)sizeof(RowState) + blocks * key_bytes);
+  return rows * ((blocks + 2) * (int64_t)sizeof(double) + (int64_t)sizeof(RowState) + pieces_per_row(num_states) * key_bytes);
 }
 
 int bn_draw_states(int dtype, const void* logits_dev, int64_t rows, int64_t num_states, int64_t row_stride,
@@ -69,17 +73,17 @@ int bn_draw_states(int dtype, const void* logits_dev, int64_t rows, int64_t num_
   if (uniform_dtype != BN_F32 && uniform_dtype != BN_F64)
     return fail(BN_ERR_INVALID, "uniform_dtype must be BN_F32 or BN_F64");
   if (rows == 0) return BN_OK;
-  a.blocks_per_row = blocks_per_row(num_states);
-  if (!logits_dev || !uniforms_dev || !out_dev || (a.blocks_per_row > 0 && !workspace_dev))
+  a.pieces_per_row = pieces_per_row(num_states);
+  if (!logits_dev || !uniforms_dev || !out_dev || (a.pieces_per_row > 0 && !workspace_dev))
     return fail(BN_ERR_INVALID, "null argument");
   if (reinterpret_cast<uintptr_t>(logits_dev) % dtype_bytes(dtype))
     return fail(BN_ERR_INVALID, "row address not aligned to its type");
   if (reinterpret_cast<uintptr_t>(workspace_dev) % 8) return fail(BN_ERR_INVALID, "workspace not aligned to 8 bytes");
-  if (a.blocks_per_row > 0) {
-    a.sums_per_row = a.blocks_per_row + 2;
+  if (a.pieces_per_row > 0) {
+    a.sums_per_row = blocks_per_row(num_states) + 2;
     a.block_sums = static_cast<double*>(workspace_dev);
     a.row_states = reinterpret_cast<RowState*>(a.block_sums + rows * a.sums_per_row);
-    a.block_keys = a.row_states + rows;
+    a.piece_keys = a.row_states + rows;
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {

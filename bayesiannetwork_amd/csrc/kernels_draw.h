@@ -8,15 +8,14 @@
 // P and K are prefixes of the order: a row's kept states are those above a threshold, a key (the logit
 // as an integer that sorts like it) and, among the states on that key, an index.
 //
-// Rows of up to 1024 states live in the registers of a group of 1 to 64 lanes, 16 states per lane, and
-// are sorted there (draw_short).  Longer rows take two launches.  The first (block_summaries) reads the
-// logits once, all rows cut over the whole GPU, and leaves of every 64 states the largest key and, where
-// a row's total weight will be needed, their weight relative to it.  The second (draw_long, a block per
-// row) works on those: without filters the prefix sums of 1/64 of the row lead to the 64 states that are
-// looked at again; with filters the largest keys of the 64s bound the threshold from below (the k largest
-// of them are k states of the row), and only the 64s that reach the bound are read again.  Where more
-// than 1024 states pass the bound, the threshold is found by counts and weights in bins of keys, 12 bits
-// of the key at a time.
+// Rows of up to 2048 states live in the registers of a group of 1 to 64 lanes, 16 states per lane (32 beyond
+// 1024), and are sorted there (draw_short).  Longer rows take two launches.  The first (block_summaries) reads
+// the logits once, all rows cut over the whole GPU, and leaves of every 64 states the largest key (up to 16384
+// states: of every 16) and, where a row's total weight will be needed, their weight relative to it.  The second
+// (draw_long, a block per row) works on those: without filters the prefix sums of 1/64 of the row lead to the 64
+// states that are looked at again; with filters the largest keys bound the threshold from below (the k largest
+// of them are k states of the row), and only the pieces that reach the bound are read again.  Rows that have
+// more than 512 states above the bound are left to a third launch (draw_wide).
 //
 // Cumulative weights decide indices, so weights are doubles everywhere, summed in an order that depends
 // on the row alone.  Bins are filled by atomics, whose order varies: they add integers (the weight times a
@@ -84,9 +83,9 @@ struct Draws {
   // long rows: the workspace
   double* block_sums;     // [rows][sums_per_row]
   RowState* row_states;   // [rows]
-  void* block_keys;       // [rows][blocks_per_row]
-  int64_t blocks_per_row;
-  int64_t sums_per_row;   // two more: draw_wide's segments, of 128 states at least, take two entries each
+  void* piece_keys;       // [rows][pieces_per_row]
+  int64_t pieces_per_row;
+  int64_t sums_per_row;   // blocks and two more: draw_wide's segments, of 128 states at least, take two entries each
   int32_t* out;
 };
 
@@ -393,70 +392,78 @@ __global__ void __launch_bounds__(kShortThreads) draw_short(const Draws a, int64
   if (lane == 0) a.out[r] = valid ? pick : -1;
 }
 
-// ---- long rows: summaries of 64 states -----------------------------------------------------------
+// ---- long rows: summaries ------------------------------------------------------------------------
 
-constexpr int kBlock = 64;          // states per summary
-constexpr int kShortStates = 1024;  // rows beyond this are long
+constexpr int kBlock = 64;          // states whose weights are added up
+constexpr int kShortStates = 2048;  // rows beyond this are long
 constexpr int kSummaryThreads = 256;
 
-// A wave summarises V blocks per pack (64 lanes of V states), kPacks packs at a time.
-template <typename T, int PACKS>
+// States that a largest key is kept of: the fewer, the closer the floor that the keys give, and up to 16384
+// states there are few blocks.
+constexpr int64_t kSmallPieceStates = 16384;
+inline int piece_states(int64_t num_states) { return num_states <= kSmallPieceStates ? 16 : kBlock; }
+
+// A wave summarises V blocks per pack (64 lanes of V states), PACKS packs at a time.
+template <typename T, int PIECE, int PACKS>
 __global__ void __launch_bounds__(kSummaryThreads) block_summaries(const Draws a, int64_t tiles_per_row) {
   using W = typename Value<T>::Wide;
   using Key = KeyType<T>;
   constexpr int V = Value<T>::kVec;
-  constexpr int kLanes = kBlock / V;  // lanes of a block
-  constexpr int64_t kWaveStates = 64 * V;
-  constexpr int64_t kTile = kWaveStates * PACKS * (kSummaryThreads / 64);
+  constexpr int kLanes = kBlock / V, kPieceLanes = PIECE / V;
+  constexpr int kWaveStates = 64 * V;
+  constexpr int kTile = kWaveStates * PACKS * (kSummaryThreads / 64);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t tiles = a.rows * tiles_per_row;
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int64_t r = tile / tiles_per_row;
-    const int64_t start = (tile - r * tiles_per_row) * kTile + wave * kWaveStates * PACKS;
-    const int64_t n = row_states(a, r);
+    const int start = (int)(tile - r * tiles_per_row) * kTile + wave * kWaveStates * PACKS;
+    const int n = (int)row_states(a, r);
     if (start >= n) continue;
     const T* x = static_cast<const T*>(a.logits) + r * a.stride;
     const Setting s = row_setting(a, r);
     // top-k draws from the k largest alone; greedy rows need no weights at all
     const bool sums = !s.has_top_k() && s.temperature > 0.0;
-    Key* keys = static_cast<Key*>(a.block_keys) + r * a.blocks_per_row;
-    W v[PACKS][V];
+    Key* keys = static_cast<Key*>(a.piece_keys) + r * a.pieces_per_row;
+    Raw raw[PACKS];
 #pragma unroll
     for (int k = 0; k < PACKS; ++k) {
-      const int64_t i = start + k * kWaveStates + lane * V;
+      const int i = start + k * kWaveStates + lane * V;
       if (i + V <= n) {
-        const Pack<T> p = load_pack(x + i);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[k][j] = Value<T>::widen(p.v[j]);
+        raw[k] = raw_of(load_pack(x + i));
       } else {
+        Pack<T> p;
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[k][j] = i + j < n ? Value<T>::widen(x[i + j]) : (W)-INFINITY;
+        for (int j = 0; j < V; ++j) p.v[j] = i + j < n ? x[i + j] : Value<T>::round(-INFINITY);
+        raw[k] = raw_of(p);
       }
     }
 #pragma unroll
     for (int k = 0; k < PACKS; ++k) {
-      const int64_t i = start + k * kWaveStates + lane * V;
-      bool bad = false;
-      W best = v[k][0];
+      const int i = start + k * kWaveStates + lane * V;
+      bn_rows::kept(raw[k]);
+      const Pack<T> p = pack_of<T>(raw[k]);
+      W v[V];
+      bool spoilt = false;
+      W best = -INFINITY;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        bad |= undrawable(v[k][j]);
-        best = fmax(best, v[k][j]);
+        v[j] = Value<T>::widen(p.v[j]);
+        best = fmax(best, v[j]);
+        spoilt |= undrawable(v[j]);
       }
-      best = lanes_max<kLanes>(best);
-      const uint64_t bad_lanes = __ballot(bad) >> (lane & ~(kLanes - 1));
-      bad = (bad_lanes & ((kLanes == 64 ? 0ull : (1ull << kLanes)) - 1)) != 0;
-      double sum = 0.0;
+      best = lanes_max<kPieceLanes>(best);
+      const uint64_t bad_lanes = __ballot(spoilt) >> (lane & ~(kPieceLanes - 1));
+      const bool bad = (bad_lanes & ((1ull << kPieceLanes) - 1)) != 0;
+      // the largest key there is marks a piece that makes its row undrawable
+      if (lane % kPieceLanes == 0 && i < n) keys[i / PIECE] = bad ? (Key)~(Key)0 : KeyOf<W>::key(best);
       if (sums) {
-        const Weight weight(isinf(best) || bad ? 0.0 : (double)best, s.temperature);
+        if constexpr (PIECE < kBlock) best = lanes_max<kLanes>(best);
+        const Weight weight(isinf(best) ? 0.0 : (double)best, s.temperature);
+        double sum = 0.0;
 #pragma unroll
-        for (int j = 0; j < V; ++j) sum += weight((double)v[k][j]);
+        for (int j = 0; j < V; ++j) sum += weight((double)v[j]);
         sum = lanes_sum<kLanes>(sum);
-      }
-      if (lane % kLanes == 0 && i < n) {
-        // the largest key there is marks a block that makes its row undrawable
-        keys[i / kBlock] = bad ? (Key)~(Key)0 : KeyOf<W>::key(best);
-        if (sums) a.block_sums[r * a.sums_per_row + i / kBlock] = sum;
+        if (lane % kLanes == 0 && i < n) a.block_sums[r * a.sums_per_row + i / kBlock] = sum;
       }
     }
   }
@@ -684,7 +691,7 @@ __device__ int locate(Lds& lds, int segments, double uniform, SumOf sum_of, Weig
   return (int)lds.answer[3];
 }
 
-constexpr int kStaged = 2048;  // summaries kept in LDS: rows of up to 131072 states
+constexpr int kStaged = 2048;  // summaries kept in LDS: all of a row of up to 131072 states
 
 template <typename Key>
 struct LongShared {
@@ -692,7 +699,7 @@ struct LongShared {
   static constexpr int kBins = 4 * kLongThreads;
   unsigned long long words[kLongThreads / 64];
   long long answer[4];
-  Key block_key[kStaged];
+  Key piece_key[kStaged];
   union {
     double block_sum[kStaged];  // done with before the others are written
     struct {
@@ -720,56 +727,62 @@ __device__ __forceinline__ int draw_among(const LongShared<Key>& lds, int count,
 
 // One row, by the whole block, from its summaries; the same answer in every thread: the state, -1, or -2 for
 // a row that is left to draw_wide, with what it needs in `state`.
-template <typename T>
+template <typename T, int PIECE>
 __device__ int draw_row(const Draws& a, int64_t r, LongShared<KeyType<T>>& lds, RowState& state) {
   using W = typename Value<T>::Wide;
   using Key = KeyType<T>;
+  constexpr int V = Value<T>::kVec;
   constexpr int THREADS = kLongThreads;
   const T* x = static_cast<const T*>(a.logits) + r * a.stride;
   const Setting s = row_setting(a, r);
   if (!s.valid) return -1;
   const int n = (int)s.n;
-  const int blocks = (n + kBlock - 1) / kBlock;
-  const Key* keys = static_cast<const Key*>(a.block_keys) + r * a.blocks_per_row;
+  const int pieces = (n + PIECE - 1) / PIECE, blocks = (n + kBlock - 1) / kBlock;
+  const Key* keys = static_cast<const Key*>(a.piece_keys) + r * a.pieces_per_row;
   const double* sums = a.block_sums + r * a.sums_per_row;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const bool staged = blocks <= kStaged;
+  const bool staged = pieces <= kStaged;
 
   unsigned long long best = 0, least = ~0ull;
 #pragma unroll 8
-  for (int b = threadIdx.x; b < blocks; b += THREADS) {
+  for (int b = threadIdx.x; b < pieces; b += THREADS) {
     const Key k = keys[b];
     best = kMax(best, (unsigned long long)k);
     least = kMin(least, (unsigned long long)k);
-    if (staged) lds.block_key[b] = k;
+    if (staged) lds.piece_key[b] = k;
   }
   best = block_all<THREADS>(best, lds.words, kMax);
   if ((Key)best == (Key)~(Key)0) return -1;
   const double largest = (double)KeyOf<W>::value((Key)best);
   if (isinf(largest)) return -1;
-  const auto key_of = [&](int b) { return staged ? lds.block_key[b] : keys[b]; };
+  const auto key_of = [&](int b) { return staged ? lds.piece_key[b] : keys[b]; };
 
   if (s.temperature == 0.0) {
-    unsigned long long block = ~0ull;
-    for (int b = threadIdx.x; b < blocks && block == ~0ull; b += THREADS)
-      if (key_of(b) == (Key)best) block = (unsigned long long)b;
-    block = block_all<THREADS>(block, lds.words, kMin);
-    const int i = (int)block * kBlock + lane;
+    unsigned long long piece = ~0ull;
+    for (int b = threadIdx.x; b < pieces && piece == ~0ull; b += THREADS)
+      if (key_of(b) == (Key)best) piece = (unsigned long long)b;
+    piece = block_all<THREADS>(piece, lds.words, kMin);
+    const int i = (int)piece * PIECE + lane % PIECE;
     const uint64_t hits = __ballot(i < n && key_at(x, std::min(i, n - 1)) == (Key)best);
-    return (int)block * kBlock + __ffsll((unsigned long long)hits) - 1;
+    return (int)piece * PIECE + __ffsll((unsigned long long)hits) - 1;
   }
 
   // ---- weights of the blocks, where the whole row's counts
   const Weight weight(largest, s.temperature);
   const bool plain = !s.has_top_k() && !s.has_top_p() && s.min_p == 0.0;
-  const int each = (blocks + THREADS - 1) / THREADS;
-  const int begin = std::min((int)threadIdx.x * each, blocks), end = std::min(begin + each, blocks);
-  const auto block_sum_of = [&](int b) { return staged ? lds.block_sum[b] : sums[b] * weight.of_key(keys[b]); };
+  const auto block_weight = [&](int b) {  // a block's sum is relative to its largest state
+    Key k = key_of(b * (kBlock / PIECE));
+#pragma unroll
+    for (int q = 1; q < kBlock / PIECE; ++q)
+      if (b * (kBlock / PIECE) + q < pieces) k = std::max(k, key_of(b * (kBlock / PIECE) + q));
+    return sums[b] * weight.of_key(k);
+  };
+  const auto block_sum_of = [&](int b) { return staged ? lds.block_sum[b] : block_weight(b); };
   double row_total = -1.0;  // W, where it is the whole row's
   if (plain || (s.has_top_p() && !s.has_top_k())) {
     if (staged) {
 #pragma unroll 8
-      for (int b = threadIdx.x; b < blocks; b += THREADS) lds.block_sum[b] = sums[b] * weight.of_key(lds.block_key[b]);
+      for (int b = threadIdx.x; b < blocks; b += THREADS) lds.block_sum[b] = block_weight(b);
       __syncthreads();
     }
     if (plain)
@@ -777,7 +790,8 @@ __device__ int draw_row(const Draws& a, int64_t r, LongShared<KeyType<T>>& lds, 
         return i < n ? weight.of_key(key_at(x, std::min(i, n - 1))) : 0.0;
       });
     double here = 0.0;
-    for (int b = begin; b < end; ++b) here += block_sum_of(b);
+    const int each = (blocks + THREADS - 1) / THREADS;
+    for (int b = (int)threadIdx.x * each; b < std::min((int)(threadIdx.x + 1) * each, blocks); ++b) here += block_sum_of(b);
     (void)block_scan<THREADS>(here, lds.words, &row_total);
   }
 
@@ -785,8 +799,8 @@ __device__ int draw_row(const Draws& a, int64_t r, LongShared<KeyType<T>>& lds, 
   least = block_all<THREADS>(least, lds.words, kMin);
   const double scale = mass_scale(n);
   const auto mass = [&](Key k) { return mass_of(weight.of_key(k), scale); };
-  const auto each_block = [&](auto fn) {
-    for (int b = threadIdx.x; b < blocks; b += THREADS) fn(key_of(b));
+  const auto each_piece = [&](auto fn) {
+    for (int b = threadIdx.x; b < pieces; b += THREADS) fn(key_of(b));
   };
   Key floor = 1;
   const auto raise_floor = [&](double least_weight) {  // only states of at least this weight are kept
@@ -796,24 +810,26 @@ __device__ int draw_row(const Draws& a, int64_t r, LongShared<KeyType<T>>& lds, 
     if (bound < (W)largest && !isinf(bound)) floor = std::max(floor, KeyOf<W>::key(bound));
   };
   if (s.has_top_k()) {
-    // the largest keys of k blocks are k states: the k-th state's key is not below the k-th of them
-    if (s.top_k < blocks) {
+    // the largest keys of k pieces are k states: the k-th state's key is not below the k-th of them
+    if (s.top_k < pieces) {
       KeyRange<Key> range{(Key)least, (Key)best, 0ull, 0ull, true};
-      narrow<false>(lds, range, each_block, mass, (double)s.top_k);
+      narrow<false>(lds, range, each_piece, mass, (double)s.top_k);
       floor = range.low;
     }
   } else if (s.has_top_p()) {
     // the states below (1 - p) W / n hold less than the share that is left out
     raise_floor((1.0 - s.top_p) * row_total / (double)n);
-    // and where blocks' largest states hold the share by themselves, nothing below those is kept
+    // and where pieces' largest states hold the share by themselves, nothing below those is kept
     KeyRange<Key> range{std::max(floor, (Key)least), (Key)best, 0ull, 0ull, true};
-    narrow<true>(lds, range, each_block, mass, s.top_p * row_total * scale * (1.0 + 1e-9));
+    narrow<true>(lds, range, each_piece, mass, s.top_p * row_total * scale * (1.0 + 1e-9));
     if (range.reached) floor = std::max(floor, range.low);
   }
   // (with top-k and top-p together W is the weight of all top-k states, those that min-p drops among them)
   if (s.min_p > 0.0 && !(s.has_top_k() && s.has_top_p())) raise_floor(s.min_p);
 
   // ---- few states at or above it: one wave draws among them
+  const int each = (pieces + THREADS - 1) / THREADS;
+  const int begin = std::min((int)threadIdx.x * each, pieces), end = std::min(begin + each, pieces);
   unsigned long long passing = 0, listed;
   for (int b = begin; b < end; ++b) passing += key_of(b) >= floor;
   unsigned long long at = block_scan<THREADS>(passing, lds.words, &listed);
@@ -821,12 +837,34 @@ __device__ int draw_row(const Draws& a, int64_t r, LongShared<KeyType<T>>& lds, 
     for (int b = begin; b < end; ++b)
       if (key_of(b) >= floor) lds.listed[at++] = b;
     __syncthreads();
-    // counts per listed block, their prefix sums, then the states in order of their index
-#pragma unroll 4
-    for (int q = wave; q < (int)listed; q += THREADS / 64) {
-      const int i = lds.listed[q] * kBlock + lane;
-      const uint64_t hits = __ballot(i < n && key_at(x, std::min(i, n - 1)) >= floor);
-      if (lane == 0) lds.count[q] = (uint32_t)__popcll(hits);
+    // V states in each of PIECE / V lanes per listed piece: counts, their prefix sums, then the states in order
+    constexpr int kLanes = PIECE / V, kTogether = 64 / kLanes;
+    const auto load = [&](int q, Key (&k)[V], int* first) {
+      uint32_t hits = 0;
+      *first = 0;
+      if (q < (int)listed) {
+        const int i = lds.listed[q] * PIECE + lane % kLanes * V;
+        *first = i;
+        if (i + V <= n) {
+          const Pack<T> p = load_pack(x + i);
+#pragma unroll
+          for (int j = 0; j < V; ++j) k[j] = KeyOf<W>::key(Value<T>::widen(p.v[j]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) k[j] = i + j < n ? key_at(x, i + j) : (Key)0;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) hits |= (uint32_t)(k[j] >= floor) << j;
+      }
+      return hits;
+    };
+#pragma unroll 2
+    for (int q0 = wave * kTogether; q0 < (int)listed; q0 += THREADS / 64 * kTogether) {
+      const int q = q0 + lane / kLanes;
+      Key k[V];
+      int first;
+      const int hits = lanes_all<kLanes>(__popc(load(q, k, &first)), [](int p, int q) { return p + q; });
+      if (lane % kLanes == 0 && q < (int)listed) lds.count[q] = (uint32_t)hits;
     }
     __syncthreads();
     constexpr int kPer = kListed / THREADS;
@@ -848,17 +886,21 @@ __device__ int draw_row(const Draws& a, int64_t r, LongShared<KeyType<T>>& lds, 
         }
       }
       __syncthreads();
-#pragma unroll 4
-      for (int q = wave; q < (int)listed; q += THREADS / 64) {
-        const int i = lds.listed[q] * kBlock + lane;
-        const Key k = key_at(x, std::min(i, n - 1));
-        const bool hit = i < n && k >= floor;
-        const uint64_t hits = __ballot(hit);
-        if (hit) {
-          const int to = (int)lds.count[q] + __popcll(hits & ((1ull << lane) - 1));
-          lds.key[to] = k;
-          lds.index[to] = i;
-        }
+#pragma unroll 2
+      for (int q0 = wave * kTogether; q0 < (int)listed; q0 += THREADS / 64 * kTogether) {
+        const int q = q0 + lane / kLanes;
+        Key k[V];
+        int first;
+        const uint32_t hits = load(q, k, &first);
+        int to = lanes_scan<kLanes>((int)__popc(hits)) - (int)__popc(hits);
+        if (hits != 0) to += (int)lds.count[q];
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (hits >> j & 1) {
+            lds.key[to] = k[j];
+            lds.index[to] = first + j;
+            ++to;
+          }
       }
       __syncthreads();
       if (wave == 0) {
@@ -880,12 +922,12 @@ __device__ int draw_row(const Draws& a, int64_t r, LongShared<KeyType<T>>& lds, 
   return -2;
 }
 
-template <typename T>
+template <typename T, int PIECE>
 __global__ void __launch_bounds__(kLongThreads) draw_long(const Draws a, int64_t first_row) {
   __shared__ LongShared<KeyType<T>> lds;
   const int64_t r = first_row + blockIdx.x;
   RowState state{};
-  const int drawn = draw_row<T>(a, r, lds, state);
+  const int drawn = draw_row<T, PIECE>(a, r, lds, state);
   if (threadIdx.x == 0) {
     if (drawn >= -1) a.out[r] = drawn;
     a.row_states[r] = state;
@@ -1248,20 +1290,29 @@ void launch_short_rows(const Draws& a, hipStream_t s) {
     launch_short<T, G, 16>(a, s);
 }
 
-template <typename T>
-void launch_long(const Draws& a, hipStream_t s) {
+template <typename T, int PIECE>
+void launch_summaries_and_draw(const Draws& a, hipStream_t s) {
   constexpr int kPacks = 4;
   constexpr int64_t kTile = (int64_t)64 * Value<T>::kVec * kPacks * (kSummaryThreads / 64);
   const int64_t tiles = (a.width + kTile - 1) / kTile;
-  const bn_draw_filters& f = a.filters;
-  const bool filter = f.top_k_dev || f.top_p_dev || f.min_p_dev || f.top_k > 0 || f.top_p < 1.0 || f.min_p > 0.0;
-  hipLaunchKernelGGL((block_summaries<T, kPacks>), dim3((uint32_t)std::min(a.rows * tiles, kMaxBlocks)),
+  hipLaunchKernelGGL((block_summaries<T, PIECE, kPacks>), dim3((uint32_t)std::min(a.rows * tiles, kMaxBlocks)),
                      dim3(kSummaryThreads), 0, s, a, tiles);
+  for (int64_t r = 0; r < a.rows; r += kMaxBlocks)
+    hipLaunchKernelGGL((draw_long<T, PIECE>), dim3((uint32_t)std::min(a.rows - r, kMaxBlocks)), dim3(kLongThreads), 0, s,
+                       a, r);
+}
+
+template <typename T>
+void launch_long(const Draws& a, hipStream_t s) {
+  if (a.width <= kSmallPieceStates)
+    launch_summaries_and_draw<T, 16>(a, s);
+  else
+    launch_summaries_and_draw<T, kBlock>(a, s);
+  const bn_draw_filters& f = a.filters;
+  if (!(f.top_k_dev || f.top_p_dev || f.min_p_dev || f.top_k > 0 || f.top_p < 1.0 || f.min_p > 0.0)) return;
   for (int64_t r = 0; r < a.rows; r += kMaxBlocks) {
     const dim3 grid((uint32_t)std::min(a.rows - r, kMaxBlocks));
-    hipLaunchKernelGGL(draw_long<T>, grid, dim3(kLongThreads), 0, s, a, r);
-    if (!filter) continue;
-    if (a.width <= 16384)
+    if (a.width <= kSmallPieceStates)
       hipLaunchKernelGGL((draw_wide<T, 256>), grid, dim3(256), 0, s, a, r);
     else
       hipLaunchKernelGGL((draw_wide<T, 1024>), grid, dim3(1024), 0, s, a, r);
@@ -1277,7 +1328,8 @@ hipError_t launch(const Draws& a, hipStream_t s) {
   else if (a.width <= 128) launch_short_rows<T, 8>(a, s);
   else if (a.width <= 256) launch_short_rows<T, 16>(a, s);
   else if (a.width <= 512) launch_short<T, 32, 16>(a, s);
-  else if (a.width <= kShortStates) launch_short<T, 64, 16>(a, s);
+  else if (a.width <= 1024) launch_short<T, 64, 16>(a, s);
+  else if (a.width <= kShortStates) launch_short<T, 64, 32>(a, s);
   else launch_long<T>(a, s);
   return hipGetLastError();
 }

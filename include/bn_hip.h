@@ -521,7 +521,7 @@ typedef struct bn_draw_filters {
   const double* min_p_dev;
 } bn_draw_filters;
 
-/* Bytes of device workspace bn_draw_states needs (0 up to 1024 states: workspace_dev may then be NULL;
+/* Bytes of device workspace bn_draw_states needs (0 up to 2048 states: workspace_dev may then be NULL;
  * else aligned to 8 bytes); -1 on a bad argument. */
 int64_t bn_draw_states_workspace_bytes(int dtype, int64_t rows, int64_t num_states);
 /*

@@ -64,7 +64,7 @@ def _draw(dtype=0, logits=A, rows=3, states=4, stride=4, counts=None, u_dtype=0,
     (dict(temperature=float("inf")), "temperature"), (dict(top_k=-1), "top_k"), (dict(top_p=0.0), "top_p"),
     (dict(top_p=1.5), "top_p"), (dict(top_p=float("nan")), "top_p"), (dict(min_p=-0.1), "min_p"),
     (dict(min_p=1.1), "min_p"), (dict(logits=None), "null"), (dict(u=None), "null"), (dict(out=None), "null"),
-    (dict(workspace=None, states=1025), "null"), (dict(workspace=B + 4, states=1025), "aligned"),
+    (dict(workspace=None, states=2049), "null"), (dict(workspace=B + 4, states=2049), "aligned"),
     (dict(logits=A + 2), "aligned"),
 ])
 def test_draw_refusals(change, message):
@@ -75,8 +75,8 @@ def test_draw_refusals(change, message):
 def test_draw_of_no_rows_and_workspace_sizes():
     lib = _native.load()
     assert _draw(rows=0, logits=None, u=None, out=None, workspace=None) == 0
-    assert lib.bn_draw_states_workspace_bytes(0, 3, 1024) == 0
-    assert lib.bn_draw_states_workspace_bytes(0, 3, 1025) > 0
+    assert lib.bn_draw_states_workspace_bytes(0, 3, 2048) == 0
+    assert lib.bn_draw_states_workspace_bytes(0, 3, 2049) > 0
     for bad in ((7, 3, 4), (0, -1, 4), (0, 3, 0), (0, 3, (1 << 24) + 1)):
         assert lib.bn_draw_states_workspace_bytes(*bad) == -1
 

@@ -52,7 +52,8 @@ int64_t bn_draw_states_workspace_bytes(int dtype, int64_t rows, int64_t num_stat
   const int64_t key_bytes = dtype == BN_F64 ? 8 : 4;
   const int64_t blocks = blocks_per_row(num_states);
   if (blocks == 0) return 0;
-  return rows * ((blocks + 2) * (int64_t)sizeof(double) + (int64_t)sizeof(RowState) + pieces_per_row(num_states) * key_bytes);
+  return rows * ((blocks + 2) * (int64_t)sizeof(double) + (int64_t)sizeof(RowState) +
+                 (rows_are_shared(rows, num_states) ? (int64_t)sizeof(SharedRow) : 0) + pieces_per_row(num_states) * key_bytes);
 }
 
 int bn_draw_states(int dtype, const void* logits_dev, int64_t rows, int64_t num_states, int64_t row_stride,
@@ -83,7 +84,12 @@ int bn_draw_states(int dtype, const void* logits_dev, int64_t rows, int64_t num_
     a.sums_per_row = blocks_per_row(num_states) + 2;
     a.block_sums = static_cast<double*>(workspace_dev);
     a.row_states = reinterpret_cast<RowState*>(a.block_sums + rows * a.sums_per_row);
-    a.piece_keys = a.row_states + rows;
+    void* rest = a.row_states + rows;
+    if (rows_are_shared(rows, num_states)) {
+      a.shared = static_cast<SharedRow*>(rest);
+      rest = a.shared + rows;
+    }
+    a.piece_keys = rest;
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {

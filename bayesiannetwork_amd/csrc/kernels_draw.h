@@ -70,6 +70,7 @@ __device__ __forceinline__ bool undrawable(float x) { return !(x < INFINITY); }
 __device__ __forceinline__ bool undrawable(double x) { return !(x < (double)INFINITY); }
 
 struct RowState;
+struct SharedRow;
 
 struct Draws {
   const void* logits;
@@ -83,6 +84,7 @@ struct Draws {
   // long rows: the workspace
   double* block_sums;     // [rows][sums_per_row]
   RowState* row_states;   // [rows]
+  SharedRow* shared;      // [rows], or null where a block does a row by itself
   void* piece_keys;       // [rows][pieces_per_row]
   int64_t pieces_per_row;
   int64_t sums_per_row;   // blocks and two more: draw_wide's segments, of 128 states at least, take two entries each
@@ -476,6 +478,19 @@ struct RowState {
   unsigned long long best, floor;  // keys: the largest, and one below which nothing is kept
   double total;                    // weight of the whole row, where top-k is off
   long long pending;               // 0: the row is drawn
+};
+
+// What the blocks that share a row's second and third pass leave for the last one.
+constexpr int kShares = 16;
+constexpr int kShareThreads = 256;
+constexpr int kRoughBins = 4 * kShareThreads;
+constexpr int kSharedRoom = 4096;  // states around the threshold
+struct SharedRow {
+  unsigned long long mass[kRoughBins];
+  double certain[kShares];
+  unsigned long long listed;
+  uint64_t key[kSharedRoom];
+  int32_t index[kSharedRoom];
 };
 
 constexpr int kCandidates = 512;  // states that one wave draws among
@@ -932,23 +947,26 @@ __global__ void __launch_bounds__(kLongThreads) draw_long(const Draws a, int64_t
     if (drawn >= -1) a.out[r] = drawn;
     a.row_states[r] = state;
   }
+  if (drawn < -1 && a.shared) {
+    for (int b = threadIdx.x; b < kRoughBins; b += kLongThreads) a.shared[r].mass[b] = 0;
+    if (threadIdx.x == 0) a.shared[r].listed = 0;
+  }
 }
 
 // ---- long rows that keep many states ----------------------------------------------------------------
 
-// Calls fn(index, logit) for all n states of a row in memory.
+// Calls fn(index, logit) for the states [begin, end) of a row in memory; begin is a multiple of a pack.
 template <typename T, int THREADS, typename Fn>
-__device__ __forceinline__ void for_each_state(const T* x, int n, Fn fn) {
+__device__ __forceinline__ void for_each_state(const T* x, int begin, int end, Fn fn) {
   constexpr int V = Value<T>::kVec;
-  const int packs = n / V;
 #pragma unroll 2
-  for (int k = threadIdx.x; k < packs; k += THREADS) {
-    const Pack<T> p = load_pack(x + k * V);
+  for (int i = begin + (int)threadIdx.x * V; i + V <= end; i += THREADS * V) {
+    const Pack<T> p = load_pack(x + i);
 #pragma unroll
-    for (int j = 0; j < V; ++j) fn(k * V + j, Value<T>::widen(p.v[j]));
+    for (int j = 0; j < V; ++j) fn(i + j, Value<T>::widen(p.v[j]));
   }
-  const int i = packs * V + (int)threadIdx.x;
-  if (i < n) fn(i, Value<T>::widen(x[i]));
+  const int i = begin + (end - begin) / V * V + (int)threadIdx.x;
+  if (i < end) fn(i, Value<T>::widen(x[i]));
 }
 
 // Bins of equal width in the logit (in the key they would be wide near the maximum, where the weight is, and
@@ -1025,33 +1043,158 @@ __device__ int last_kept(const T* x, int n, KeyType<T> key, unsigned long long k
   return (int)lds.answer[0];
 }
 
-// One row by the whole block, over the row in memory: one pass counts its states by logit, a second one adds up
-// what is certainly kept, and the few thousand states around the threshold are settled in LDS.
+// A row that is left, as every block that works on it sees it.
+template <typename T>
+struct WideRow {
+  using W = typename Value<T>::Wide;
+  using Key = KeyType<T>;
+  static constexpr int V = Value<T>::kVec;
+  static constexpr int kSegment = 64 * V;  // states whose sum a wave takes
+  const T* x;
+  Setting s;
+  int n, segments;
+  Key best, floor;
+  double largest;
+  Weight weight;
+  Steps<W> steps;
+  double* sums;               // the block sums have served: one entry per segment, what certainly is kept of it,
+  unsigned long long* extra;  // and what the states around the threshold add, as integers of 2^-50
+  __device__ __forceinline__ static double floor_value(Key floor) {
+    const double v = floor == 1 ? -INFINITY : (double)KeyOf<W>::value(floor);
+    return v > -INFINITY ? v : -INFINITY;
+  }
+  __device__ __forceinline__ WideRow(const Draws& a, int64_t r, const RowState& state, int bins)
+      : x(static_cast<const T*>(a.logits) + r * a.stride),
+        s(row_setting(a, r)),
+        n((int)s.n),
+        segments((n + kSegment - 1) / kSegment),
+        best((Key)state.best),
+        floor((Key)state.floor),
+        largest((double)KeyOf<W>::value(best)),
+        weight(largest, s.temperature),
+        steps(floor_value(floor), largest, s.temperature, bins),
+        sums(a.block_sums + r * a.sums_per_row),
+        extra(reinterpret_cast<unsigned long long*>(sums + segments)) {}
+};
+constexpr double kListScale = 1125899906842624.0;  // 2^50: at most 4096 weights add up
+
+// Masses by logit of a prefix's states in [begin, end), from weights of single precision.
+constexpr double kRoughScale = 274877906944.0;  // 2^38: 2^24 weights add up within 62 bits
 template <typename T, int THREADS>
-__device__ int draw_wide_row(const Draws& a, int64_t r, const RowState& state, Bins<THREADS>& lds,
+__device__ void add_rough_masses(const WideRow<T>& row, const Prefix<KeyType<T>>& in, int begin, int end,
+                                 unsigned long long* mass) {
+  using W = typename Value<T>::Wide;
+  const float rate = (float)row.weight.rate;
+  for_each_state<T, THREADS>(row.x, begin, end, [&](int i, W v) {
+    if (!in.has(i, KeyOf<W>::key(v))) return;
+    const float rough = __builtin_amdgcn_exp2f((float)((double)v - row.largest) * rate);
+    atomicAdd(&mass[row.steps.bin(v)], mass_of((double)rough, kRoughScale));
+  });
+}
+
+// The bins around the threshold at which the mass from the top reaches `target`: what lies above these is kept,
+// what lies below is not.  Three roundings of the exponent t make a rough weight wrong by 3 * 2^-24 * ln 2 * |t|,
+// the exponential itself by 2^-22; a sum that starts with the largest weight, 1, has a mean |t| of 25 at most
+// (2^24 states of weight 2^-24 double it), so it is off by less than 4e-6 of itself, a fifth of kSlack, and by
+// the integers' rounding.
+template <int THREADS>
+__device__ int2 bins_around(const unsigned long long* mass, double target, int n, unsigned long long* words) {
+  constexpr int kBins = 4 * THREADS;
+  constexpr double kSlack = 2e-5;
+  const double rounding = (double)n + 1.0, goal = target * kRoughScale;
+  unsigned long long own[4], sum = 0, total;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    own[b] = mass[kBins - 1 - 4 * (int)threadIdx.x - b];
+    sum += own[b];
+  }
+  unsigned long long upto = block_scan<THREADS>(sum, words, &total);
+  uint32_t first = ~0u, last = ~0u;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const uint32_t at = 4 * threadIdx.x + b;
+    upto += own[b];
+    if (first == ~0u && (double)upto * (1.0 + kSlack) + rounding >= goal) first = at;
+    if (last == ~0u && (double)upto * (1.0 - kSlack) - rounding >= goal) last = at;
+  }
+  const unsigned long long ends = block_all<THREADS>(((unsigned long long)first << 32) | last, words, kMinOfHalves);
+  const int lowest = std::min((uint32_t)ends, (uint32_t)kBins - 1);
+  const int highest = std::min((int)std::min((uint32_t)(ends >> 32), (uint32_t)kBins - 1), lowest);
+  return make_int2(kBins - 1 - lowest, kBins - 1 - highest);
+}
+
+// Weights of a prefix's states in the bins above one: their sum over the segments [begin, end), and by segment
+// those that min-p leaves.
+template <typename T, int THREADS>
+__device__ double add_up(const WideRow<T>& row, const Prefix<KeyType<T>>& in, int above, int begin, int end,
+                         unsigned long long* words) {
+  using W = typename Value<T>::Wide;
+  constexpr int V = Value<T>::kVec;
+  const int lane = threadIdx.x & 63;
+  const auto load = [&](int q) {
+    const int i = (q * 64 + lane) * V;
+    Pack<T> p;
+    if (i + V <= row.n) {
+      p = load_pack(row.x + i);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) p.v[j] = i + j < row.n ? row.x[i + j] : Value<T>::round(-INFINITY);
+    }
+    return raw_of(p);
+  };
+  double all = 0.0;
+  int q = begin + (int)(threadIdx.x >> 6);
+  Raw next = load(q);  // the segment after this one is on its way while this one is worked on
+  for (; q < end; q += THREADS / 64) {
+    Raw raw = next;
+    next = load(q + THREADS / 64);
+    bn_rows::kept(raw);
+    const Pack<T> p = pack_of<T>(raw);
+    const int i = (q * 64 + lane) * V;
+    double drawn = 0.0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const W v = Value<T>::widen(p.v[j]);
+      if (in.has(i + j, KeyOf<W>::key(v)) && row.steps.bin(v) > above) {
+        const double w = row.weight((double)v);
+        all += w;
+        drawn += w >= row.s.min_p ? w : 0.0;
+      }
+    }
+    drawn = lanes_sum<64>(drawn);
+    if (lane == 0) {
+      row.sums[q] = drawn;
+      row.extra[q] = 0;
+    }
+  }
+  double total;
+  (void)block_scan<THREADS>(all, words, &total);  // (its barriers also publish the segments' sums)
+  return total;
+}
+
+// One row by the whole block, over the row in memory: one pass weighs its states roughly, by logit, a second
+// one adds up what is certainly kept, and the few thousand states around the threshold are settled in LDS.
+// Where the blocks of draw_wide_masses and draw_wide_sums have shared those passes, `shared` holds their results.
+template <typename T, int THREADS>
+__device__ int draw_wide_row(const WideRow<T>& row, const SharedRow* shared, double row_total, Bins<THREADS>& lds,
                              Listed<KeyType<T>, THREADS>& list) {
   using W = typename Value<T>::Wide;
   using Key = KeyType<T>;
   using Sum = unsigned long long;
   constexpr int V = Value<T>::kVec;
-  constexpr int kBins = Bins<THREADS>::kBins;
   constexpr uint32_t kRoom = Listed<Key, THREADS>::kRoom;
-  const T* x = static_cast<const T*>(a.logits) + r * a.stride;
-  const Setting s = row_setting(a, r);
-  const int n = (int)s.n;
-  const Key best = (Key)state.best, floor = (Key)state.floor;
-  const double largest = (double)KeyOf<W>::value(best);
-  const Weight weight(largest, s.temperature);
+  const Setting& s = row.s;
+  const Weight& weight = row.weight;
+  const int n = row.n;
+  const T* x = row.x;
   const double scale = mass_scale(n);
   const auto mass = [&](Key k) { return mass_of(weight.of_key(k), scale); };
   const auto no_mass = [](auto) { return 0ull; };
-  const double floor_value = floor == 1 ? -INFINITY : (double)KeyOf<W>::value(floor);
-  const Steps<W> steps(isnan(floor_value) ? -INFINITY : floor_value, largest, s.temperature, kBins);
 
   // the states of a prefix in bins lowest..highest, by key
   const auto each_in = [&](const Prefix<Key>& in, int lowest, int highest, auto fn) {
-    for_each_state<T, THREADS>(x, n, [&](int i, W v) {
-      const int bin = steps.bin(v);
+    for_each_state<T, THREADS>(x, 0, n, [&](int i, W v) {
+      const int bin = row.steps.bin(v);
       if (bin < lowest || bin > highest) return;
       const Key k = KeyOf<W>::key(v);
       if (in.has(i, k)) fn(i, k);
@@ -1064,6 +1207,7 @@ __device__ int draw_wide_row(const Draws& a, int64_t r, const RowState& state, B
     each_in(in, lowest, highest, [&](int i, Key k) {
       if (k < low || k > high) return;
       const uint32_t at = atomicAdd(&list.count, 1u);
+      if (at >= kRoom) return;
       list.key[at] = k;
       list.index[at] = i;
     });
@@ -1075,16 +1219,16 @@ __device__ int draw_wide_row(const Draws& a, int64_t r, const RowState& state, B
   };
 
   // ---- top-k: the k-th key by counting
-  Prefix<Key> kept{floor, n};
+  Prefix<Key> kept{row.floor, n};
   if (s.has_top_k()) {
     const Prefix<Key> all = kept;
     const auto each_state = [&](auto fn) {
-      for_each_state<T, THREADS>(x, n, [&](int, W v) {
-        if (KeyOf<W>::key(v) >= floor) fn(v);
+      for_each_state<T, THREADS>(x, 0, n, [&](int, W v) {
+        if (KeyOf<W>::key(v) >= all.key) fn(v);
       });
     };
-    const Found f = find_bin<false>(lds, each_state, [&](W v) { return steps.bin(v); }, no_mass, 0ull, (double)s.top_k);
-    KeyRange<Key> range{floor, best, f.above, f.states, true};
+    const Found f = find_bin<false>(lds, each_state, [&](W v) { return row.steps.bin(v); }, no_mass, 0ull, (double)s.top_k);
+    KeyRange<Key> range{row.floor, row.best, f.above, f.states, true};
     const auto each_key = [&](auto fn) {
       each_in(all, f.bin, f.bin, [&](int, Key k) { fn(k); });
     };
@@ -1099,118 +1243,47 @@ __device__ int draw_wide_row(const Draws& a, int64_t r, const RowState& state, B
     if (ties < range.states) kept.last = last_kept<T, THREADS>(x, n, range.low, ties, lds, list, in_list);
   }
 
-  const int segments = (n + 64 * V - 1) / (64 * V);
-  double* sums = a.block_sums + r * a.sums_per_row;  // the block sums have served: one entry per segment,
-  Sum* extra = reinterpret_cast<Sum*>(sums + segments);  // and what the list adds to it
-  // Weights of the states of a prefix in the bins above one: their sum, and by segments those that min-p leaves.
-  const auto add_up = [&](const Prefix<Key>& in, int above) {
-    double all = 0.0;
-    const auto load = [&](int q) {
-      const int i = (q * 64 + (int)(threadIdx.x & 63)) * V;
-      Pack<T> p;
-      if (i + V <= n) {
-        p = load_pack(x + i);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) p.v[j] = i + j < n ? x[i + j] : Value<T>::round(-INFINITY);
-      }
-      return raw_of(p);
-    };
-    int q = threadIdx.x >> 6;
-    Raw next = load(q);  // the segment after this one is on its way while this one is worked on
-    for (; q < segments; q += THREADS / 64) {
-      Raw raw = next;
-      next = load(q + THREADS / 64);
-      bn_rows::kept(raw);
-      const Pack<T> p = pack_of<T>(raw);
-      const int i = (q * 64 + (int)(threadIdx.x & 63)) * V;
-      double drawn = 0.0;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const W v = Value<T>::widen(p.v[j]);
-        if (in.has(i + j, KeyOf<W>::key(v)) && steps.bin(v) > above) {
-          const double w = weight((double)v);
-          all += w;
-          drawn += w >= s.min_p ? w : 0.0;
-        }
-      }
-      drawn = lanes_sum<64>(drawn);
-      if ((threadIdx.x & 63) == 0) {
-        sums[q] = drawn;
-        extra[q] = 0;
-      }
-    }
-    double total;
-    (void)block_scan<THREADS>(all, lds.words, &total);  // (its barriers also publish the segments' sums)
-    return total;
-  };
-
-  constexpr double kListScale = 1125899906842624.0;  // 2^50: at most 4096 weights add up
   bool added = false;
   if (s.has_top_p()) {
-    const double w_all = s.has_top_k() ? add_up(kept, -1) : state.total;
-    const double target = s.top_p * w_all;
-    // Masses by logit, from weights of single precision, tell the bins around the threshold: what lies above
-    // these is kept, what lies below is not.  Three roundings of the exponent t make a weight wrong by
-    // 3 * 2^-24 * ln 2 * |t|, the exponential itself by 2^-22; a sum that starts with the largest weight, 1, has a
-    // mean |t| of 25 at most (2^24 states of weight 2^-24 double it), so it is off by less than 4e-6 of
-    // itself, a fifth of kSlack, and by the integers' rounding.
-    __syncthreads();
+    const double target = s.top_p * (s.has_top_k() ? add_up<T, THREADS>(row, kept, -1, 0, row.segments, lds.words) : row_total);
+    const double reach = target * scale;
+    KeyRange<Key> range{kept.key, row.best, 0ull, 0ull, true};
+    bool in_list, whole_list;  // the list holds the threshold's states; all those around it
+    if (shared && shared->listed <= kRoom) {
+      double certain = 0.0;
+      for (int c = 0; c < kShares; ++c) certain += shared->certain[c];
+      range.above = (Sum)llrint(certain * scale);
+      const uint32_t count = (uint32_t)shared->listed;
+      for (uint32_t q = threadIdx.x; q < count; q += THREADS) {
+        list.key[q] = (Key)shared->key[q];
+        list.index[q] = shared->index[q];
+      }
+      if (threadIdx.x == 0) list.count = count;
+      __syncthreads();
+      in_list = whole_list = true;
+    } else {
+      __syncthreads();
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      lds.count[b * THREADS + threadIdx.x] = 0;
-      lds.mass[b * THREADS + threadIdx.x] = 0;
-    }
-    __syncthreads();
-    constexpr double kRoughScale = 274877906944.0;  // 2^38: 2^24 weights add up within 62 bits
-    constexpr double kSlack = 2e-5;
-    const double rough_error = (double)n + 1.0;
-    const float rate = (float)weight.rate;
-    for_each_state<T, THREADS>(x, n, [&](int i, W v) {
-      if (!kept.has(i, KeyOf<W>::key(v))) return;
-      const int bin = steps.bin(v);
-      const float rough = __builtin_amdgcn_exp2f((float)((double)v - largest) * rate);
-      atomicAdd(&lds.count[bin], 1u);
-      atomicAdd(&lds.mass[bin], mass_of((double)rough, kRoughScale));
-    });
-    __syncthreads();
-    Sum own[4], own_sum = 0, ignored;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      own[b] = lds.mass[kBins - 1 - 4 * (int)threadIdx.x - b];
-      own_sum += own[b];
-    }
-    Sum upto = block_scan<THREADS>(own_sum, lds.words, &ignored);
-    uint32_t first = ~0u, last = ~0u, lowest = ~0u;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const uint32_t at = 4 * threadIdx.x + b;
-      upto += own[b];
-      if (lds.count[kBins - 1 - at] != 0) {
-        if (first == ~0u && (double)upto * (1.0 + kSlack) + rough_error >= target * kRoughScale) first = at;
-        if (last == ~0u && (double)upto * (1.0 - kSlack) - rough_error >= target * kRoughScale) last = at;
-        lowest = kBins - 1 - at;
+      for (int b = 0; b < 4; ++b) lds.mass[b * THREADS + threadIdx.x] = 0;
+      __syncthreads();
+      add_rough_masses<T, THREADS>(row, kept, 0, n, lds.mass);
+      __syncthreads();
+      const int2 around = bins_around<THREADS>(lds.mass, target, n, lds.words);
+      range.above = (Sum)llrint(add_up<T, THREADS>(row, kept, around.y, 0, row.segments, lds.words) * scale);
+      fill_list(kept, around.x, around.y, range.low, range.high);
+      in_list = whole_list = list.count <= kRoom;
+      if (!in_list) {
+        const auto each_key = [&](auto fn) {
+          each_in(kept, around.x, around.y, [&](int, Key k) { fn(k); });
+        };
+        do {
+          narrow<true>(lds, range, each_key, mass, reach);
+        } while (range.low != range.high && range.states > kRoom);
+        in_list = range.states <= kRoom;
+        if (in_list) fill_list(kept, around.x, around.y, range.low, range.high);
       }
     }
-    const Sum ends = block_all<THREADS>(((Sum)first << 32) | last, lds.words, kMinOfHalves);
-    lowest = kBins - 1 - (uint32_t)block_all<THREADS>((Sum)lowest, lds.words, kMin);
-    last = std::min((uint32_t)ends, lowest);
-    first = std::min((uint32_t)(ends >> 32), last);
-    const int bin_low = kBins - 1 - (int)last, bin_high = kBins - 1 - (int)first;
-    Sum around = 0;
-    for (int b = bin_low + (int)threadIdx.x; b <= bin_high; b += THREADS) around += lds.count[b];
-    around = block_all<THREADS>(around, lds.words, [](Sum p, Sum q) { return p + q; });
-    const double certain = add_up(kept, bin_high);
-    const double reach = target * scale;
-    KeyRange<Key> range{kept.key, best, (Sum)llrint(certain * scale), around, true};
-    const auto each_key = [&](auto fn) {
-      each_in(kept, bin_low, bin_high, [&](int, Key k) { fn(k); });
-    };
-    const bool narrowed = around > kRoom;
-    while (range.low != range.high && range.states > kRoom) narrow<true>(lds, range, each_key, mass, reach);
-    const bool in_list = range.states <= kRoom;
     if (in_list) {
-      fill_list(kept, bin_low, bin_high, range.low, range.high);
       do {
         narrow<true>(lds, range, each_listed, mass, reach);
       } while (range.low != range.high);
@@ -1224,25 +1297,25 @@ __device__ int draw_wide_row(const Draws& a, int64_t r, const RowState& state, B
     const int bound = range.low == kept.key ? kept.last : n;
     kept.key = range.low;
     kept.last = ties < range.states ? last_kept<T, THREADS>(x, n, range.low, ties, lds, list, in_list) : bound;
-    if (in_list && !narrowed) {
+    if (whole_list) {
       // the segments hold what lies above the bins, the list what lies in them
       const uint32_t count = list.count;
       for (uint32_t q = threadIdx.x; q < count; q += THREADS)
         if (kept.has(list.index[q], list.key[q])) {
           const double w = weight.of_key(list.key[q]);
-          if (w >= s.min_p) atomicAdd(&extra[list.index[q] / (64 * V)], mass_of(w, kListScale));
+          if (w >= s.min_p) atomicAdd(&row.extra[list.index[q] / WideRow<T>::kSegment], mass_of(w, kListScale));
         }
       __threadfence();
       added = true;
     }
   }
-  if (!added) (void)add_up(kept, -1);
+  if (!added) (void)add_up<T, THREADS>(row, kept, -1, 0, row.segments, lds.words);
   __syncthreads();
   return locate<V>(
-      lds, segments, s.uniform,
+      lds, row.segments, s.uniform,
       [&](int q) {
-        const Sum more = __hip_atomic_load(&extra[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        return sums[q] + (double)more / kListScale;
+        const Sum more = __hip_atomic_load(&row.extra[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return row.sums[q] + (double)more / kListScale;
       },
       [&](int i) {
         if (i >= n) return 0.0;
@@ -1259,8 +1332,62 @@ __global__ void __launch_bounds__(THREADS) draw_wide(const Draws a, int64_t firs
   const int64_t r = first_row + blockIdx.x;
   const RowState state = a.row_states[r];
   if (!state.pending) return;
-  const int drawn = draw_wide_row<T, THREADS>(a, r, state, lds, list);
+  const WideRow<T> row(a, r, state, Bins<THREADS>::kBins);
+  const bool prepared = a.shared && row.s.has_top_p() && !row.s.has_top_k();
+  const int drawn = draw_wide_row<T, THREADS>(row, prepared ? a.shared + r : nullptr, state.total, lds, list);
   if (threadIdx.x == 0) a.out[r] = drawn;
+}
+
+// The same passes over a row with top-p alone, by kShares blocks: a block is bound by its arithmetic (a row of
+// 131072 states took one block 110 us), and a call of few rows leaves most of the GPU idle.
+template <typename T>
+__global__ void __launch_bounds__(kShareThreads) draw_wide_masses(const Draws a) {
+  __shared__ unsigned long long mass[kRoughBins];
+  const int64_t r = blockIdx.x / kShares;
+  const int share = blockIdx.x % kShares;
+  const RowState state = a.row_states[r];
+  if (!state.pending) return;
+  const WideRow<T> row(a, r, state, kRoughBins);
+  if (!row.s.has_top_p() || row.s.has_top_k()) return;
+  for (int b = threadIdx.x; b < kRoughBins; b += kShareThreads) mass[b] = 0;
+  __syncthreads();
+  const int each = (row.segments + kShares - 1) / kShares * WideRow<T>::kSegment;
+  const int begin = std::min(share * each, row.n), end = std::min(begin + each, row.n);
+  add_rough_masses<T, kShareThreads>(row, Prefix<KeyType<T>>{row.floor, row.n}, begin, end, mass);
+  __syncthreads();
+  for (int b = threadIdx.x; b < kRoughBins; b += kShareThreads)
+    if (mass[b] != 0) atomicAdd(&a.shared[r].mass[b], mass[b]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kShareThreads) draw_wide_sums(const Draws a) {
+  using W = typename Value<T>::Wide;
+  using Key = KeyType<T>;
+  __shared__ unsigned long long words[kShareThreads / 64];
+  const int64_t r = blockIdx.x / kShares;
+  const int share = blockIdx.x % kShares;
+  const RowState state = a.row_states[r];
+  if (!state.pending) return;
+  const WideRow<T> row(a, r, state, kRoughBins);
+  if (!row.s.has_top_p() || row.s.has_top_k()) return;
+  SharedRow& shared = a.shared[r];
+  const int2 around = bins_around<kShareThreads>(shared.mass, row.s.top_p * state.total, row.n, words);
+  const int each = (row.segments + kShares - 1) / kShares;
+  const int begin = std::min(share * each, row.segments), end = std::min(begin + each, row.segments);
+  const Prefix<Key> in{row.floor, row.n};
+  const double certain = add_up<T, kShareThreads>(row, in, around.y, begin, end, words);
+  if (threadIdx.x == 0) shared.certain[share] = certain;
+  for_each_state<T, kShareThreads>(row.x, std::min(begin * WideRow<T>::kSegment, row.n),
+                                   std::min(end * WideRow<T>::kSegment, row.n), [&](int i, W v) {
+    const int bin = row.steps.bin(v);
+    if (bin < around.x || bin > around.y) return;
+    const Key k = KeyOf<W>::key(v);
+    if (!in.has(i, k)) return;
+    const unsigned long long at = atomicAdd(&shared.listed, 1ull);
+    if (at >= kSharedRoom) return;
+    shared.key[at] = (uint64_t)k;
+    shared.index[at] = i;
+  });
 }
 
 constexpr int64_t kMaxStates = 1 << 24;
@@ -1310,6 +1437,11 @@ void launch_long(const Draws& a, hipStream_t s) {
     launch_summaries_and_draw<T, kBlock>(a, s);
   const bn_draw_filters& f = a.filters;
   if (!(f.top_k_dev || f.top_p_dev || f.min_p_dev || f.top_k > 0 || f.top_p < 1.0 || f.min_p > 0.0)) return;
+  if (a.shared && (f.top_p_dev || f.top_p < 1.0) && (f.top_k_dev || f.top_k == 0)) {
+    const dim3 grid((uint32_t)(a.rows * kShares));
+    hipLaunchKernelGGL(draw_wide_masses<T>, grid, dim3(kShareThreads), 0, s, a);
+    hipLaunchKernelGGL(draw_wide_sums<T>, grid, dim3(kShareThreads), 0, s, a);
+  }
   for (int64_t r = 0; r < a.rows; r += kMaxBlocks) {
     const dim3 grid((uint32_t)std::min(a.rows - r, kMaxBlocks));
     if (a.width <= kSmallPieceStates)
@@ -1318,6 +1450,9 @@ void launch_long(const Draws& a, hipStream_t s) {
       hipLaunchKernelGGL((draw_wide<T, 1024>), grid, dim3(1024), 0, s, a, r);
   }
 }
+
+// Rows of which several blocks take a share: long ones, and no more of them than leave CUs (256) idle.
+inline bool rows_are_shared(int64_t rows, int64_t num_states) { return num_states > kSmallPieceStates && rows <= 512; }
 
 template <typename T>
 hipError_t launch(const Draws& a, hipStream_t s) {

@@ -41,8 +41,26 @@ struct Rows {
 
 enum Mode { kForward, kBoth, kBackward };
 
-__device__ __forceinline__ float exp_wide(float t) { return __builtin_amdgcn_exp2f(t * 1.44269504088896340736f); }
+__device__ __forceinline__ float exp_wide(float t) { return __builtin_amdgcn_exp2f(t * 1.44269502162933349609f); }
 __device__ __forceinline__ double exp_wide(double t) { return exp(t); }
+
+// exp(t), t <= 0, for gradients.  With float32 logits the roundings of t log2(e) are made good (five instructions;
+// without it a gradient of 64 states was off by 1.2e-7 of its norm, with it by 4e-8).  They hardly
+// move a sum of exponentials, and what 16-bit logits lead to is rounded far above them.
+template <typename T>
+__device__ __forceinline__ float exp_precise(float t) {
+  constexpr float kLog2e = 1.44269502162933349609f, kRest = 1.92596303e-8f;  // together log2(e) to 48 bits
+  if (sizeof(T) == 2) return exp_wide(t);
+  const float y = t * kLog2e;
+  const float e = __builtin_amdgcn_exp2f(y);
+  // NaN or infinite where y is infinite: any finite number does, since e is 0 there
+  const float r = fminf(fmaxf(fmaf(t, kRest, fmaf(t, kLog2e, -y)), -1.0f), 1.0f);
+  return fmaf(e, r * 0.693147180559945f, e);
+}
+template <typename T>
+__device__ __forceinline__ double exp_precise(double t) {
+  return exp(t);
+}
 
 __device__ __forceinline__ int64_t row_count(const Rows& a, int64_t r) {
   if (!a.counts) return a.width;
@@ -88,12 +106,13 @@ __device__ __forceinline__ void finish_row(const Rows& a, int64_t r, bool observ
 }
 
 // Gradient of a row: weight * ([i = state] - exp(x_i - best) / sum), 0 for a row that was not observed.
-template <typename W>
+template <typename T>
 struct Slope {
+  using W = typename Value<T>::Wide;
   W reference, scale, weight;
   bool observed;
   __device__ __forceinline__ W at(W x, bool is_state) const {
-    const W p = exp_wide(x - reference) * scale;
+    const W p = exp_precise<T>(x - reference) * scale;
     return weight * ((is_state ? (W)1 : (W)0) - p);
   }
 };
@@ -104,8 +123,8 @@ __device__ __forceinline__ typename Value<T>::Wide row_weight(const Rows& a, int
   return a.weights ? static_cast<const W*>(a.weights)[r * a.weights_stride] : (W)1;
 }
 
-template <typename W>
-__device__ __forceinline__ Slope<W> slope_from_total(W weight, bool observed, const Total<W>& total) {
+template <typename T, typename W>
+__device__ __forceinline__ Slope<T> slope_from_total(W weight, bool observed, const Total<W>& total) {
   // sum 0: no possible state, no gradient
   const bool none = total.sum == (W)0;
   return {total.reference(), none ? (W)0 : (W)1 / total.sum, none ? (W)0 : weight, observed};
@@ -113,8 +132,8 @@ __device__ __forceinline__ Slope<W> slope_from_total(W weight, bool observed, co
 
 // The gradient at the V states from i on, of which the row has n (x: their logits); the row's state is `at`
 // places behind i.  0 beyond the row.
-template <typename T, typename W>
-__device__ __forceinline__ Pack<T> gradient_pack(const Slope<W>& slope, Pack<T> x, int64_t at, int64_t inside) {
+template <typename T>
+__device__ __forceinline__ Pack<T> gradient_pack(const Slope<T>& slope, Pack<T> x, int64_t at, int64_t inside) {
   constexpr int V = Value<T>::kVec;
   const int place = (uint64_t)at < (uint64_t)V ? (int)at : -1;
   if (!slope.observed) inside = 0;
@@ -124,17 +143,20 @@ __device__ __forceinline__ Pack<T> gradient_pack(const Slope<W>& slope, Pack<T> 
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      x.v[j] = Value<T>::round(j < inside ? slope.at(Value<T>::widen(x.v[j]), place == j) : (W)0);
+      x.v[j] = Value<T>::round(j < inside ? slope.at(Value<T>::widen(x.v[j]), place == j) : (typename Value<T>::Wide)0);
   }
   return x;
 }
 
 // Stores the part of a pack that lies inside a row of `width` states.
-template <typename T, typename Index>
+template <bool STREAM, typename T, typename Index>
 __device__ __forceinline__ void store_row_pack(T* out, Index i, Index width, const Pack<T>& p) {
   constexpr int V = Value<T>::kVec;
   if (i + V <= width) {
-    store_pack(out + i, p);
+    if (STREAM)
+      store_pack_streamed(out + i, p);
+    else
+      store_pack(out + i, p);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
@@ -172,7 +194,8 @@ __device__ __forceinline__ Raw row_raw(const T* x, Index i, Index n) {
 
 // A group takes KEEP rows, all loaded before the first is worked on; the logarithms of their sums (a hundred
 // double instructions, whatever the number of lanes that need one) are left to the end, where lane k has
-// row k's.
+// row k's.  (The gradient goes past the caches' order as in rows_in_block: 131072 x 64 float32 13.8 us, 17.9 us
+// otherwise.)
 template <typename T, int LANES, int PACKS, int KEEP, int MODE>
 __global__ void __launch_bounds__(256) rows_in_lanes(const Rows a) {
   using W = typename Value<T>::Wide;
@@ -229,13 +252,14 @@ __global__ void __launch_bounds__(256) rows_in_lanes(const Rows a) {
       if constexpr (MODE == kBoth) {
         if (base + q >= a.rows) continue;
         const int n = __shfl(own_count, q, LANES), state = __shfl(own_state, q, LANES);
-        const Slope<W> slope = slope_from_total(__shfl(own_weight, q, LANES), state >= 0, total);
+        const Slope<T> slope = slope_from_total<T>(__shfl(own_weight, q, LANES), state >= 0, total);
         T* out = static_cast<T*>(a.gradient) + (base + q) * a.gradient_stride;
 #pragma unroll
         for (int k = 0; k < PACKS; ++k) {
           const int i = (k * LANES + lane) * V;
           kept(raw[q][k]);
-          if (i < width) store_row_pack(out, i, width, gradient_pack(slope, pack_of<T>(raw[q][k]), state - i, n - i));
+          if (i < width)
+            store_row_pack<true>(out, i, width, gradient_pack(slope, pack_of<T>(raw[q][k]), state - i, n - i));
         }
       }
     }
@@ -278,10 +302,12 @@ __device__ __forceinline__ W block_sum(W v, W* lds) {
 // 5003 float32, where what reads it next is no slower for it (18.7 against 20.7 us together); between about
 // 100 and 256 MB the next reader loses more than is won here (4096 x 16000: 44 against 46 us alone, 99
 // against 92 together).
+// HOLD: false where the exponentials do not fit the registers beside the logits.  They are taken twice then, and
+// the next row is requested as this one is written.
 //
 // A row is up to PACKS rounds of THREADS whole packs, by uniform addresses and without checks, and a rest of
 // less than a round with them (checks in the unrolled rounds cost more registers than the row itself).
-template <typename T, int THREADS, int PACKS>
+template <typename T, int THREADS, int PACKS, bool HOLD>
 __global__ void __launch_bounds__(THREADS) rows_in_block(const Rows a) {
   using W = typename Value<T>::Wide;
   constexpr int V = Value<T>::kVec;
@@ -333,24 +359,31 @@ __global__ void __launch_bounds__(THREADS) rows_in_block(const Rows a) {
     for (int k = 0; k < PACKS; ++k) raise(raw[k]);
     raise(rest);
     const W reference = own == (W)-INFINITY ? (W)0 : own;
-    W e[PACKS + 1][V], sum = 0;
-    const auto add = [&](Raw& from, W (&to)[V]) {
+    W e[HOLD ? PACKS + 1 : 1][V], sum = 0;
+    const auto add = [&](Raw& from, int k) {
       kept(from);
       const Pack<T> p = pack_of<T>(from);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        to[j] = exp_wide(Value<T>::widen(p.v[j]) - reference);
-        sum += to[j];
+        const W power = exp_precise<T>(Value<T>::widen(p.v[j]) - reference);
+        if (HOLD) e[HOLD ? k : 0][j] = power;
+        sum += power;
       }
     };
     const T* next_x = static_cast<const T*>(a.logits) + next * a.stride;
+    const auto load_next = [&](int k) {  // nothing if there is no next row
+      if (k < PACKS)
+        raw[k < PACKS ? k : 0] = load(next_x, k, next_n);
+      else
+        rest = row_raw(next_x, next_n / kRound * kRound + (int)place, next_n);
+    };
 #pragma unroll
     for (int k = 0; k < PACKS; ++k) {
-      add(raw[k], e[k]);
-      raw[k] = load(next_x, k, next_n);  // nothing if there is no next row
+      add(raw[k], k);
+      if (HOLD) load_next(k);
     }
-    add(rest, e[PACKS]);
-    rest = row_raw(next_x, next_n / kRound * kRound + (int)place, next_n);
+    add(rest, PACKS);
+    if (HOLD) load_next(PACKS);
     // (a thread or wave without possible states has sum 0 and stays out through the factor 0; NaN stays in)
     const W wave_best = lanes_max<64>(own);
     const W wave_sum = lanes_sum<64>(sum * (own == (W)-INFINITY ? (W)0 : exp_wide(own - wave_best)));
@@ -365,27 +398,37 @@ __global__ void __launch_bounds__(THREADS) rows_in_block(const Rows a) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
       total.sum += sums[turn][w] * (maxima[turn][w] == (W)-INFINITY ? (W)0 : exp_wide(maxima[turn][w] - total.best));
-    const Slope<W> slope = slope_from_total(weight, state >= 0, total);
-    const W factor = (own == (W)-INFINITY ? (W)0 : exp_wide(own - total.best)) * slope.scale * -slope.weight;
+    const Slope<T> slope = slope_from_total<T>(weight, state >= 0, total);
+    const W factor = (own == (W)-INFINITY ? (W)0 : exp_precise<T>(own - total.best)) * slope.scale * -slope.weight;
     T* out = static_cast<T*>(a.gradient) + r * a.gradient_stride;
+    const auto gradient_of = [&](Raw& from, int k) {
+      Pack<T> g;
+      if (HOLD) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) g.v[j] = Value<T>::round(e[HOLD ? k : 0][j] * factor);
+      } else {
+        kept(from);
+        const Pack<T> p = pack_of<T>(from);
+#pragma unroll
+        for (int j = 0; j < V; ++j) g.v[j] = Value<T>::round(exp_precise<T>(Value<T>::widen(p.v[j]) - reference) * factor);
+      }
+      return g;
+    };
     int written = 0;  // states behind which the gradient is 0
     if (state >= 0) {
 #pragma unroll
       for (int k = 0; k < PACKS; ++k) {
-        if ((k + 1) * kRound <= n) {
-          Pack<T> g;
-#pragma unroll
-          for (int j = 0; j < V; ++j) g.v[j] = Value<T>::round(e[k][j] * factor);
-          store_pack_streamed((out + k * kRound) + place, g);
-        }
+        if ((k + 1) * kRound <= n) store_pack_streamed((out + k * kRound) + place, gradient_of(raw[k], k));
+        if (!HOLD) load_next(k);
       }
       const int i = n / kRound * kRound + (int)place;
-      Pack<T> g;
-#pragma unroll
-      for (int j = 0; j < V; ++j) g.v[j] = Value<T>::round(e[PACKS][j] * factor);
-      if (i < n) store_row_pack(out, i, n, g);
+      if (i < n) store_row_pack<false>(out, i, n, gradient_of(rest, PACKS));
       written = n;
+    } else if (!HOLD) {
+#pragma unroll
+      for (int k = 0; k < PACKS; ++k) load_next(k);
     }
+    if (!HOLD) load_next(PACKS);
     for (int i = written + (int)threadIdx.x; i < width; i += THREADS) out[i] = Value<T>::round((W)0);
     if (owner) {
       if (state >= 0) out[state] = Value<T>::round(slope.at(target, true));
@@ -430,11 +473,11 @@ __global__ void __launch_bounds__(THREADS) rows_streamed(const Rows a) {
     if (own.sum != (W)0) own.sum *= exp_wide(own.reference() - total.reference());
     total.sum = block_sum<THREADS>(own.sum, sums);
     if constexpr (MODE == kBoth) {
-      const Slope<W> slope = slope_from_total(row_weight<T>(a, r), state >= 0, total);
+      const Slope<T> slope = slope_from_total<T>(row_weight<T>(a, r), state >= 0, total);
       T* out = static_cast<T*>(a.gradient) + r * a.gradient_stride;
 #pragma unroll 2
       for (int64_t i = (int64_t)threadIdx.x * V; i < a.width; i += THREADS * V)
-        store_row_pack(out, i, a.width, gradient_pack(slope, row_pack(x, i, n), state - i, n - i));
+        store_row_pack<true>(out, i, a.width, gradient_pack(slope, row_pack(x, i, n), state - i, n - i));
     }
     if (threadIdx.x == 0) finish_row<T>(a, r, state >= 0, target, total);
     __syncthreads();  // the next row writes maxima and sums
@@ -461,8 +504,8 @@ __global__ void __launch_bounds__(kBackwardThreads) rows_backward(const Rows a, 
     const Pack<T> p = row_pack(x, i, n);
     const Total<W> total{(W)a.totals[2 * r], (W)a.totals[2 * r + 1]};
     const int64_t state = row_state(a, r, n);
-    const Slope<W> slope = slope_from_total(row_weight<T>(a, r), state >= 0, total);
-    store_row_pack(static_cast<T*>(a.gradient) + r * a.gradient_stride, i, a.width,
+    const Slope<T> slope = slope_from_total<T>(row_weight<T>(a, r), state >= 0, total);
+    store_row_pack<false>(static_cast<T*>(a.gradient) + r * a.gradient_stride, i, a.width,
                    gradient_pack(slope, p, state - i, n - i));
     if (packs - q <= step) return;
     q += step;
@@ -491,19 +534,20 @@ void launch_lanes(const Rows& a, hipStream_t s) {
 
 template <typename T, int LANES, int PACKS, int MODE>
 void launch_short(const Rows& a, hipStream_t s) {
-  constexpr int kKeep = std::min(LANES, PACKS == 1 ? 8 : PACKS == 2 ? 4 : 2);
-  // several rows per group once that leaves every SIMD (1024) four waves
+  constexpr int kKeep = std::min(LANES, PACKS == 4 ? 2 : 4);
+  // several rows per group once that leaves every SIMD (1024) four waves (131072 x 64 float32, forward: 14.6 us at
+  // one row per group, 10.4 at two, 8.9 at four and at eight)
   if (kKeep > 1 && a.rows * LANES >= (int64_t)64 * 4096 * kKeep)
     launch_lanes<T, LANES, PACKS, kKeep, MODE>(a, s);
   else
     launch_lanes<T, LANES, PACKS, 1, MODE>(a, s);
 }
 
-template <typename T, int THREADS, int PACKS>
+template <typename T, int THREADS, int PACKS, bool HOLD = true>
 void launch_block(const Rows& a, hipStream_t s) {
   // as many blocks as the 256 CUs' registers hold at a time
   constexpr int64_t kPerCu = PACKS == 16 ? 1 : PACKS == 8 ? 768 / THREADS : 1024 / THREADS;
-  hipLaunchKernelGGL((rows_in_block<T, THREADS, PACKS>), dim3((uint32_t)std::min<int64_t>(a.rows, 256 * kPerCu)),
+  hipLaunchKernelGGL((rows_in_block<T, THREADS, PACKS, HOLD>), dim3((uint32_t)std::min<int64_t>(a.rows, 256 * kPerCu)),
                      dim3(THREADS), 0, s, a);
 }
 
@@ -524,6 +568,7 @@ int launch_forward(const Rows& a, hipStream_t s) {
   else if (MODE == kBoth && packs <= 256 * 8) launch_block<T, 256, 8>(a, s);
   else if (MODE == kBoth && packs <= 512 * 8) launch_block<T, 512, 8>(a, s);
   else if (MODE == kBoth && packs <= 512 * 16) launch_block<T, 512, 16>(a, s);
+  else if (MODE == kBoth && packs <= 1024 * 16) launch_block<T, 1024, 16, false>(a, s);
   else
     hipLaunchKernelGGL((rows_streamed<T, 512, MODE>), dim3((uint32_t)std::min(a.rows, kMaxBlocks)), dim3(512), 0, s, a);
   BN_HIP_CHECK(hipGetLastError());

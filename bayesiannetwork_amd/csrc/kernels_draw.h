@@ -17,9 +17,9 @@
 // of them are k states of the row), and only the pieces that reach the bound are read again.  Rows that have
 // more than 512 states above the bound are left to a third launch (draw_wide).
 //
-// Cumulative weights decide indices, so weights are doubles everywhere, summed in an order that depends
-// on the row alone.  Bins are filled by atomics, whose order varies: they add integers (the weight times a
-// power of two), whose sum does not.
+// Cumulative weights decide indices, so weights are doubles, summed in an order that depends on the call's
+// sizes alone.  Bins are filled by atomics, whose order varies: they add integers (the weight times a power
+// of two), whose sum does not.
 #pragma once
 
 #include <algorithm>
@@ -623,7 +623,7 @@ __device__ Found find_bin(Lds& lds, Each each, BinOf bin_of, Mass mass, unsigned
   }
   const unsigned long long both = block_all<THREADS>(((unsigned long long)found << 32) | lowest, lds.words, kMinOfHalves);
   const bool reached = (uint32_t)(both >> 32) != ~0u;
-  const int at = reached ? (int)(both >> 32) : kBins - 1 - (int)(uint32_t)both;
+  const int at = reached ? (int)(both >> 32) : kBins - 1 - (int)std::min((uint32_t)both, (uint32_t)kBins - 1);
   if (threadIdx.x == (unsigned)(at / 4)) lds.answer[0] = (long long)(reached ? found_above : lowest_above);
   __syncthreads();
   return {kBins - 1 - at, (unsigned long long)lds.answer[0], lds.count[kBins - 1 - at], reached};
@@ -678,7 +678,7 @@ __device__ int locate(Lds& lds, int segments, double uniform, SumOf sum_of, Weig
   const uint32_t filled = here > 0.0 ? THREADS - 1 - threadIdx.x : ~0u;
   const unsigned long long both = block_all<THREADS>(((unsigned long long)over << 32) | filled, lds.words, kMinOfHalves);
   const bool none = (uint32_t)(both >> 32) == ~0u;
-  const uint32_t owner = none ? THREADS - 1 - (uint32_t)both : (uint32_t)(both >> 32);
+  const uint32_t owner = none ? THREADS - 1 - std::min((uint32_t)both, (uint32_t)THREADS - 1) : (uint32_t)(both >> 32);
   if (threadIdx.x == owner) {
     double before = left;
     int segment = begin;

@@ -58,7 +58,7 @@ def draw_states(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: Se
     if isinstance(top_k, torch.Tensor):
         per_row(top_k, "top_k", (torch.int64, torch.int32), torch.int64)
     elif top_k is not None:
-        if int(top_k) != top_k or not 0 <= top_k < 2**63:
+        if not 0 <= top_k < 2**63 or int(top_k) != top_k:
             raise ValueError(f"top_k must be a whole number that is not negative, not {top_k}")
         filters.top_k = int(top_k)
     if not 0.0 <= filters.temperature < float("inf"):

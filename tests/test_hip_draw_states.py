@@ -249,6 +249,41 @@ def test_rows_that_keep_many_states(states, dtype):
         _check(draw_states(x.cuda(), u.cuda(), **settings), x.double().numpy(), u.numpy(), settings)
 
 
+def test_many_long_rows_that_keep_many_states():
+    """More rows than are shared between blocks, each with settings of its own that leave a flat row nearly
+    whole."""
+    from bayesiannetwork_amd.samplers import draw_states
+
+    gen = torch.Generator().manual_seed(77)
+    rows, states = 530, 16400
+    x = torch.randn((rows, states), generator=gen).bfloat16()
+    u = torch.rand((rows,), generator=gen, dtype=torch.float64)
+    settings = dict(top_p=0.8 + 0.15 * torch.rand((rows,), generator=gen, dtype=torch.float64),
+                    top_k=torch.where(torch.arange(rows) % 5 == 0, 9000, 0))
+    got = draw_states(x.cuda(), u.cuda(), **{k: v.cuda() for k, v in settings.items()})
+    _check(got, x.double().numpy(), u.numpy(), {k: v.numpy() for k, v in settings.items()})
+
+
+@pytest.mark.parametrize("states", [64, 5000, 40000])
+def test_two_streams_at_once(states):
+    from bayesiannetwork_amd.samplers import draw_states
+
+    gen = torch.Generator().manual_seed(states)
+    inputs = [(torch.randn((200, states), generator=gen).cuda(), torch.rand((200,), generator=gen).cuda())
+              for _ in range(2)]
+    want = [draw_states(x, u, top_p=0.9) for x, u in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for k, (x, u) in enumerate(inputs):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(draw_states(x, u, top_p=0.9))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(g, want[k]) for g in got[k])
+
+
 def test_frequencies_of_a_posterior():
     """Draws from a machine's posterior follow it (chi-square, alpha = 0.001)."""
     from scipy import stats

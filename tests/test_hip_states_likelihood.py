@@ -111,7 +111,7 @@ def test_follows_the_definition(n, dtype, ragged):
     assert torch.equal(ll_in.nan_to_num(7.0), ll.nan_to_num(7.0))
 
 
-@pytest.mark.parametrize("n", [70001, 140003])
+@pytest.mark.parametrize("n", [65536, 65537, 70001, 131072, 140003])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
 def test_rows_that_no_block_holds(n, dtype):
     from bayesiannetwork_amd.optimizers import states_log_likelihood, states_log_likelihood_and_gradient
@@ -236,6 +236,42 @@ def test_refusals():
         g.sum().backward()  # once differentiable
     assert states_log_likelihood(x[:0], s[:0]).shape == (0,)
     assert states_log_likelihood_and_gradient(x[:0], s[:0])[1].shape == (0, 4)
+
+
+def test_backward_captured_while_an_eager_graph_lives():
+    """Forward and backward of one leaf captured into a graph and replayed with new logits, with another
+    eager result of the same kind still waiting for its backward."""
+    from bayesiannetwork_amd.optimizers import states_log_likelihood
+
+    gen = torch.Generator().manual_seed(14)
+    x = torch.randn((50, 33), generator=gen).cuda()
+    states = torch.randint(0, 33, (50,), generator=gen).cuda()
+    weights = torch.rand((50,), generator=gen).cuda()
+    other = x.clone().requires_grad_(True)
+    waiting = states_log_likelihood(other, states)  # its backward comes last
+    leaf = x.clone().requires_grad_(True)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        torch.autograd.grad(states_log_likelihood(leaf, states), leaf, grad_outputs=weights)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        ll = states_log_likelihood(leaf, states)
+        (gradient,) = torch.autograd.grad(ll, leaf, grad_outputs=weights)
+    for _ in range(3):
+        with torch.no_grad():
+            leaf.copy_(torch.randn((50, 33), generator=gen))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = leaf.detach().clone().requires_grad_(True)
+        want = states_log_likelihood(eager, states)
+        (want_gradient,) = torch.autograd.grad(want, eager, grad_outputs=weights)
+        assert torch.equal(ll, want) and torch.equal(gradient, want_gradient)
+    (late,) = torch.autograd.grad(waiting, other, grad_outputs=weights)
+    again = x.clone().requires_grad_(True)
+    (want,) = torch.autograd.grad(states_log_likelihood(again, states), again, grad_outputs=weights)
+    assert torch.equal(late, want)
 
 
 @pytest.mark.parametrize("n", [10, 3001, 70001])

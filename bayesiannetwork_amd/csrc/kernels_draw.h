@@ -492,7 +492,7 @@ struct RowState {
 };
 
 // What the blocks that share a row's second and third pass leave for the last one.
-constexpr int kShares = 32;
+constexpr int kShares = 32;  // at most a wave's lanes
 constexpr int kShareThreads = 256;
 constexpr int kRoughBins = 4 * kShareThreads;
 constexpr int kSharedRoom = 4096;  // states around the threshold
@@ -1261,9 +1261,8 @@ __device__ int draw_wide_row(const WideRow<T>& row, const SharedRow* shared, dou
     KeyRange<Key> range{kept.key, row.best, 0ull, 0ull, true};
     bool in_list, whole_list;  // the list holds the threshold's states; all those around it
     if (shared && shared->listed <= kRoom) {
-      double certain = 0.0;
-      for (int c = 0; c < kShares; ++c) certain += shared->certain[c];
-      range.above = (Sum)llrint(certain * scale);
+      const int lane = threadIdx.x & 63;  // one load for all shares, and the same tree in every wave
+      range.above = (Sum)llrint(lanes_sum<64>(lane < kShares ? shared->certain[lane] : 0.0) * scale);
       const uint32_t count = (uint32_t)shared->listed;
       for (uint32_t q = threadIdx.x; q < count; q += THREADS) {
         list.key[q] = (Key)shared->key[q];

@@ -131,8 +131,8 @@ __device__ __forceinline__ Setting row_setting(const Draws& a, int64_t r) {
 // exp((x - best) / T) for x <= best, as 2^t with t = (x - best) log2(e) / T: 2^t = 2^k * 2^f, k = round(t), with
 // a polynomial of degree 9 in f (interpolating (2^f - 1) / f at the Chebyshev nodes of [-1/2, 1/2]: 4e-14
 // relative, exactly 1 at f = 0).  k comes from adding 1.5 * 2^52, whose sum carries it in its low bits, and goes
-// into an exponent by shifting: 17 instructions of the full double rate, none of the conversions and
-// scalings that take four times as long (256 x 131072 bfloat16: block_summaries 36 -> 20 us with it).
+// into an exponent by shifting: 17 of the 30 instructions that block_summaries spends on a state, and it is bound by
+// their issue, 4.6 cycles each (256 x 131072 bfloat16, every row weighed: 35 us).
 struct Weight {
   double best;
   double rate;    // log2(e) / T; T is taken within 1e-290 .. 1e290
@@ -434,8 +434,8 @@ __global__ void __launch_bounds__(kSummaryThreads) block_summaries(const Draws a
     if (start >= n) continue;
     const T* x = static_cast<const T*>(a.logits) + r * a.stride;
     const Setting s = row_setting(a, r);
-    // top-k draws from the k largest alone; greedy rows need no weights at all
-    const bool sums = !s.has_top_k() && s.temperature > 0.0;
+    // top-k draws from the k largest alone, min-p from those near the largest; greedy rows need no weights at all
+    const bool sums = !s.has_top_k() && (s.has_top_p() || s.min_p == 0.0) && s.temperature > 0.0;
     Key* keys = static_cast<Key*>(a.piece_keys) + r * a.pieces_per_row;
     Raw raw[PACKS];
 #pragma unroll
@@ -505,7 +505,7 @@ struct SharedRow {
 };
 
 constexpr int kCandidates = 512;  // states that one wave draws among
-constexpr int kListed = 512;      // blocks they may come from
+constexpr int kListed = 512;      // pieces they may come from
 constexpr int kLongThreads = 256;
 
 template <int THREADS>
@@ -580,7 +580,7 @@ struct Found {
 // The bin in which the count (BY_MASS: the mass) from the top, `above` included, reaches `target`.  each(fn)
 // calls fn(key) for every key there is; bin_of(key) is its bin, ascending with the key, or negative.
 template <bool BY_MASS, typename Lds, typename Each, typename BinOf, typename Mass>
-__device__ Found find_bin(Lds& lds, Each each, BinOf bin_of, Mass mass, unsigned long long above, double target) {
+__device__ __forceinline__ Found find_bin(Lds& lds, Each each, BinOf bin_of, Mass mass, unsigned long long above, double target) {
   constexpr int THREADS = Lds::kThreads, kBins = Lds::kBins;
   __syncthreads();
 #pragma unroll
@@ -639,7 +639,7 @@ struct KeyRange {
 
 // find_bin with as many bins of equal width as there are for the keys of a range; narrows it to the one found.
 template <bool BY_MASS, typename Lds, typename Key, typename Each, typename Mass>
-__device__ void narrow(Lds& lds, KeyRange<Key>& range, Each each, Mass mass, double target) {
+__device__ __forceinline__ void narrow(Lds& lds, KeyRange<Key>& range, Each each, Mass mass, double target) {
   constexpr int kLog = Lds::kThreads == 1024 ? 12 : 10;
   static_assert((1 << kLog) == Lds::kBins, "four bins per thread");
   const Key low = range.low, high = range.high, span = high - low;
@@ -655,11 +655,18 @@ __device__ void narrow(Lds& lds, KeyRange<Key>& range, Each each, Mass mass, dou
   range.reached = f.reached;
 }
 
+// The logit of a floor; 1, below all states' keys, stands for none.
+template <typename W, typename Key>
+__device__ __forceinline__ double floor_value(Key floor) {
+  const double v = floor == 1 ? -INFINITY : (double)KeyOf<W>::value(floor);
+  return v > -INFINITY ? v : -INFINITY;
+}
+
 // Finds the state at which a cumulative sum exceeds its target: segment sums in index order first, then the
 // 64 * PER states of one segment by one wave.  sum_of(segment) is the segment's weight, weight_at(index) a
 // state's (0: not kept).
 template <int PER, typename Lds, typename SumOf, typename WeightAt>
-__device__ int locate(Lds& lds, int segments, double uniform, SumOf sum_of, WeightAt weight_at) {
+__device__ __forceinline__ int locate(Lds& lds, int segments, double uniform, SumOf sum_of, WeightAt weight_at) {
   constexpr int THREADS = Lds::kThreads;
   const int each = (segments + THREADS - 1) / THREADS;
   const int begin = std::min((int)threadIdx.x * each, segments);
@@ -731,22 +738,22 @@ struct LongShared {
     struct {
       unsigned long long mass[kBins];
       uint32_t count[kBins];
-      Key key[kCandidates];
       int32_t index[kCandidates];
       int32_t listed[kListed];
+      uint8_t hits[kListed * kBlock * sizeof(Key) / 32];  // a pack of a listed piece holds four 4-byte keys or two of 8
     };
   };
 };
 
-template <int E, typename Key>
-__device__ __forceinline__ int draw_among(const LongShared<Key>& lds, int count, const Setting& s, const Weight& weight,
-                                          double row_total) {
-  using W = typename std::conditional<sizeof(Key) == 8, double, float>::type;
-  W x[E];
+// The draw by one wave among the states of a list.
+template <int E, typename T>
+__device__ __forceinline__ int draw_among(const T* row, const int32_t* index, int count, const Setting& s,
+                                          const Weight& weight, double row_total) {
+  typename Value<T>::Wide x[E];
 #pragma unroll
   for (int j = 0; j < E; ++j) {
     const int at = (int)(threadIdx.x & 63) * E + j;
-    x[j] = at < count ? KeyOf<W>::value(lds.key[at]) : (W)-INFINITY;
+    x[j] = at < count ? Value<T>::widen(row[index[at]]) : (typename Value<T>::Wide)-INFINITY;
   }
   return draw_in_group<true, 64, E>(x, count, s, weight, row_total);
 }
@@ -754,15 +761,13 @@ __device__ __forceinline__ int draw_among(const LongShared<Key>& lds, int count,
 // One row, by the whole block, from its summaries; the same answer in every thread: the state, -1, or -2 for
 // a row that is left to draw_wide, with what it needs in `state`.
 template <typename T, int PIECE>
-__device__ int draw_row(const Draws& a, int64_t r, LongShared<KeyType<T>>& lds, RowState& state) {
+__device__ __forceinline__ int draw_row(const Draws& a, int64_t r, LongShared<KeyType<T>>& lds, RowState& state) {
   using W = typename Value<T>::Wide;
   using Key = KeyType<T>;
   constexpr int V = Value<T>::kVec;
   constexpr int THREADS = kLongThreads;
   const T* x = static_cast<const T*>(a.logits) + r * a.stride;
-  const Setting s = row_setting(a, r);
-  if (!s.valid) return -1;
-  const int n = (int)s.n;
+  const int n = (int)row_states(a, r);
   const int pieces = (n + PIECE - 1) / PIECE, blocks = (n + kBlock - 1) / kBlock;
   const Key* keys = static_cast<const Key*>(a.piece_keys) + r * a.pieces_per_row;
   const double* sums = a.block_sums + r * a.sums_per_row;
@@ -777,6 +782,8 @@ __device__ int draw_row(const Draws& a, int64_t r, LongShared<KeyType<T>>& lds, 
     least = kMin(least, (unsigned long long)k);
     if (staged) lds.piece_key[b] = k;
   }
+  const Setting s = row_setting(a, r);  // (its loads on their way together with the summaries)
+  if (!s.valid) return -1;
   best = block_all<THREADS>(best, lds.words, kMax);
   if ((Key)best == (Key)~(Key)0) return -1;
   const double largest = (double)KeyOf<W>::value((Key)best);
@@ -863,34 +870,40 @@ __device__ int draw_row(const Draws& a, int64_t r, LongShared<KeyType<T>>& lds, 
     for (int b = begin; b < end; ++b)
       if (key_of(b) >= floor) lds.listed[at++] = b;
     __syncthreads();
-    // V states in each of PIECE / V lanes per listed piece: counts, their prefix sums, then the states in order
-    constexpr int kLanes = PIECE / V, kTogether = 64 / kLanes;
-    const auto load = [&](int q, Key (&k)[V], int* first) {
-      uint32_t hits = 0;
-      *first = 0;
-      if (q < (int)listed) {
-        const int i = lds.listed[q] * PIECE + lane % kLanes * V;
-        *first = i;
-        if (i + V <= n) {
-          const Pack<T> p = load_pack(x + i);
+    // V states in each of PIECE / V lanes per listed piece: which are at or above the floor, as bits, and their
+    // number; prefix sums; then their indices in order.  A block has a SIMD per wave, so that this is bound by a
+    // wave's own instructions and waits: logits are compared, not keys, up to four packs per lane are on their way at
+    // once, and the second half works on the bits alone (row of 500 listed pieces: 15.7 -> 6.5 us).
+    constexpr int kLanes = PIECE / V, kTogether = 64 / kLanes, kStride = THREADS / 64 * kTogether, kAhead = 4;
+    const int part = lane % kLanes, slots = (int)listed * kLanes;
+    const W lowest = (W)floor_value<W>(floor);
+    const auto first_of = [&](int from) { return std::max(std::min(from, n - V), 0); };  // a row's last pack ends with it
+    for (int base = wave * kTogether; base < (int)listed; base += kAhead * kStride) {
+      Raw raw[kAhead];
+      int from[kAhead];
 #pragma unroll
-          for (int j = 0; j < V; ++j) k[j] = KeyOf<W>::key(Value<T>::widen(p.v[j]));
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) k[j] = i + j < n ? key_at(x, i + j) : (Key)0;
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) hits |= (uint32_t)(k[j] >= floor) << j;
+      for (int u = 0; u < kAhead; ++u) {
+        const int q = std::min(base + u * kStride + lane / kLanes, (int)listed - 1);
+        from[u] = lds.listed[q] * PIECE + part * V;
+        raw[u] = raw_of(load_pack(x + first_of(from[u])));
       }
-      return hits;
-    };
-#pragma unroll 2
-    for (int q0 = wave * kTogether; q0 < (int)listed; q0 += THREADS / 64 * kTogether) {
-      const int q = q0 + lane / kLanes;
-      Key k[V];
-      int first;
-      const int hits = lanes_all<kLanes>(__popc(load(q, k, &first)), [](int p, int q) { return p + q; });
-      if (lane % kLanes == 0 && q < (int)listed) lds.count[q] = (uint32_t)hits;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (base + u * kStride >= (int)listed) break;
+        const int q = base + u * kStride + lane / kLanes, first = first_of(from[u]);
+        const Pack<T> p = pack_of<T>(raw[u]);
+        uint32_t hits = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) hits |= (uint32_t)(Value<T>::widen(p.v[j]) >= lowest) << j;
+        hits = hits >> std::min(from[u] - first, V) << std::min(from[u] - first, V);
+        if (n < V) hits &= (1u << n) - 1;
+        if (q >= (int)listed) hits = 0;
+        const int count = lanes_all<kLanes>(__popc(hits), [](int p, int q) { return p + q; });
+        if (q < (int)listed) {
+          lds.hits[q * kLanes + part] = (uint8_t)hits;
+          if (part == 0) lds.count[q] = (uint32_t)count;
+        }
+      }
     }
     __syncthreads();
     constexpr int kPer = kListed / THREADS;
@@ -912,32 +925,25 @@ __device__ int draw_row(const Draws& a, int64_t r, LongShared<KeyType<T>>& lds, 
         }
       }
       __syncthreads();
-#pragma unroll 2
-      for (int q0 = wave * kTogether; q0 < (int)listed; q0 += THREADS / 64 * kTogether) {
-        const int q = q0 + lane / kLanes;
-        Key k[V];
-        int first;
-        const uint32_t hits = load(q, k, &first);
+      for (int base = wave * 64; base < slots; base += THREADS) {
+        const int q = (base + lane) / kLanes;
+        uint32_t hits = base + lane < slots ? lds.hits[base + lane] : 0u;
         int to = lanes_scan<kLanes>((int)__popc(hits)) - (int)__popc(hits);
-        if (hits != 0) to += (int)lds.count[q];
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (hits >> j & 1) {
-            lds.key[to] = k[j];
-            lds.index[to] = first + j;
-            ++to;
-          }
+        if (hits == 0) continue;
+        to += (int)lds.count[q];
+        const int first = first_of(lds.listed[q] * PIECE + part * V);
+        for (; hits != 0; hits &= hits - 1) lds.index[to++] = first + __ffs((int)hits) - 1;
       }
       __syncthreads();
       if (wave == 0) {
         const int count = (int)candidates;
         int slot;
         if (count <= 64)
-          slot = draw_among<1>(lds, count, s, weight, row_total);
+          slot = draw_among<1>(x, lds.index, count, s, weight, row_total);
         else if (count <= 256)
-          slot = draw_among<4>(lds, count, s, weight, row_total);
+          slot = draw_among<4>(x, lds.index, count, s, weight, row_total);
         else
-          slot = draw_among<8>(lds, count, s, weight, row_total);
+          slot = draw_among<8>(x, lds.index, count, s, weight, row_total);
         if (lane == 0) lds.answer[3] = lds.index[slot];
       }
       __syncthreads();
@@ -998,12 +1004,18 @@ struct Steps {
   }
 };
 
-template <typename Key, int THREADS>
+template <typename Key, int ROOM>
 struct Listed {
-  static constexpr int kRoom = 4 * THREADS;
+  static constexpr int kRoom = ROOM;
   Key key[kRoom];
   int32_t index[kRoom];
-  uint32_t count;
+  uint32_t count;  // those that found no room counted too
+  __device__ __forceinline__ void add(int i, Key k) {
+    const uint32_t at = atomicAdd(&count, 1u);
+    if (at >= kRoom) return;
+    key[at] = k;
+    index[at] = i;
+  }
 };
 
 // The states of a prefix of the order: keys above `key`, and those on it up to an index.
@@ -1015,9 +1027,9 @@ struct Prefix {
 };
 
 // The index of the `kept`-th state, in ascending index, on a key; all of them are in the list if `in_list`.
-template <typename T, int THREADS>
-__device__ int last_kept(const T* x, int n, KeyType<T> key, unsigned long long kept, Bins<THREADS>& lds,
-                         const Listed<KeyType<T>, THREADS>& list, bool in_list) {
+template <typename T, int THREADS, int ROOM>
+__device__ __forceinline__ int last_kept(const T* x, int n, KeyType<T> key, unsigned long long kept, Bins<THREADS>& lds,
+                         const Listed<KeyType<T>, ROOM>& list, bool in_list) {
   constexpr int V = Value<T>::kVec;
   if (in_list) {
     const uint32_t count = list.count;
@@ -1028,8 +1040,12 @@ __device__ int last_kept(const T* x, int n, KeyType<T> key, unsigned long long k
     KeyRange<uint32_t> range{~(uint32_t)n, ~0u, 0ull, 0ull, true};
     do {
       narrow<false>(lds, range, each, [](uint32_t) { return 0ull; }, (double)kept);
-    } while (range.low != range.high);
-    return (int)~range.low;
+    } while (range.low != range.high && range.states > 1);
+    each([&](uint32_t i) {
+      if (i >= range.low && i <= range.high) lds.answer[1] = (long long)~i;
+    });
+    __syncthreads();
+    return (int)lds.answer[1];
   }
   unsigned long long seen = 0;
   for (int base = 0; base < n && seen < kept; base += THREADS * V) {
@@ -1070,10 +1086,6 @@ struct WideRow {
   Steps<W> steps;
   double* sums;               // the block sums have served: one entry per segment, what certainly is kept of it,
   unsigned long long* extra;  // and what the states around the threshold add, as integers of 2^-50
-  __device__ __forceinline__ static double floor_value(Key floor) {
-    const double v = floor == 1 ? -INFINITY : (double)KeyOf<W>::value(floor);
-    return v > -INFINITY ? v : -INFINITY;
-  }
   __device__ __forceinline__ WideRow(const Draws& a, int64_t r, const RowState& state, int bins)
       : x(static_cast<const T*>(a.logits) + r * a.stride),
         s(row_setting(a, r)),
@@ -1083,7 +1095,7 @@ struct WideRow {
         floor((Key)state.floor),
         largest((double)KeyOf<W>::value(best)),
         weight(largest, s.temperature),
-        steps(floor_value(floor), largest, s.temperature, bins),
+        steps(floor_value<W>(floor), largest, s.temperature, bins),
         sums(a.block_sums + r * a.sums_per_row),
         extra(reinterpret_cast<unsigned long long*>(sums + segments)) {}
 };
@@ -1092,7 +1104,7 @@ constexpr double kListScale = 1125899906842624.0;  // 2^50: at most 4096 weights
 // Masses by logit of a prefix's states in [begin, end), from weights of single precision.
 constexpr double kRoughScale = 274877906944.0;  // 2^38: 2^24 weights add up within 62 bits
 template <typename T, int THREADS>
-__device__ void add_rough_masses(const WideRow<T>& row, const Prefix<KeyType<T>>& in, int begin, int end,
+__device__ __forceinline__ void add_rough_masses(const WideRow<T>& row, const Prefix<KeyType<T>>& in, int begin, int end,
                                  unsigned long long* mass) {
   using W = typename Value<T>::Wide;
   const float rate = (float)row.weight.rate;
@@ -1109,7 +1121,7 @@ __device__ void add_rough_masses(const WideRow<T>& row, const Prefix<KeyType<T>>
 // (2^24 states of weight 2^-24 double it), so it is off by less than 4e-6 of itself, a fifth of kSlack, and by
 // the integers' rounding.
 template <int THREADS>
-__device__ int2 bins_around(const unsigned long long* mass, double target, int n, unsigned long long* words) {
+__device__ __forceinline__ int2 bins_around(const unsigned long long* mass, double target, int n, unsigned long long* words) {
   constexpr int kBins = 4 * THREADS;
   constexpr double kSlack = 2e-5;
   const double rounding = (double)n + 1.0, goal = target * kRoughScale;
@@ -1135,11 +1147,12 @@ __device__ int2 bins_around(const unsigned long long* mass, double target, int n
 }
 
 // Weights of a prefix's states in the bins above one: their sum over the segments [begin, end), and by segment
-// those that min-p leaves.
-template <typename T, int THREADS>
-__device__ double add_up(const WideRow<T>& row, const Prefix<KeyType<T>>& in, int above, int begin, int end,
-                         unsigned long long* words) {
+// those that min-p leaves.  others(index, key) is called for its states in the bins lowest..above.
+template <typename T, int THREADS, typename Others>
+__device__ __forceinline__ double add_up(const WideRow<T>& row, const Prefix<KeyType<T>>& in, int lowest, int above, int begin, int end,
+                         unsigned long long* words, Others others) {
   using W = typename Value<T>::Wide;
+  using Key = KeyType<T>;
   constexpr int V = Value<T>::kVec;
   const int lane = threadIdx.x & 63;
   const auto load = [&](int q) {
@@ -1166,10 +1179,15 @@ __device__ double add_up(const WideRow<T>& row, const Prefix<KeyType<T>>& in, in
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const W v = Value<T>::widen(p.v[j]);
-      if (in.has(i + j, KeyOf<W>::key(v)) && row.steps.bin(v) > above) {
+      const Key k = KeyOf<W>::key(v);
+      if (!in.has(i + j, k)) continue;
+      const int bin = row.steps.bin(v);
+      if (bin > above) {
         const double w = row.weight((double)v);
         all += w;
         drawn += w >= row.s.min_p ? w : 0.0;
+      } else if (bin >= lowest) {
+        others(i + j, k);
       }
     }
     drawn = lanes_sum<64>(drawn);
@@ -1182,24 +1200,122 @@ __device__ double add_up(const WideRow<T>& row, const Prefix<KeyType<T>>& in, in
   (void)block_scan<THREADS>(all, words, &total);  // (its barriers also publish the segments' sums)
   return total;
 }
+template <typename T, int THREADS>
+__device__ __forceinline__ double add_up(const WideRow<T>& row, const Prefix<KeyType<T>>& in, unsigned long long* words) {
+  return add_up<T, THREADS>(row, in, 0, -1, 0, row.segments, words, [](int, KeyType<T>) {});
+}
+
+// A wide row's last steps: what top-p keeps of a prefix when the states around the threshold are listed, and the draw.
+template <typename T, int THREADS, int ROOM>
+struct Settling {
+  using Key = KeyType<T>;
+  using Sum = unsigned long long;
+  const WideRow<T>& row;
+  Bins<THREADS>& lds;
+  Listed<Key, ROOM>& list;
+  double scale;  // of masses
+  __device__ __forceinline__ Settling(const WideRow<T>& row_, Bins<THREADS>& lds_, Listed<Key, ROOM>& list_)
+      : row(row_), lds(lds_), list(list_), scale(mass_scale(row_.n)) {}
+
+  __device__ __forceinline__ Sum mass(Key k) const { return mass_of(row.weight.of_key(k), scale); }
+  template <typename Fn>
+  __device__ __forceinline__ void each_listed(Fn fn) const {
+    const uint32_t count = list.count;
+    for (uint32_t q = threadIdx.x; q < count; q += THREADS) fn(list.key[q]);
+  }
+
+  // The key at which the mass reaches `reach`, among the listed ones.
+  __device__ __forceinline__ void narrow_listed(KeyRange<Key>& range, double reach) {
+    // the list's own range, which is a bin or two, instead of all keys
+    Sum low = ~0ull, high = 0;
+    each_listed([&](Key k) {
+      low = kMin(low, (Sum)k);
+      high = kMax(high, (Sum)k);
+    });
+    range.low = (Key)block_all<THREADS>(low, lds.words, kMin);
+    range.high = (Key)block_all<THREADS>(high, lds.words, kMax);
+    do {
+      narrow<true>(lds, range, [&](auto fn) { each_listed(fn); }, [&](Key k) { return mass(k); }, reach);
+    } while (range.low != range.high);
+  }
+
+  // Ends `kept` in the states on the range's key: those with less than the target before them, one at least.
+  __device__ __forceinline__ void end_on_key(Prefix<Key>& kept, const KeyRange<Key>& range, double reach, bool in_list) {
+    const double each = (double)mass(range.low), above = (double)range.above;
+    Sum ties = range.states;
+    if (each > 0.0) ties = (Sum)fmin(fmax(ceil((reach - above) / each), 1.0), (double)range.states);
+    while (ties > 1 && above + (double)(ties - 1) * each >= reach) --ties;
+    while (ties < range.states && above + (double)ties * each < reach) ++ties;
+    const int bound = range.low == kept.key ? kept.last : row.n;
+    kept.key = range.low;
+    kept.last = ties < range.states ? last_kept<T>(row.x, row.n, range.low, ties, lds, list, in_list) : bound;
+  }
+
+  // The segments hold what lies above the bins around the threshold, the list what lies in them.
+  __device__ __forceinline__ void add_listed(const Prefix<Key>& kept) {
+    const uint32_t count = list.count;
+    for (uint32_t q = threadIdx.x; q < count; q += THREADS)
+      if (kept.has(list.index[q], list.key[q])) {
+        const double w = row.weight.of_key(list.key[q]);
+        if (w >= row.s.min_p) atomicAdd(&row.extra[list.index[q] / WideRow<T>::kSegment], mass_of(w, kListScale));
+      }
+  }
+
+  // The state drawn from a prefix, once the segments' sums are there.
+  __device__ __forceinline__ int drawn(const Prefix<Key>& kept) {
+    __syncthreads();
+    return locate<WideRow<T>::V>(
+        lds, row.segments, row.s.uniform,
+        [&](int q) {
+          const Sum more = __hip_atomic_load(&row.extra[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          return row.sums[q] + (double)more / kListScale;
+        },
+        [&](int i) {
+          if (i >= row.n) return 0.0;
+          const Key k = key_at(row.x, std::min(i, row.n - 1));
+          const double w = kept.has(i, k) ? row.weight.of_key(k) : 0.0;
+          return w >= row.s.min_p ? w : 0.0;
+        });
+  }
+};
+
+// A row with top-p alone whose passes the blocks of draw_wide_masses and draw_wide_sums have shared, from what these
+// have left.
+template <typename T, int THREADS>
+__device__ __forceinline__ int draw_shared_row(const WideRow<T>& row, const SharedRow& shared, double row_total, Bins<THREADS>& lds,
+                               Listed<KeyType<T>, kSharedRoom>& list) {
+  using Key = KeyType<T>;
+  Settling<T, THREADS, kSharedRoom> settling(row, lds, list);
+  const int lane = threadIdx.x & 63;  // one load for all shares, and the same tree in every wave
+  const double certain = lanes_sum<64>(lane < kShares ? shared.certain[lane] : 0.0);
+  const uint32_t count = (uint32_t)shared.listed;
+  for (uint32_t q = threadIdx.x; q < count; q += THREADS) {
+    list.key[q] = (Key)shared.key[q];
+    list.index[q] = shared.index[q];
+  }
+  if (threadIdx.x == 0) list.count = count;
+  __syncthreads();
+  Prefix<Key> kept{row.floor, row.n};
+  KeyRange<Key> range{row.floor, row.best, (unsigned long long)llrint(certain * settling.scale), 0ull, true};
+  const double reach = row.s.top_p * row_total * settling.scale;
+  settling.narrow_listed(range, reach);
+  settling.end_on_key(kept, range, reach, true);
+  settling.add_listed(kept);
+  return settling.drawn(kept);
+}
 
 // One row by the whole block, over the row in memory: one pass weighs its states roughly, by logit, a second
 // one adds up what is certainly kept, and the few thousand states around the threshold are settled in LDS.
-// Where the blocks of draw_wide_masses and draw_wide_sums have shared those passes, `shared` holds their results.
-template <typename T, int THREADS>
-__device__ int draw_wide_row(const WideRow<T>& row, const SharedRow* shared, double row_total, Bins<THREADS>& lds,
-                             Listed<KeyType<T>, THREADS>& list) {
+template <typename T, int THREADS, int ROOM>
+__device__ __forceinline__ int draw_wide_row(const WideRow<T>& row, double row_total, Bins<THREADS>& lds, Listed<KeyType<T>, ROOM>& list) {
   using W = typename Value<T>::Wide;
   using Key = KeyType<T>;
   using Sum = unsigned long long;
-  constexpr int V = Value<T>::kVec;
-  constexpr uint32_t kRoom = Listed<Key, THREADS>::kRoom;
   const Setting& s = row.s;
-  const Weight& weight = row.weight;
   const int n = row.n;
   const T* x = row.x;
-  const double scale = mass_scale(n);
-  const auto mass = [&](Key k) { return mass_of(weight.of_key(k), scale); };
+  Settling<T, THREADS, ROOM> settling(row, lds, list);
+  const auto mass = [&](Key k) { return settling.mass(k); };
   const auto no_mass = [](auto) { return 0ull; };
 
   // the states of a prefix in bins lowest..highest, by key
@@ -1211,23 +1327,19 @@ __device__ int draw_wide_row(const WideRow<T>& row, const SharedRow* shared, dou
       if (in.has(i, k)) fn(i, k);
     });
   };
-  const auto fill_list = [&](const Prefix<Key>& in, int lowest, int highest, Key low, Key high) {
+  const auto clear_list = [&]() {
     __syncthreads();
     if (threadIdx.x == 0) list.count = 0;
     __syncthreads();
+  };
+  const auto fill_list = [&](const Prefix<Key>& in, int lowest, int highest, Key low, Key high) {
+    clear_list();
     each_in(in, lowest, highest, [&](int i, Key k) {
-      if (k < low || k > high) return;
-      const uint32_t at = atomicAdd(&list.count, 1u);
-      if (at >= kRoom) return;
-      list.key[at] = k;
-      list.index[at] = i;
+      if (k >= low && k <= high) list.add(i, k);
     });
     __syncthreads();
   };
-  const auto each_listed = [&](auto fn) {
-    const uint32_t count = list.count;
-    for (uint32_t q = threadIdx.x; q < count; q += THREADS) fn(list.key[q]);
-  };
+  const auto each_listed = [&](auto fn) { settling.each_listed(fn); };
 
   // ---- top-k: the k-th key by counting
   Prefix<Key> kept{row.floor, n};
@@ -1243,116 +1355,85 @@ __device__ int draw_wide_row(const WideRow<T>& row, const SharedRow* shared, dou
     const auto each_key = [&](auto fn) {
       each_in(all, f.bin, f.bin, [&](int, Key k) { fn(k); });
     };
-    while (range.low != range.high && range.states > kRoom) narrow<false>(lds, range, each_key, no_mass, (double)s.top_k);
-    const bool in_list = range.states <= kRoom;
+    while (range.low != range.high && range.states > ROOM) narrow<false>(lds, range, each_key, no_mass, (double)s.top_k);
+    const bool in_list = range.states <= ROOM;
     if (in_list) {
       fill_list(all, f.bin, f.bin, range.low, range.high);
       while (range.low != range.high) narrow<false>(lds, range, each_listed, no_mass, (double)s.top_k);
     }
     kept.key = range.low;
     const Sum ties = (Sum)s.top_k - range.above;
-    if (ties < range.states) kept.last = last_kept<T, THREADS>(x, n, range.low, ties, lds, list, in_list);
+    if (ties < range.states) kept.last = last_kept<T>(x, n, range.low, ties, lds, list, in_list);
   }
 
   bool added = false;
   if (s.has_top_p()) {
-    const double target = s.top_p * (s.has_top_k() ? add_up<T, THREADS>(row, kept, -1, 0, row.segments, lds.words) : row_total);
-    const double reach = target * scale;
-    KeyRange<Key> range{kept.key, row.best, 0ull, 0ull, true};
-    bool in_list, whole_list;  // the list holds the threshold's states; all those around it
-    if (shared && shared->listed <= kRoom) {
-      const int lane = threadIdx.x & 63;  // one load for all shares, and the same tree in every wave
-      range.above = (Sum)llrint(lanes_sum<64>(lane < kShares ? shared->certain[lane] : 0.0) * scale);
-      const uint32_t count = (uint32_t)shared->listed;
-      for (uint32_t q = threadIdx.x; q < count; q += THREADS) {
-        list.key[q] = (Key)shared->key[q];
-        list.index[q] = shared->index[q];
-      }
-      if (threadIdx.x == 0) list.count = count;
-      __syncthreads();
-      in_list = whole_list = true;
-    } else {
-      __syncthreads();
+    const double target = s.top_p * (s.has_top_k() ? add_up<T, THREADS>(row, kept, lds.words) : row_total);
+    const double reach = target * settling.scale;
+    __syncthreads();
 #pragma unroll
-      for (int b = 0; b < 4; ++b) lds.mass[b * THREADS + threadIdx.x] = 0;
-      __syncthreads();
-      add_rough_masses<T, THREADS>(row, kept, 0, n, lds.mass);
-      __syncthreads();
-      const int2 around = bins_around<THREADS>(lds.mass, target, n, lds.words);
-      range.above = (Sum)llrint(add_up<T, THREADS>(row, kept, around.y, 0, row.segments, lds.words) * scale);
-      fill_list(kept, around.x, around.y, range.low, range.high);
-      in_list = whole_list = list.count <= kRoom;
-      if (!in_list) {
-        const auto each_key = [&](auto fn) {
-          each_in(kept, around.x, around.y, [&](int, Key k) { fn(k); });
-        };
-        do {
-          narrow<true>(lds, range, each_key, mass, reach);
-        } while (range.low != range.high && range.states > kRoom);
-        in_list = range.states <= kRoom;
-        if (in_list) fill_list(kept, around.x, around.y, range.low, range.high);
-      }
-    }
-    if (in_list) {
-      // the list's own range, which is a bin or two, instead of all keys
-      Sum low = ~0ull, high = 0;
-      each_listed([&](Key k) {
-        low = kMin(low, (Sum)k);
-        high = kMax(high, (Sum)k);
-      });
-      range.low = (Key)block_all<THREADS>(low, lds.words, kMin);
-      range.high = (Key)block_all<THREADS>(high, lds.words, kMax);
+    for (int b = 0; b < 4; ++b) lds.mass[b * THREADS + threadIdx.x] = 0;
+    __syncthreads();
+    add_rough_masses<T, THREADS>(row, kept, 0, n, lds.mass);
+    __syncthreads();
+    const int2 around = bins_around<THREADS>(lds.mass, target, n, lds.words);
+    clear_list();
+    const double certain = add_up<T, THREADS>(row, kept, around.x, around.y, 0, row.segments, lds.words,
+                                              [&](int i, Key k) { list.add(i, k); });
+    KeyRange<Key> range{kept.key, row.best, (Sum)llrint(certain * settling.scale), 0ull, true};
+    const bool whole_list = list.count <= ROOM;  // the list holds all those around the threshold
+    bool in_list = whole_list;                   // ... those on its key
+    if (!in_list) {
+      const auto each_key = [&](auto fn) {
+        each_in(kept, around.x, around.y, [&](int, Key k) { fn(k); });
+      };
       do {
-        narrow<true>(lds, range, each_listed, mass, reach);
-      } while (range.low != range.high);
+        narrow<true>(lds, range, each_key, mass, reach);
+      } while (range.low != range.high && range.states > ROOM);
+      in_list = range.states <= ROOM;
+      if (in_list) fill_list(kept, around.x, around.y, range.low, range.high);
     }
-    // of the states on the key: those with less than the target before them, one at least
-    const double each = (double)mass(range.low), above = (double)range.above;
-    Sum ties = range.states;
-    if (each > 0.0) ties = (Sum)fmin(fmax(ceil((reach - above) / each), 1.0), (double)range.states);
-    while (ties > 1 && above + (double)(ties - 1) * each >= reach) --ties;
-    while (ties < range.states && above + (double)ties * each < reach) ++ties;
-    const int bound = range.low == kept.key ? kept.last : n;
-    kept.key = range.low;
-    kept.last = ties < range.states ? last_kept<T, THREADS>(x, n, range.low, ties, lds, list, in_list) : bound;
-    if (whole_list) {
-      // the segments hold what lies above the bins, the list what lies in them
-      const uint32_t count = list.count;
-      for (uint32_t q = threadIdx.x; q < count; q += THREADS)
-        if (kept.has(list.index[q], list.key[q])) {
-          const double w = weight.of_key(list.key[q]);
-          if (w >= s.min_p) atomicAdd(&row.extra[list.index[q] / WideRow<T>::kSegment], mass_of(w, kListScale));
-        }
-      __threadfence();
-      added = true;
-    }
+    if (in_list) settling.narrow_listed(range, reach);
+    settling.end_on_key(kept, range, reach, in_list);
+    if (whole_list) settling.add_listed(kept);
+    added = whole_list;
   }
-  if (!added) (void)add_up<T, THREADS>(row, kept, -1, 0, row.segments, lds.words);
-  __syncthreads();
-  return locate<V>(
-      lds, row.segments, s.uniform,
-      [&](int q) {
-        const Sum more = __hip_atomic_load(&row.extra[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        return row.sums[q] + (double)more / kListScale;
-      },
-      [&](int i) {
-        if (i >= n) return 0.0;
-        const Key k = key_at(x, std::min(i, n - 1));
-        const double w = kept.has(i, k) ? weight.of_key(k) : 0.0;
-        return w >= s.min_p ? w : 0.0;
-      });
+  if (!added) (void)add_up<T, THREADS>(row, kept, lds.words);
+  return settling.drawn(kept);
 }
 
+// A row whose passes were shared is left with short lists, over which fewer waves meet sooner: the others of its
+// block end (serving batch of 256 x 131072: 30 -> 14.5 us).
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS) draw_wide(const Draws a, int64_t first_row) {
-  __shared__ Bins<THREADS> lds;
-  __shared__ Listed<KeyType<T>, THREADS> list;
+  using Key = KeyType<T>;
+  constexpr bool kMayShare = THREADS > kShareThreads;
+  constexpr int kSharedList = kMayShare ? kSharedRoom : 1;
+  __shared__ union {
+    struct {
+      Bins<THREADS> lds;
+      Listed<Key, 4 * THREADS> list;
+    } whole;
+    struct {
+      Bins<kShareThreads> lds;
+      Listed<Key, kSharedList> list;
+    } shared;
+  } space;
   const int64_t r = first_row + blockIdx.x;
   const RowState state = a.row_states[r];
   if (!state.pending) return;
+  if constexpr (kMayShare) {
+    const Setting s = row_setting(a, r);
+    if (a.shared && s.has_top_p() && !s.has_top_k() && a.shared[r].listed <= (unsigned long long)kSharedRoom) {
+      if (threadIdx.x >= kShareThreads) return;
+      const WideRow<T> row(a, r, state, kRoughBins);
+      const int drawn = draw_shared_row<T, kShareThreads>(row, a.shared[r], state.total, space.shared.lds, space.shared.list);
+      if (threadIdx.x == 0) a.out[r] = drawn;
+      return;
+    }
+  }
   const WideRow<T> row(a, r, state, Bins<THREADS>::kBins);
-  const bool prepared = a.shared && row.s.has_top_p() && !row.s.has_top_k();
-  const int drawn = draw_wide_row<T, THREADS>(row, prepared ? a.shared + r : nullptr, state.total, lds, list);
+  const int drawn = draw_wide_row<T>(row, state.total, space.whole.lds, space.whole.list);
   if (threadIdx.x == 0) a.out[r] = drawn;
 }
 
@@ -1379,9 +1460,10 @@ __global__ void __launch_bounds__(kShareThreads) draw_wide_masses(const Draws a)
 
 template <typename T>
 __global__ void __launch_bounds__(kShareThreads) draw_wide_sums(const Draws a) {
-  using W = typename Value<T>::Wide;
   using Key = KeyType<T>;
-  __shared__ unsigned long long words[kShareThreads / 64];
+  constexpr int kRoom = 1024;
+  __shared__ unsigned long long words[kShareThreads / 64], base;
+  __shared__ Listed<Key, kRoom> list;
   const int64_t r = blockIdx.x / kShares;
   const int share = blockIdx.x % kShares;
   const RowState state = a.row_states[r];
@@ -1393,19 +1475,22 @@ __global__ void __launch_bounds__(kShareThreads) draw_wide_sums(const Draws a) {
   const int each = (row.segments + kShares - 1) / kShares;
   const int begin = std::min(share * each, row.segments), end = std::min(begin + each, row.segments);
   const Prefix<Key> in{row.floor, row.n};
-  const double certain = add_up<T, kShareThreads>(row, in, around.y, begin, end, words);
-  if (threadIdx.x == 0) shared.certain[share] = certain;
-  for_each_state<T, kShareThreads>(row.x, std::min(begin * WideRow<T>::kSegment, row.n),
-                                   std::min(end * WideRow<T>::kSegment, row.n), [&](int i, W v) {
-    const int bin = row.steps.bin(v);
-    if (bin < around.x || bin > around.y) return;
-    const Key k = KeyOf<W>::key(v);
-    if (!in.has(i, k)) return;
-    const unsigned long long at = atomicAdd(&shared.listed, 1ull);
-    if (at >= kSharedRoom) return;
-    shared.key[at] = (uint64_t)k;
-    shared.index[at] = i;
-  });
+  if (threadIdx.x == 0) list.count = 0;
+  __syncthreads();
+  const double certain = add_up<T, kShareThreads>(row, Prefix<Key>{row.floor, row.n}, around.x, around.y, begin, end, words,
+                                                  [&](int i, Key k) { list.add(i, k); });
+  // the share's states around the threshold go behind those of the shares before
+  if (threadIdx.x == 0) {
+    shared.certain[share] = certain;
+    base = atomicAdd(&shared.listed, list.count > kRoom ? kSharedRoom + 1ull : (unsigned long long)list.count);
+  }
+  __syncthreads();
+  const uint32_t count = list.count;
+  if (count > kRoom || base + count > kSharedRoom) return;  // draw_wide sees from their number that some are missing
+  for (uint32_t q = threadIdx.x; q < count; q += kShareThreads) {
+    shared.key[base + q] = (uint64_t)list.key[q];
+    shared.index[base + q] = list.index[q];
+  }
 }
 
 constexpr int64_t kMaxStates = 1 << 24;

@@ -168,6 +168,14 @@ struct Weight {
     return p * __hiloint2double((int)((k + 1023u) << 20), 0);
   }
   __device__ __forceinline__ double operator()(double x) const { return at(x); }
+  // In single precision.  Three roundings of t (the difference, the rate, their product) and the exponential's own:
+  // wrong by less than (3 * ln 2 * |t| + 4) * 2^-24 of the weight, and 0 below 2^-126.  Rates beyond 1e30 either way
+  // are left to doubles.
+  template <typename W>
+  __device__ __forceinline__ float rough(W x) const {
+    return __builtin_amdgcn_exp2f((float)(x - (W)best) * (float)rate);
+  }
+  __device__ __forceinline__ bool rough_is_usable() const { return rate > 1e-30 && rate < 1e30; }
   template <typename Key>
   __device__ __forceinline__ double of_key(Key k) const;
 };
@@ -258,6 +266,105 @@ __device__ __forceinline__ void sort_group(W (&c)[E], int lane) {
   }
 }
 
+// Sums over a row's weights in R.  Doubles decide every comparison; floats, at a quarter of the cost, those that are
+// not close, and tell where one is, so that the wave makes it again in doubles.  Of a sum of G * E <= 2048 floats the
+// weights' errors make (3 * ln 2 * 11 + 4) * 2^-24 at most (the mean |t| of weights that are shares of a sum with a 1
+// in it stays below log2 of their number), its additions 2 E + 6 roundings, and both sides of a comparison have them.
+template <typename R, int E>
+struct Sums {
+  static constexpr bool kRough = sizeof(R) == 4;
+  static constexpr R kSlack = kRough ? (R)((80 + 4 * E) * 0x1p-24) : (R)0;
+  template <typename W>
+  __device__ __forceinline__ static R weight_of(const Weight& weight, W x) {
+    if constexpr (kRough)
+      return weight.rough(x);
+    else
+      return weight.template at<true>((double)x);
+  }
+  // (a NaN is close to anything)
+  __device__ __forceinline__ static bool close(R a, R b, R within) { return kRough && !(fabs(a - b) > within); }
+};
+
+// The prefix of an order that top-p keeps: its length and the last one's logit in this lane.  Returns whether a float
+// is too close to tell.
+template <typename R, int G, int E, typename W>
+__device__ __forceinline__ bool keep_share(const W (&c)[E], int top, const Setting& s, const Weight& weight,
+                                           double row_total, int* length, W* last) {
+  using S = Sums<R, E>;
+  const int lane = threadIdx.x % G;
+  R w[E], here = 0, all;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    w[j] = lane * E + j < top ? S::weight_of(weight, c[j]) : (R)0;
+    here += w[j];
+  }
+  R before = group_scan<G>(here, &all);
+  const double whole = row_total >= 0.0 ? row_total : (double)all;
+  const R target = (R)(s.top_p * whole), within = S::kSlack * (R)whole;
+  bool close = false;
+  *length = 0;
+  *last = INFINITY;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    const int at = lane * E + j;
+    // those with less than the target before them, and the first one in any case
+    const bool kept = at < top && (at == 0 || before < target);
+    close |= at < top && at > 0 && S::close(before, target, within);
+    *length += kept;
+    *last = kept ? c[j] : *last;
+    before += w[j];
+  }
+  return close;
+}
+
+// The draw among the states above a threshold, the first `ties` of those on it, and at least min-p of the largest
+// weight: the slot, or -1 if a float is too close to tell (or none is left).
+template <typename R, bool FILTER, int G, int E, typename W>
+__device__ __forceinline__ int draw_kept(const W (&x)[E], const Setting& s, const Weight& weight, W threshold, int ties) {
+  using S = Sums<R, E>;
+  const int lane = threadIdx.x % G;
+  int on_threshold = 0;
+  if (FILTER) {  // ties are kept in the order of their slots
+#pragma unroll
+    for (int j = 0; j < E; ++j) on_threshold += x[j] == threshold;
+    on_threshold = lanes_scan<G>(on_threshold) - on_threshold;  // in the lanes before
+  }
+  const R min_p = (R)s.min_p;
+  bool close = false;
+  R w[E], here = 0, all;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    w[j] = S::weight_of(weight, x[j]);
+    bool kept = w[j] >= min_p;
+    close |= s.min_p > 0.0 && S::close(w[j], min_p, (R)2e-5 * min_p);  // |t| is below 126
+    if (FILTER) {
+      const bool tie = x[j] == threshold;
+      kept = kept && (x[j] > threshold || (tie && on_threshold < ties));
+      on_threshold += tie;
+    }
+    if (!kept) w[j] = 0;
+    here += w[j];
+  }
+  R upto = group_scan<G>(here, &all);
+  const R target = (R)(s.uniform * (double)all), within = S::kSlack * all;
+  close |= S::close(target, 0, within);
+  int pick = INT32_MAX, last = -1;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    upto += w[j];
+    if (w[j] > 0) {
+      close |= S::close(upto, target, within);
+      last = lane * E + j;
+      if (upto > target && pick == INT32_MAX) pick = last;
+    }
+  }
+  if (S::kRough && close) pick = -1;
+  pick = lanes_all<G>(pick, [](int p, int q) { return p < q ? p : q; });
+  if (S::kRough) return pick == INT32_MAX ? -1 : pick;
+  last = lanes_all<G>(last, [](int p, int q) { return p > q ? p : q; });
+  return pick == INT32_MAX ? last : pick;  // u = 1, or the sums' rounding: the last kept state
+}
+
 // The draw among `count` states held by a group of lanes, x[j] of slot lane * E + j (-inf beyond the count);
 // slots ascend with the states' indices.  `row_total`: the weight that top-p is a share of, when top-k is off
 // and states outside the group hold some of it; negative: the group's.  Returns the slot, the same in every
@@ -267,6 +374,7 @@ __device__ int draw_in_group(const W (&x)[E], int count, const Setting& s, const
   const int lane = threadIdx.x % G;
   const auto least = [](W p, W q) { return fmin(p, q); };
   const auto add = [](int p, int q) { return p + q; };
+  const bool usable = weight.rough_is_usable();
   W threshold = -INFINITY;
   int ties = INT32_MAX;  // states on the threshold that are kept
   // rows of one wave differ in their settings: the wave sorts if any of them has to
@@ -281,23 +389,9 @@ __device__ int draw_in_group(const W (&x)[E], int count, const Setting& s, const
     int length = 0;
     W last = INFINITY;
     if (__any(s.has_top_p())) {
-      double w[E], here = 0.0, all;
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        w[j] = lane * E + j < top ? weight.template at<true>((double)c[j]) : 0.0;
-        here += w[j];
-      }
-      double before = group_scan<G>(here, &all);
-      const double target = s.top_p * (row_total >= 0.0 ? row_total : all);
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const int at = lane * E + j;
-        // those with less than the target before them, and the first one in any case
-        const bool kept = at < top && (at == 0 || before < target);
-        length += kept;
-        last = kept ? c[j] : last;
-        before += w[j];
-      }
+      const bool close = keep_share<float, G, E>(c, top, s, weight, row_total, &length, &last);
+      if (__any((close || !usable) && s.has_top_p()))
+        keep_share<double, G, E>(c, top, s, weight, row_total, &length, &last);
     } else {
 #pragma unroll
       for (int j = 0; j < E; ++j) {
@@ -317,39 +411,9 @@ __device__ int draw_in_group(const W (&x)[E], int count, const Setting& s, const
       ties = length - above;
     }
   }
-  int on_threshold = 0;
-  if (FILTER) {  // ties are kept in the order of their slots
-#pragma unroll
-    for (int j = 0; j < E; ++j) on_threshold += x[j] == threshold;
-    on_threshold = lanes_scan<G>(on_threshold) - on_threshold;  // in the lanes before
-  }
-  double w[E], here = 0.0, all;
-#pragma unroll
-  for (int j = 0; j < E; ++j) {
-    w[j] = weight.template at<true>((double)x[j]);
-    bool kept = w[j] >= s.min_p;
-    if (FILTER) {
-      const bool tie = x[j] == threshold;
-      kept = kept && (x[j] > threshold || (tie && on_threshold < ties));
-      on_threshold += tie;
-    }
-    if (!kept) w[j] = 0.0;
-    here += w[j];
-  }
-  double upto = group_scan<G>(here, &all);
-  const double target = s.uniform * all;
-  int pick = INT32_MAX, last = -1;
-#pragma unroll
-  for (int j = 0; j < E; ++j) {
-    upto += w[j];
-    if (w[j] > 0.0) {
-      last = lane * E + j;
-      if (upto > target && pick == INT32_MAX) pick = last;
-    }
-  }
-  pick = lanes_all<G>(pick, [](int p, int q) { return p < q ? p : q; });
-  last = lanes_all<G>(last, [](int p, int q) { return p > q ? p : q; });
-  return pick == INT32_MAX ? last : pick;  // u = 1, or the sums' rounding: the last kept state
+  const int pick = draw_kept<float, FILTER, G, E>(x, s, weight, threshold, ties);
+  if (!__any(pick < 0 || !usable)) return pick;
+  return draw_kept<double, FILTER, G, E>(x, s, weight, threshold, ties);
 }
 
 // The lowest slot that holds `best`.
@@ -377,12 +441,12 @@ __global__ void __launch_bounds__(kShortThreads) draw_short(const Draws a, int64
   const Setting s = row_setting(a, r);
   const int n = (int)s.n, first = lane * E;
   W x[E];
-  if (E >= V && first + E <= n) {
+  if (E >= V && first + E <= a.width) {  // a shorter row has room behind it
 #pragma unroll
     for (int k = 0; k + V <= E; k += V) {
       const Pack<T> p = load_pack(row + first + k);
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[k + j] = Value<T>::widen(p.v[j]);
+      for (int j = 0; j < V; ++j) x[k + j] = first + k + j < n ? Value<T>::widen(p.v[j]) : (W)-INFINITY;
     }
   } else {
 #pragma unroll
@@ -1107,11 +1171,9 @@ template <typename T, int THREADS>
 __device__ __forceinline__ void add_rough_masses(const WideRow<T>& row, const Prefix<KeyType<T>>& in, int begin, int end,
                                  unsigned long long* mass) {
   using W = typename Value<T>::Wide;
-  const float rate = (float)row.weight.rate;
   for_each_state<T, THREADS>(row.x, begin, end, [&](int i, W v) {
     if (!in.has(i, KeyOf<W>::key(v))) return;
-    const float rough = __builtin_amdgcn_exp2f((float)((double)v - row.largest) * rate);
-    atomicAdd(&mass[row.steps.bin(v)], mass_of((double)rough, kRoughScale));
+    atomicAdd(&mass[row.steps.bin(v)], mass_of((double)row.weight.rough(v), kRoughScale));
   });
 }
 

@@ -217,20 +217,28 @@ __device__ __forceinline__ void order(double& a, double& b) {
   b = lo;
 }
 
+// The larger of two where `keep` is +infinity, the smaller where it is -infinity.
+__device__ __forceinline__ float one_of(float a, float b, float keep) {
+  float out;
+  asm("v_med3_f32 %0, %1, %2, %3" : "=v"(out) : "v"(a), "v"(b), "v"(keep));
+  return out;
+}
+__device__ __forceinline__ double one_of(double a, double b, double keep) {
+  order(a, b);
+  return keep > 0.0 ? a : b;
+}
+
 template <int MASK, int E, bool MIRROR, typename W>
 __device__ __forceinline__ void exchange_lanes(W (&c)[E], bool lower) {
+  const W keep = lower ? INFINITY : -INFINITY;
   // two at a time, since a mirrored pair reads each other's place
   static_assert(!MIRROR || E == 1 || E % 2 == 0, "mirrored in pairs");
 #pragma unroll
   for (int j = 0; j < (E + 1) / 2; ++j) {
     const int k = E - 1 - j;
-    W at_j = lane_xor<MASK>(c[MIRROR ? k : j]), at_k = lane_xor<MASK>(c[MIRROR ? j : k]);
-    order(c[j], at_j);
-    if (!lower) c[j] = at_j;
-    if (k != j) {
-      order(c[k], at_k);
-      if (!lower) c[k] = at_k;
-    }
+    const W at_j = lane_xor<MASK>(c[MIRROR ? k : j]), at_k = lane_xor<MASK>(c[MIRROR ? j : k]);
+    c[j] = one_of(c[j], at_j, keep);
+    if (k != j) c[k] = one_of(c[k], at_k, keep);
   }
 }
 
@@ -281,8 +289,6 @@ struct Sums {
     else
       return weight.template at<true>((double)x);
   }
-  // (a NaN is close to anything)
-  __device__ __forceinline__ static bool close(R a, R b, R within) { return kRough && !(fabs(a - b) > within); }
 };
 
 // The prefix of an order that top-p keeps: its length and the last one's logit in this lane.  Returns whether a float
@@ -291,40 +297,41 @@ template <typename R, int G, int E, typename W>
 __device__ __forceinline__ bool keep_share(const W (&c)[E], int top, const Setting& s, const Weight& weight,
                                            double row_total, int* length, W* last) {
   using S = Sums<R, E>;
-  const int lane = threadIdx.x % G;
+  const int lane = threadIdx.x % G, mine = top - lane * E;
   R w[E], here = 0, all;
 #pragma unroll
   for (int j = 0; j < E; ++j) {
-    w[j] = lane * E + j < top ? S::weight_of(weight, c[j]) : (R)0;
+    w[j] = j < mine ? S::weight_of(weight, c[j]) : (R)0;
     here += w[j];
   }
   R before = group_scan<G>(here, &all);
   const double whole = row_total >= 0.0 ? row_total : (double)all;
-  const R target = (R)(s.top_p * whole), within = S::kSlack * (R)whole;
-  bool close = false;
+  const R target = (R)(s.top_p * whole);
+  R nearest = lane == 0 ? (R)INFINITY : fabs(before - target);
   *length = 0;
   *last = INFINITY;
 #pragma unroll
   for (int j = 0; j < E; ++j) {
-    const int at = lane * E + j;
     // those with less than the target before them, and the first one in any case
-    const bool kept = at < top && (at == 0 || before < target);
-    close |= at < top && at > 0 && S::close(before, target, within);
+    const bool kept = j < mine && ((j == 0 && lane == 0) || before < target);
     *length += kept;
     *last = kept ? c[j] : *last;
     before += w[j];
+    if (S::kRough) nearest = fmin(nearest, fabs(before - target));
   }
-  return close;
+  return S::kRough && !(nearest > S::kSlack * (R)whole);  // a NaN is close to anything
 }
 
-// The draw among the states above a threshold, the first `ties` of those on it, and at least min-p of the largest
-// weight: the slot, or -1 if a float is too close to tell (or none is left).
-template <typename R, bool FILTER, int G, int E, typename W>
+// The draw among the states of at least min-p of the largest weight that are kept: all of them (kAll), those down to
+// a threshold, or those above it and the first `ties` of those on it.  The slot, or -1 if a float is too close to tell
+// (or none is left).
+enum Keep { kAll, kDownTo, kTies };
+template <typename R, Keep KEEP, int G, int E, typename W>
 __device__ __forceinline__ int draw_kept(const W (&x)[E], const Setting& s, const Weight& weight, W threshold, int ties) {
   using S = Sums<R, E>;
   const int lane = threadIdx.x % G;
   int on_threshold = 0;
-  if (FILTER) {  // ties are kept in the order of their slots
+  if (KEEP == kTies) {  // ties are kept in the order of their slots
 #pragma unroll
     for (int j = 0; j < E; ++j) on_threshold += x[j] == threshold;
     on_threshold = lanes_scan<G>(on_threshold) - on_threshold;  // in the lanes before
@@ -332,33 +339,57 @@ __device__ __forceinline__ int draw_kept(const W (&x)[E], const Setting& s, cons
   const R min_p = (R)s.min_p;
   bool close = false;
   R w[E], here = 0, all;
+  if (S::kRough && __any(s.min_p > 0.0)) {
+    R nearest = INFINITY;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      w[j] = S::weight_of(weight, x[j]);
+      nearest = fmin(nearest, fabs(w[j] - min_p));
+      w[j] = w[j] >= min_p ? w[j] : (R)0;
+    }
+    close = s.min_p > 0.0 && !(nearest > (R)2e-5 * min_p);  // |t| is below 126
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      w[j] = S::weight_of(weight, x[j]);
+      if (!S::kRough) w[j] = w[j] >= min_p ? w[j] : (R)0;
+    }
+  }
 #pragma unroll
   for (int j = 0; j < E; ++j) {
-    w[j] = S::weight_of(weight, x[j]);
-    bool kept = w[j] >= min_p;
-    close |= s.min_p > 0.0 && S::close(w[j], min_p, (R)2e-5 * min_p);  // |t| is below 126
-    if (FILTER) {
+    if (KEEP == kDownTo) w[j] = x[j] >= threshold ? w[j] : (R)0;
+    if (KEEP == kTies) {
       const bool tie = x[j] == threshold;
-      kept = kept && (x[j] > threshold || (tie && on_threshold < ties));
+      w[j] = x[j] > threshold || (tie && on_threshold < ties) ? w[j] : (R)0;
       on_threshold += tie;
     }
-    if (!kept) w[j] = 0;
     here += w[j];
   }
   R upto = group_scan<G>(here, &all);
-  const R target = (R)(s.uniform * (double)all), within = S::kSlack * all;
-  close |= S::close(target, 0, within);
+  const R target = (R)(s.uniform * (double)all);
   int pick = INT32_MAX, last = -1;
+  if constexpr (S::kRough) {
+    // a lane that starts beyond the target is not the one; borders of lanes are borders too, and so is 0
+    int below = upto > target ? E : 0;
+    R nearest = fmin(target, fabs(upto - target));
 #pragma unroll
-  for (int j = 0; j < E; ++j) {
-    upto += w[j];
-    if (w[j] > 0) {
-      close |= S::close(upto, target, within);
-      last = lane * E + j;
-      if (upto > target && pick == INT32_MAX) pick = last;
+    for (int j = 0; j < E; ++j) {
+      upto += w[j];
+      below += upto <= target;
+      nearest = fmin(nearest, fabs(upto - target));
+    }
+    if (below < E) pick = lane * E + below;
+    if (close || !(nearest > S::kSlack * all)) pick = -1;
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      upto += w[j];
+      if (w[j] > 0) {
+        last = lane * E + j;
+        if (upto > target && pick == INT32_MAX) pick = last;
+      }
     }
   }
-  if (S::kRough && close) pick = -1;
   pick = lanes_all<G>(pick, [](int p, int q) { return p < q ? p : q; });
   if (S::kRough) return pick == INT32_MAX ? -1 : pick;
   last = lanes_all<G>(last, [](int p, int q) { return p > q ? p : q; });
@@ -377,6 +408,7 @@ __device__ int draw_in_group(const W (&x)[E], int count, const Setting& s, const
   const bool usable = weight.rough_is_usable();
   W threshold = -INFINITY;
   int ties = INT32_MAX;  // states on the threshold that are kept
+  bool all_ties = true;
   // rows of one wave differ in their settings: the wave sorts if any of them has to
   const bool filtered = s.has_top_k() || s.has_top_p();
   if (FILTER && __any(filtered)) {
@@ -402,18 +434,29 @@ __device__ int draw_in_group(const W (&x)[E], int count, const Setting& s, const
     }
     length = lanes_all<G>(length, add);
     last = lanes_all<G>(last, least);
-    int above = 0;
+    int above = 0, down_to = 0;
 #pragma unroll
-    for (int j = 0; j < E; ++j) above += c[j] > last;
+    for (int j = 0; j < E; ++j) {
+      above += c[j] > last;
+      down_to += c[j] >= last;
+    }
     above = lanes_all<G>(above, add);
+    down_to = lanes_all<G>(down_to, add);
     if (filtered) {
       threshold = last;
       ties = length - above;
+      all_ties = down_to == length;
     }
   }
-  const int pick = draw_kept<float, FILTER, G, E>(x, s, weight, threshold, ties);
+  int pick;
+  if (!FILTER)
+    pick = draw_kept<float, kAll, G, E>(x, s, weight, threshold, ties);
+  else if (__all(all_ties))
+    pick = draw_kept<float, kDownTo, G, E>(x, s, weight, threshold, ties);
+  else
+    pick = draw_kept<float, kTies, G, E>(x, s, weight, threshold, ties);
   if (!__any(pick < 0 || !usable)) return pick;
-  return draw_kept<double, FILTER, G, E>(x, s, weight, threshold, ties);
+  return draw_kept<double, FILTER ? kTies : kAll, G, E>(x, s, weight, threshold, ties);
 }
 
 // The lowest slot that holds `best`.
@@ -430,7 +473,7 @@ constexpr int kShortThreads = 256;
 
 // Rows of up to G * E states.
 template <typename T, bool FILTER, int G, int E>
-__global__ void __launch_bounds__(kShortThreads) draw_short(const Draws a, int64_t first_row) {
+__global__ void __launch_bounds__(kShortThreads, 2) draw_short(const Draws a, int64_t first_row) {
   using W = typename Value<T>::Wide;
   constexpr int V = Value<T>::kVec;
   constexpr int kRows = kShortThreads / G;

@@ -6,7 +6,7 @@
 // Bound by memory: every gradient is read for the norm and, since no element can be scaled before the
 // last one has been seen, read again for the copy.  A set lists its tensors once, cut into chunks of
 // at most 8 KiB that one wave streams with 16-byte loads; tensors of any number, size and type are
-// then two launches (785 tables of 20 elements: 2.6 + 3.1 us).  Neighbours in memory are joined before they
+// then two launches (785 tables of 20 elements: 2.7 + 3.4 us).  Neighbours in memory are joined before they
 // are cut, so a model whose tables are slices of one buffer is one tensor to the kernels; what precedes the
 // first cache line of an output is a chunk of its own, since 16-byte stores across lines cost twice.
 //

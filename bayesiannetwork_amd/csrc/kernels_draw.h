@@ -15,10 +15,12 @@
 // (draw_long, a block per row) works on those: without filters the prefix sums of 1/64 of the row lead to the 64
 // states that are looked at again; with filters the largest keys bound the threshold from below (the k largest
 // of them are k states of the row), and only the pieces that reach the bound are read again.  Rows that have
-// more than 512 states above the bound are left to a third launch (draw_wide).
+// more than 512 states above the bound are left to a third kernel (draw_wide); where such rows of a small batch
+// have top-p alone, its passes over the row are shared by 32 blocks first (draw_wide_masses, draw_wide_sums).
 //
 // Cumulative weights decide indices, so weights are doubles, summed in an order that depends on the call's
-// sizes alone.  Bins are filled by atomics, whose order varies: they add integers (the weight times a power
+// sizes alone; rows in registers take floats first, with a bound on what they are wrong by, and make the
+// comparisons again in doubles that are closer than that.  Bins are filled by atomics, whose order varies: they add integers (the weight times a power
 // of two), whose sum does not.
 #pragma once
 
@@ -139,35 +141,24 @@ struct Weight {
   double lowest;  // x - best from which on the weight is 0: t = -1023, whose exponent field is 0
   __device__ __forceinline__ Weight(double best_, double temperature)
       : best(best_), rate(1.4426950408889634074 / fmin(fmax(temperature, 1e-290), 1e290)), lowest(-1023.0 / rate) {}
-  // HELD: many weights of logits in registers at once, where left to itself the compiler copies every constant
-  // to where v_fmac adds to it, two moves per step (64-state rows with top-p: 34.2 -> 32.5 us without; a kernel
-  // that streams is 1 us in 22 slower for the scalar moves instead).
-  template <bool HELD = false>
-  __device__ __forceinline__ double at(double x) const {
+  __device__ __forceinline__ double operator()(double x) const {
     constexpr double kShift = 6755399441055744.0;
     const double d = fmax(x - best, lowest);
     const double shifted = fma(d, rate, kShift);
     const double f = fma(d, rate, kShift - shifted);
     double p = 1.0203121063391729e-07;
-    const auto step = [&](double c) {
-      if (HELD)
-        asm("v_fma_f64 %0, %1, %2, %3" : "=v"(p) : "v"(p), "v"(f), "s"(c));
-      else
-        p = fma(p, f, c);
-    };
-    step(1.3255224878668817e-06);
-    step(1.525268684626772e-05);
-    step(0.00015403455852453838);
-    step(0.0013333558179043112);
-    step(0.009618129159402558);
-    step(0.055504108664760424);
-    step(0.2402265069581299);
-    step(0.6931471805599453);
+    p = fma(p, f, 1.3255224878668817e-06);
+    p = fma(p, f, 1.525268684626772e-05);
+    p = fma(p, f, 0.00015403455852453838);
+    p = fma(p, f, 0.0013333558179043112);
+    p = fma(p, f, 0.009618129159402558);
+    p = fma(p, f, 0.055504108664760424);
+    p = fma(p, f, 0.2402265069581299);
+    p = fma(p, f, 0.6931471805599453);
     p = fma(p, f, 1.0);
     const uint32_t k = (uint32_t)(uint64_t)__double_as_longlong(shifted);
     return p * __hiloint2double((int)((k + 1023u) << 20), 0);
   }
-  __device__ __forceinline__ double operator()(double x) const { return at(x); }
   // In single precision.  Three roundings of t (the difference, the rate, their product) and the exponential's own:
   // wrong by less than (3 * ln 2 * |t| + 4) * 2^-24 of the weight, and 0 below 2^-126.  Rates beyond 1e30 either way
   // are left to doubles.
@@ -287,7 +278,7 @@ struct Sums {
     if constexpr (kRough)
       return weight.rough(x);
     else
-      return weight.template at<true>((double)x);
+      return weight((double)x);
   }
 };
 

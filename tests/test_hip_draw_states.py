@@ -329,3 +329,73 @@ def test_captured_and_on_another_stream(states):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, draw_states(x, u, **kwargs))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("states", [3, 5, 16, 64, 300, 1500, 5000, 40000])
+def test_borders_that_single_precision_does_not_resolve(states, dtype):
+    """Uniform numbers, shares and smallest weights 2e-9 to either side of a border of the row's own: closer than
+    sums of floats can tell (6e-8), twenty times farther than sums of doubles need."""
+    from bayesiannetwork_amd.samplers import draw_states
+
+    gen = torch.Generator().manual_seed(11 * states)
+    rows = 24
+    x = (2.0 * torch.randn((rows, states), generator=gen)).to(dtype)
+    side = torch.where(torch.arange(rows) % 2 == 0, 2e-9, -2e-9).double()
+    w = torch.softmax(x.double(), dim=1)
+    place = torch.randint(0, states - 1, (rows,), generator=gen)
+    u = (w.cumsum(1)[torch.arange(rows), place] + side).clamp(0.0, 1.0)
+    _check(draw_states(x.cuda(), u.cuda()), x.double().numpy(), u.numpy(), {})
+
+    place = torch.randint(0, min(states - 1, 40), (rows,), generator=gen)
+    p = torch.sort(w, dim=1, descending=True).values.cumsum(1)[torch.arange(rows), place] + side
+    u = torch.ones((rows,), dtype=torch.float64)  # the last kept state tells where the kept ones end
+    u[::3] = torch.rand((8,), generator=gen, dtype=torch.float64)
+    got = draw_states(x.cuda(), u.cuda(), top_p=p.cuda())
+    _check(got, x.double().numpy(), u.numpy(), dict(top_p=p.numpy()))
+
+    least = torch.sort(w / w.max(1, keepdim=True).values, dim=1, descending=True).values
+    m = least[torch.arange(rows), torch.clamp(place, max=3)].clamp(min=0.1) + side
+    got = draw_states(x.cuda(), u.cuda(), min_p=m.cuda())
+    _check(got, x.double().numpy(), u.numpy(), dict(min_p=m.numpy()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("states", [2100, 20000])
+def test_rows_of_a_few_states_in_a_long_tensor(states, dtype):
+    """Rows shorter than 16 bytes of logits, and some that end just behind a piece of 16 or 64 states."""
+    from bayesiannetwork_amd.samplers import draw_states
+
+    gen = torch.Generator().manual_seed(states)
+    counts = torch.tensor([1, 2, 3, 4, 5, 6, 7, 8, 9, 15, 16, 17, 63, 64, 65, 66, 1025, 2049])
+    rows = counts.numel()
+    x = torch.randn((rows, states), generator=gen).to(dtype)
+    u = torch.rand((rows,), generator=gen, dtype=torch.float64)
+    padded = x.clone()
+    for r in range(rows):
+        padded[r, int(counts[r]):] = float("nan")
+    for settings in (dict(), dict(top_k=2), dict(top_p=0.8), dict(top_k=3, top_p=0.9), dict(min_p=0.3), dict(temperature=0.0)):
+        got = draw_states(padded.cuda(), u.cuda(), num_states=counts.cuda(), **settings)
+        _check(got, [x[r, : int(counts[r])].double().numpy() for r in range(rows)], u.numpy(), settings)
+
+
+@pytest.mark.parametrize("tied", [900, 2500, 6000])
+def test_ties_around_the_threshold_side_by_side(tied):
+    """A share's threshold among states on one key that lie next to each other: the blocks that share a row find
+    nearly all of them in one block's part, or in two."""
+    from bayesiannetwork_amd.samplers import draw_states
+
+    gen = torch.Generator().manual_seed(tied)
+    rows, states = 5, 131072
+    x = torch.randn((rows, states), generator=gen)
+    x[:, 5000 : 5000 + tied] = 1.25
+    w = torch.softmax(x.double(), dim=1)
+    above, on = torch.where(x > 1.25, w, 0.0).sum(1), torch.where(x == 1.25, w, 0.0).sum(1)
+    p = above + on * torch.tensor([0.0004, 0.25, 0.5, 0.75, 0.9996], dtype=torch.float64)
+    u = torch.tensor([1.0, 0.3, 1.0, 0.8, 0.041], dtype=torch.float64)
+    got = draw_states(x.cuda(), u.cuda(), top_p=p.cuda()).cpu().tolist()
+    # a quarter of 900 ties is 225 of them: where a border lies on the share itself, the sums' roundings decide, and the
+    # states of both neighbours are right
+    for r in range(rows):
+        row = x[r].double().numpy()
+        assert got[r] in {_oracle(row, float(u[r]), top_p=float(p[r]) + d)[0] for d in (-1e-10, 0.0, 1e-10)}, r

@@ -1629,14 +1629,17 @@ void launch_summaries_and_draw(const Draws& a, hipStream_t s) {
 }
 
 template <typename T>
-void launch_long(const Draws& a, hipStream_t s) {
+void launch_long(Draws a, hipStream_t s) {
+  const bn_draw_filters& f = a.filters;
+  // a row may have top-p alone: without top-k, or with one that is no less than the row's states
+  const bool top_p = f.top_p_dev || f.top_p < 1.0;
+  if (!(top_p && (f.top_k_dev || f.top_k == 0 || f.top_k >= a.width || a.counts))) a.shared = nullptr;
   if (a.width <= kSmallPieceStates)
     launch_summaries_and_draw<T, 16>(a, s);
   else
     launch_summaries_and_draw<T, kBlock>(a, s);
-  const bn_draw_filters& f = a.filters;
-  if (!(f.top_k_dev || f.top_p_dev || f.min_p_dev || f.top_k > 0 || f.top_p < 1.0 || f.min_p > 0.0)) return;
-  if (a.shared && (f.top_p_dev || f.top_p < 1.0) && (f.top_k_dev || f.top_k == 0)) {
+  if (!(f.top_k_dev || top_p || f.min_p_dev || f.top_k > 0 || f.min_p > 0.0)) return;
+  if (a.shared) {
     const dim3 grid((uint32_t)(a.rows * kShares));
     hipLaunchKernelGGL(draw_wide_masses<T>, grid, dim3(kShareThreads), 0, s, a);
     hipLaunchKernelGGL(draw_wide_sums<T>, grid, dim3(kShareThreads), 0, s, a);

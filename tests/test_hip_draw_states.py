@@ -399,3 +399,21 @@ def test_ties_around_the_threshold_side_by_side(tied):
     for r in range(rows):
         row = x[r].double().numpy()
         assert got[r] in {_oracle(row, float(u[r]), top_p=float(p[r]) + d)[0] for d in (-1e-10, 0.0, 1e-10)}, r
+
+
+@pytest.mark.parametrize("states", [40, 3000, 16384, 60001])
+def test_top_k_of_all_of_a_row(states):
+    """A top-k that is no less than the row's states (all of them, or of those that a padded row has) leaves top-p
+    alone at work."""
+    from bayesiannetwork_amd.samplers import draw_states
+
+    gen = torch.Generator().manual_seed(3 * states)
+    rows = 6
+    x = torch.randn((rows, states), generator=gen)
+    u = torch.rand((rows,), generator=gen, dtype=torch.float64)
+    counts = torch.tensor([states, states // 2, states // 2 + 1, states - 1, 7 * states // 8, 3])
+    for top_k in (states // 2, states - 1, states, states + 1, 10**9):
+        settings = dict(top_k=top_k, top_p=0.9)
+        _check(draw_states(x.cuda(), u.cuda(), **settings), x.double().numpy(), u.numpy(), settings)
+        got = draw_states(x.cuda(), u.cuda(), num_states=counts.cuda(), **settings)
+        _check(got, [x[r, : int(counts[r])].double().numpy() for r in range(rows)], u.numpy(), settings)

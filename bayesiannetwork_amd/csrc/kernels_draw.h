@@ -838,7 +838,7 @@ struct LongShared {
       uint32_t count[kBins];
       int32_t index[kCandidates];
       int32_t listed[kListed];
-      uint8_t hits[kListed * kBlock * sizeof(Key) / 32];  // a pack of a listed piece holds four 4-byte keys or two of 8
+      uint8_t hits[kListed * kBlock * sizeof(Key) / 16];  // per pack of a listed piece, at least 16 / sizeof(Key) states
     };
   };
 };
@@ -973,6 +973,7 @@ __device__ __forceinline__ int draw_row(const Draws& a, int64_t r, LongShared<Ke
     // wave's own instructions and waits: logits are compared, not keys, up to four packs per lane are on their way at
     // once, and the second half works on the bits alone (row of 500 listed pieces: 15.7 -> 6.5 us).
     constexpr int kLanes = PIECE / V, kTogether = 64 / kLanes, kStride = THREADS / 64 * kTogether, kAhead = 4;
+    static_assert(sizeof(lds.hits) >= kListed * kLanes, "a byte per pack");
     const int part = lane % kLanes, slots = (int)listed * kLanes;
     const W lowest = (W)floor_value<W>(floor);
     const auto first_of = [&](int from) { return std::max(std::min(from, n - V), 0); };  // a row's last pack ends with it
@@ -1050,22 +1051,6 @@ __device__ __forceinline__ int draw_row(const Draws& a, int64_t r, LongShared<Ke
   }
   state = {best, (unsigned long long)floor, row_total, 1};
   return -2;
-}
-
-template <typename T, int PIECE>
-__global__ void __launch_bounds__(kLongThreads) draw_long(const Draws a, int64_t first_row) {
-  __shared__ LongShared<KeyType<T>> lds;
-  const int64_t r = first_row + blockIdx.x;
-  RowState state{};
-  const int drawn = draw_row<T, PIECE>(a, r, lds, state);
-  if (threadIdx.x == 0) {
-    if (drawn >= -1) a.out[r] = drawn;
-    a.row_states[r] = state;
-  }
-  if (drawn < -1 && a.shared) {
-    for (int b = threadIdx.x; b < kRoughBins; b += kLongThreads) a.shared[r].mass[b] = 0;
-    if (threadIdx.x == 0) a.shared[r].listed = 0;
-  }
 }
 
 // ---- long rows that keep many states ----------------------------------------------------------------
@@ -1498,6 +1483,39 @@ __device__ __forceinline__ int draw_wide_row(const WideRow<T>& row, double row_t
   return settling.drawn(kept);
 }
 
+// The second launch.  ALONE: it draws the rows with many states as well, a block's threads over all of the row.
+template <typename T, int PIECE, bool ALONE>
+__global__ void __launch_bounds__(kLongThreads) draw_long(const Draws a, int64_t first_row) {
+  using Key = KeyType<T>;
+  __shared__ union {
+    LongShared<Key> few;
+    struct {
+      Bins<kLongThreads> lds;
+      Listed<Key, 4 * kLongThreads> list;
+    } many;
+  } space;
+  const int64_t r = first_row + blockIdx.x;
+  RowState state{};
+  int drawn = draw_row<T, PIECE>(a, r, space.few, state);
+  if constexpr (ALONE) {
+    if (drawn < -1) {
+      __syncthreads();
+      const WideRow<T> row(a, r, state, Bins<kLongThreads>::kBins);
+      drawn = draw_wide_row<T>(row, state.total, space.many.lds, space.many.list);
+    }
+    if (threadIdx.x == 0) a.out[r] = drawn;
+    return;
+  }
+  if (threadIdx.x == 0) {
+    if (drawn >= -1) a.out[r] = drawn;
+    a.row_states[r] = state;
+  }
+  if (drawn < -1 && a.shared) {
+    for (int b = threadIdx.x; b < kRoughBins; b += kLongThreads) a.shared[r].mass[b] = 0;
+    if (threadIdx.x == 0) a.shared[r].listed = 0;
+  }
+}
+
 // A row whose passes were shared is left with short lists, over which fewer waves meet sooner: the others of its
 // block end (serving batch of 256 x 131072: 30 -> 14.5 us).
 template <typename T, int THREADS>
@@ -1617,15 +1635,19 @@ void launch_short_rows(const Draws& a, hipStream_t s) {
 }
 
 template <typename T, int PIECE>
-void launch_summaries_and_draw(const Draws& a, hipStream_t s) {
+void launch_summaries_and_draw(const Draws& a, bool alone, hipStream_t s) {
   constexpr int kPacks = 4;
   constexpr int64_t kTile = (int64_t)64 * Value<T>::kVec * kPacks * (kSummaryThreads / 64);
   const int64_t tiles = (a.width + kTile - 1) / kTile;
   hipLaunchKernelGGL((block_summaries<T, PIECE, kPacks>), dim3((uint32_t)std::min(a.rows * tiles, kMaxBlocks)),
                      dim3(kSummaryThreads), 0, s, a, tiles);
-  for (int64_t r = 0; r < a.rows; r += kMaxBlocks)
-    hipLaunchKernelGGL((draw_long<T, PIECE>), dim3((uint32_t)std::min(a.rows - r, kMaxBlocks)), dim3(kLongThreads), 0, s,
-                       a, r);
+  for (int64_t r = 0; r < a.rows; r += kMaxBlocks) {
+    const dim3 grid((uint32_t)std::min(a.rows - r, kMaxBlocks));
+    if (alone)
+      hipLaunchKernelGGL((draw_long<T, PIECE, true>), grid, dim3(kLongThreads), 0, s, a, r);
+    else
+      hipLaunchKernelGGL((draw_long<T, PIECE, false>), grid, dim3(kLongThreads), 0, s, a, r);
+  }
 }
 
 template <typename T>
@@ -1633,12 +1655,16 @@ void launch_long(Draws a, hipStream_t s) {
   const bn_draw_filters& f = a.filters;
   // a row may have top-p alone: without top-k, or with one that is no less than the row's states
   const bool top_p = f.top_p_dev || f.top_p < 1.0;
-  if (!(top_p && (f.top_k_dev || f.top_k == 0 || f.top_k >= a.width || a.counts))) a.shared = nullptr;
+  // A small top-k leaves few states in all but the rarest rows (ties at the k-th, or most of the k largest in a few
+  // pieces): no third launch for them then, though such a row takes longer (XX).  Without any filter no row is left.
+  const bool filtered = f.top_k_dev || top_p || f.min_p_dev || f.top_k > 0 || f.min_p > 0.0;
+  const bool alone = !f.top_k_dev && f.top_k > 0 && f.top_k <= kCandidates / 2;
+  if (alone || !(top_p && (f.top_k_dev || f.top_k == 0 || f.top_k >= a.width || a.counts))) a.shared = nullptr;
   if (a.width <= kSmallPieceStates)
-    launch_summaries_and_draw<T, 16>(a, s);
+    launch_summaries_and_draw<T, 16>(a, alone, s);
   else
-    launch_summaries_and_draw<T, kBlock>(a, s);
-  if (!(f.top_k_dev || top_p || f.min_p_dev || f.top_k > 0 || f.min_p > 0.0)) return;
+    launch_summaries_and_draw<T, kBlock>(a, alone, s);
+  if (alone || !filtered) return;
   if (a.shared) {
     const dim3 grid((uint32_t)(a.rows * kShares));
     hipLaunchKernelGGL(draw_wide_masses<T>, grid, dim3(kShareThreads), 0, s, a);

@@ -417,3 +417,27 @@ def test_top_k_of_all_of_a_row(states):
         _check(draw_states(x.cuda(), u.cuda(), **settings), x.double().numpy(), u.numpy(), settings)
         got = draw_states(x.cuda(), u.cuda(), num_states=counts.cuda(), **settings)
         _check(got, [x[r, : int(counts[r])].double().numpy() for r in range(rows)], u.numpy(), settings)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("states", [2049, 9000, 70001])
+def test_small_top_k_of_rows_with_many_states_around_it(states, dtype):
+    """Sorted rows (the largest states side by side, so that the pieces they are in say little), a few levels that
+    hundreds of states share, and flat rows, at the largest top-k of that kind and one beyond it."""
+    from bayesiannetwork_amd.samplers import draw_states
+
+    gen = torch.Generator().manual_seed(13 * states)
+    rows = 8
+    x = torch.randn((rows, states), generator=gen)
+    x[0:2] = torch.sort(x[0:2], dim=1, descending=True).values
+    x[2] = torch.sort(x[2]).values
+    x[3:5] = torch.round(x[3:5])
+    x[5] = 0.25
+    x[6, : states // 2] = -float("inf")
+    x = x.to(dtype)
+    u = torch.rand((rows,), generator=gen, dtype=torch.float64)
+    u[4:6] = torch.tensor([1.0, 1.0])
+    for settings in (dict(top_k=1), dict(top_k=50), dict(top_k=256), dict(top_k=257), dict(top_k=256, top_p=0.7),
+                     dict(top_k=200, min_p=0.4), dict(top_k=250, top_p=0.9, min_p=0.3, temperature=3.0)):
+        got = draw_states(x.cuda(), u.cuda(), **settings)
+        _check(got, x.double().numpy(), u.numpy(), settings, exact_sums=False)

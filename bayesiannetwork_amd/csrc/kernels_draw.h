@@ -15,7 +15,8 @@
 // (draw_long, a block per row) works on those: without filters the prefix sums of 1/64 of the row lead to the 64
 // states that are looked at again; with filters the largest keys bound the threshold from below (the k largest
 // of them are k states of the row), and only the pieces that reach the bound are read again.  Rows that have
-// more than 512 states above the bound are left to a third kernel (draw_wide); where such rows of a small batch
+// more than 512 states above the bound are left to a third kernel (draw_wide; with a small top-k the same
+// block goes on); where such rows of a small batch
 // have top-p alone, its passes over the row are shared by 32 blocks first (draw_wide_masses, draw_wide_sums).
 //
 // Cumulative weights decide indices, so weights are doubles, summed in an order that depends on the call's

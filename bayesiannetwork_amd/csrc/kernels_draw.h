@@ -1201,7 +1201,8 @@ __device__ __forceinline__ void add_rough_masses(const WideRow<T>& row, const Pr
 // what lies below is not.  Three roundings of the exponent t make a rough weight wrong by 3 * 2^-24 * ln 2 * |t|,
 // the exponential itself by 2^-22; a sum that starts with the largest weight, 1, has a mean |t| of 25 at most
 // (2^24 states of weight 2^-24 double it), so it is off by less than 4e-6 of itself, a fifth of kSlack, and by
-// the integers' rounding.
+// the integers' rounding.  Where all bins together stay below the target (min-p has raised the floor over states
+// that the share counts), there is no threshold: bins 0..-1, with every state above them.
 template <int THREADS>
 __device__ __forceinline__ int2 bins_around(const unsigned long long* mass, double target, int n, unsigned long long* words) {
   constexpr int kBins = 4 * THREADS;
@@ -1223,6 +1224,7 @@ __device__ __forceinline__ int2 bins_around(const unsigned long long* mass, doub
     if (last == ~0u && (double)upto * (1.0 - kSlack) - rounding >= goal) last = at;
   }
   const unsigned long long ends = block_all<THREADS>(((unsigned long long)first << 32) | last, words, kMinOfHalves);
+  if ((uint32_t)(ends >> 32) == ~0u) return make_int2(0, -1);
   const int lowest = std::min((uint32_t)ends, (uint32_t)kBins - 1);
   const int highest = std::min((int)std::min((uint32_t)(ends >> 32), (uint32_t)kBins - 1), lowest);
   return make_int2(kBins - 1 - lowest, kBins - 1 - highest);
@@ -1380,9 +1382,11 @@ __device__ __forceinline__ int draw_shared_row(const WideRow<T>& row, const Shar
   Prefix<Key> kept{row.floor, row.n};
   KeyRange<Key> range{row.floor, row.best, (unsigned long long)llrint(certain * settling.scale), 0ull, true};
   const double reach = row.s.top_p * row_total * settling.scale;
-  settling.narrow_listed(range, reach);
-  settling.end_on_key(kept, range, reach, true);
-  settling.add_listed(kept);
+  if (count != 0) {  // none: the share is not reached, all of the prefix is kept
+    settling.narrow_listed(range, reach);
+    settling.end_on_key(kept, range, reach, true);
+    settling.add_listed(kept);
+  }
   return settling.drawn(kept);
 }
 
@@ -1475,9 +1479,11 @@ __device__ __forceinline__ int draw_wide_row(const WideRow<T>& row, double row_t
       in_list = range.states <= ROOM;
       if (in_list) fill_list(kept, around.x, around.y, range.low, range.high);
     }
-    if (in_list) settling.narrow_listed(range, reach);
-    settling.end_on_key(kept, range, reach, in_list);
-    if (whole_list) settling.add_listed(kept);
+    if (list.count != 0) {  // none: the share is not reached, all of the prefix is kept
+      if (in_list) settling.narrow_listed(range, reach);
+      settling.end_on_key(kept, range, reach, in_list);
+      if (whole_list) settling.add_listed(kept);
+    }
     added = whole_list;
   }
   if (!added) (void)add_up<T, THREADS>(row, kept, lds.words);

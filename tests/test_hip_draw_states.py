@@ -441,3 +441,35 @@ def test_small_top_k_of_rows_with_many_states_around_it(states, dtype):
                      dict(top_k=200, min_p=0.4), dict(top_k=250, top_p=0.9, min_p=0.3, temperature=3.0)):
         got = draw_states(x.cuda(), u.cuda(), **settings)
         _check(got, x.double().numpy(), u.numpy(), settings, exact_sums=False)
+
+
+@pytest.mark.parametrize("dtype,states", [(torch.bfloat16, 131072), (torch.float32, 50000), (torch.float64, 12000)], ids=str)
+@pytest.mark.parametrize("rows", [12, 520])
+def test_a_share_that_min_p_does_not_leave(dtype, states, rows):
+    """More than 512 states are left by min-p, and together they hold less than top-p's share of the row: all of them
+    are kept, and finding that out takes no longer than finding a threshold (a search through keys that no state has
+    would take a hundred times as long)."""
+    from bayesiannetwork_amd.samplers import draw_states
+
+    gen = torch.Generator().manual_seed(states + rows)
+    x = (-torch.randint(0, 256, (rows, states), generator=gen) / 64.0).to(dtype)
+    u = torch.rand((rows,), generator=gen, dtype=torch.float64)
+    settings = dict(top_p=0.95, min_p=0.1)
+    dx, du = x.cuda(), u.cuda()
+    w = torch.exp(dx[:12].double() - dx[:12].double().max(1, keepdim=True).values)
+    assert ((w >= 0.1).sum(1) > 512).all() and (torch.where(w >= 0.1, w, 0.0).sum(1) < 0.95 * w.sum(1)).all()
+    got = draw_states(dx, du, **settings)
+    _check(got[:12], x[:12].double().numpy(), u.numpy(), settings)
+
+    def shortest(**kwargs):
+        times = []
+        for _ in range(6):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            draw_states(dx, du, **kwargs)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times)
+
+    assert shortest(**settings) < 10 * shortest(top_p=0.95)

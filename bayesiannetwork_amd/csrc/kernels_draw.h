@@ -21,8 +21,10 @@
 //
 // Cumulative weights decide indices, so weights are doubles, summed in an order that depends on the call's
 // sizes alone; rows in registers take floats first, with a bound on what they are wrong by, and make the
-// comparisons again in doubles that are closer than that.  Bins are filled by atomics, whose order varies: they add integers (the weight times a power
-// of two), whose sum does not.
+// comparisons again in doubles that are closer than that.  Bins are filled by atomics, whose order varies: they add
+// integers (the weight times a power of two), whose sum does not.  Where these decide a border they are of 2^-49 of
+// the largest weight for at most 4096 states, and a pair of them (ByMassAndRest) for a whole row: a border is
+// off by less than 1e-11 of the row's weight.
 #pragma once
 
 #include <algorithm>
@@ -668,50 +670,87 @@ __device__ __forceinline__ unsigned long long mass_of(double w, double scale) {
   return (unsigned long long)__double_as_longlong(shifted) & 0xFFFFFFFFFFFFFull;
 }
 
+// What find_bin adds up by bin: states,
+struct ByCount {
+  const uint32_t* count;
+  __device__ __forceinline__ void clear(int) const {}
+  template <typename Key>
+  __device__ __forceinline__ void add(int, Key) const {}
+  __device__ __forceinline__ double of(int bin) const { return (double)count[bin]; }
+};
+// their weights as integers,
+struct ByMass {
+  const Weight& weight;
+  unsigned long long* mass;
+  double scale, unit = 1.0 / scale;  // powers of two
+  __device__ __forceinline__ void clear(int bin) const { mass[bin] = 0; }
+  template <typename Key>
+  __device__ __forceinline__ void add(int bin, Key k) const {
+    atomicAdd(&mass[bin], mass_of(weight.of_key(k), scale));
+  }
+  __device__ __forceinline__ double of(int bin) const { return (double)mass[bin] * unit; }
+};
+// or as integers and what these leave of each weight, as integers again.  One integer per weight has room for
+// 2^-37 of the largest at 2^24 states: a tail of weights below half of that counts as nothing, however much it
+// holds together.  Two have room for 2^-74.
+struct ByMassAndRest {
+  const Weight& weight;
+  unsigned long long* mass;
+  unsigned long long* rest;
+  double scale, unit = 1.0 / scale;
+  __device__ __forceinline__ void clear(int bin) const { mass[bin] = rest[bin] = 0; }
+  template <typename Key>
+  __device__ __forceinline__ void add(int bin, Key k) const {
+    const double scaled = weight.of_key(k) * scale, whole = floor(scaled);
+    atomicAdd(&mass[bin], mass_of(whole, 1.0));
+    atomicAdd(&rest[bin], mass_of(scaled - whole, scale));
+  }
+  __device__ __forceinline__ double of(int bin) const { return ((double)mass[bin] + (double)rest[bin] * unit) * unit; }
+};
+
 // A bin, and what lies above it.
 struct Found {
   int bin;
-  unsigned long long above;   // count or mass of the bins above
+  double above;               // count or weight of the bins above
   unsigned long long states;  // in the bin
   bool reached;               // the target is reached in it; else it is the lowest that holds a state
 };
 
-// The bin in which the count (BY_MASS: the mass) from the top, `above` included, reaches `target`.  each(fn)
+// The bin in which what `by` adds up from the top, `above` included, reaches `target`.  each(fn)
 // calls fn(key) for every key there is; bin_of(key) is its bin, ascending with the key, or negative.
-template <bool BY_MASS, typename Lds, typename Each, typename BinOf, typename Mass>
-__device__ __forceinline__ Found find_bin(Lds& lds, Each each, BinOf bin_of, Mass mass, unsigned long long above, double target) {
+template <typename Lds, typename Each, typename BinOf, typename By>
+__device__ __forceinline__ Found find_bin(Lds& lds, Each each, BinOf bin_of, By by, double above, double target) {
   constexpr int THREADS = Lds::kThreads, kBins = Lds::kBins;
   __syncthreads();
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
     lds.count[b * THREADS + threadIdx.x] = 0;
-    if (BY_MASS) lds.mass[b * THREADS + threadIdx.x] = 0;
+    by.clear(b * THREADS + (int)threadIdx.x);
   }
   __syncthreads();
   each([&](auto k) {
     const int bin = bin_of(k);
     if (bin < 0) return;
     atomicAdd(&lds.count[bin], 1u);
-    if (BY_MASS) atomicAdd(&lds.mass[bin], mass(k));
+    by.add(bin, k);
   });
   __syncthreads();
   // thread t holds bins kBins - 1 - 4 t downwards
-  unsigned long long own[4], sum = 0, total;
+  double own[4], sum = 0.0, total;
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
-    const int bin = kBins - 1 - 4 * (int)threadIdx.x - b;
-    own[b] = BY_MASS ? lds.mass[bin] : (unsigned long long)lds.count[bin];
+    own[b] = by.of(kBins - 1 - 4 * (int)threadIdx.x - b);
     sum += own[b];
   }
-  unsigned long long before = above + block_scan<THREADS>(sum, lds.words, &total);
+  double before = above + block_scan<THREADS>(sum, lds.words, &total);
   // the first bin that reaches the target and, counted from the other end, the last one that holds a state
   uint32_t found = ~0u, lowest = ~0u;
-  unsigned long long found_above = 0, lowest_above = 0;
+  double found_above = 0.0, lowest_above = 0.0;
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
     const uint32_t at = 4 * threadIdx.x + b;
     if (lds.count[kBins - 1 - at] != 0) {
-      if (found == ~0u && (double)(before + own[b]) >= target) {
+      if (found == ~0u && before + own[b] >= target) {
         found = at;
         found_above = before;
       }
@@ -723,29 +762,30 @@ __device__ __forceinline__ Found find_bin(Lds& lds, Each each, BinOf bin_of, Mas
   const unsigned long long both = block_all<THREADS>(((unsigned long long)found << 32) | lowest, lds.words, kMinOfHalves);
   const bool reached = (uint32_t)(both >> 32) != ~0u;
   const int at = reached ? (int)(both >> 32) : kBins - 1 - (int)std::min((uint32_t)both, (uint32_t)kBins - 1);
-  if (threadIdx.x == (unsigned)(at / 4)) lds.answer[0] = (long long)(reached ? found_above : lowest_above);
+  if (threadIdx.x == (unsigned)(at / 4)) lds.answer[0] = __double_as_longlong(reached ? found_above : lowest_above);
   __syncthreads();
-  return {kBins - 1 - at, (unsigned long long)lds.answer[0], lds.count[kBins - 1 - at], reached};
+  return {kBins - 1 - at, __longlong_as_double(lds.answer[0]), lds.count[kBins - 1 - at], reached};
 }
 
 // A range of keys, what lies above it and how many states it holds.
 template <typename Key>
 struct KeyRange {
   Key low, high;
-  unsigned long long above, states;
+  double above;
+  unsigned long long states;
   bool reached;
 };
 
 // find_bin with as many bins of equal width as there are for the keys of a range; narrows it to the one found.
-template <bool BY_MASS, typename Lds, typename Key, typename Each, typename Mass>
-__device__ __forceinline__ void narrow(Lds& lds, KeyRange<Key>& range, Each each, Mass mass, double target) {
+template <typename Lds, typename Key, typename Each, typename By>
+__device__ __forceinline__ void narrow(Lds& lds, KeyRange<Key>& range, Each each, By by, double target) {
   constexpr int kLog = Lds::kThreads == 1024 ? 12 : 10;
   static_assert((1 << kLog) == Lds::kBins, "four bins per thread");
   const Key low = range.low, high = range.high, span = high - low;
   const int bits = sizeof(Key) == 8 ? 64 - __clzll((long long)span) : 32 - __clz((int)(uint32_t)span);
   const int shift = bits > kLog ? bits - kLog : 0;
-  const Found f = find_bin<BY_MASS>(
-      lds, each, [&](Key k) { return k < low || k > high ? -1 : (int)((k - low) >> shift); }, mass, range.above, target);
+  const Found f = find_bin(
+      lds, each, [&](Key k) { return k < low || k > high ? -1 : (int)((k - low) >> shift); }, by, range.above, target);
   range.low = low + ((Key)f.bin << shift);
   const Key top = range.low + (((Key)1 << shift) - 1);
   range.high = top > high || top < range.low ? high : top;
@@ -929,8 +969,6 @@ __device__ __forceinline__ int draw_row(const Draws& a, int64_t r, LongShared<Ke
 
   // ---- a floor below which nothing is kept
   least = block_all<THREADS>(least, lds.words, kMin);
-  const double scale = mass_scale(n);
-  const auto mass = [&](Key k) { return mass_of(weight.of_key(k), scale); };
   const auto each_piece = [&](auto fn) {
     for (int b = threadIdx.x; b < pieces; b += THREADS) fn(key_of(b));
   };
@@ -944,16 +982,19 @@ __device__ __forceinline__ int draw_row(const Draws& a, int64_t r, LongShared<Ke
   if (s.has_top_k()) {
     // the largest keys of k pieces are k states: the k-th state's key is not below the k-th of them
     if (s.top_k < pieces) {
-      KeyRange<Key> range{(Key)least, (Key)best, 0ull, 0ull, true};
-      narrow<false>(lds, range, each_piece, mass, (double)s.top_k);
+      KeyRange<Key> range{(Key)least, (Key)best, 0.0, 0ull, true};
+      narrow(lds, range, each_piece, ByCount{lds.count}, (double)s.top_k);
       floor = range.low;
     }
   } else if (s.has_top_p()) {
     // the states below (1 - p) W / n hold less than the share that is left out
     raise_floor((1.0 - s.top_p) * row_total / (double)n);
     // and where pieces' largest states hold the share by themselves, nothing below those is kept
-    KeyRange<Key> range{std::max(floor, (Key)least), (Key)best, 0ull, 0ull, true};
-    narrow<true>(lds, range, each_piece, mass, s.top_p * row_total * scale * (1.0 + 1e-9));
+    // (with room for the sums' roundings and for the integers', half a unit per piece)
+    KeyRange<Key> range{std::max(floor, (Key)least), (Key)best, 0.0, 0ull, true};
+    const double scale = mass_scale(n);
+    narrow(lds, range, each_piece, ByMass{weight, lds.mass, scale},
+           s.top_p * row_total * (1.0 + 1e-9) + (double)pieces / scale);
     if (range.reached) floor = std::max(floor, range.low);
   }
   // (with top-k and top-p together W is the weight of all top-k states, those that min-p drops among them)
@@ -1091,8 +1132,13 @@ struct Steps {
 template <typename Key, int ROOM>
 struct Listed {
   static constexpr int kRoom = ROOM;
-  Key key[kRoom];
-  int32_t index[kRoom];
+  union {
+    struct {
+      Key key[kRoom];
+      int32_t index[kRoom];
+    };
+    unsigned long long rest[kRoom];  // of the bins' masses, where there is no list
+  };
   uint32_t count;  // those that found no room counted too
   __device__ __forceinline__ void add(int i, Key k) {
     const uint32_t at = atomicAdd(&count, 1u);
@@ -1121,9 +1167,9 @@ __device__ __forceinline__ int last_kept(const T* x, int n, KeyType<T> key, unsi
       for (uint32_t q = threadIdx.x; q < count; q += THREADS)
         if (list.key[q] == key) fn(~(uint32_t)list.index[q]);
     };
-    KeyRange<uint32_t> range{~(uint32_t)n, ~0u, 0ull, 0ull, true};
+    KeyRange<uint32_t> range{~(uint32_t)n, ~0u, 0.0, 0ull, true};
     do {
-      narrow<false>(lds, range, each, [](uint32_t) { return 0ull; }, (double)kept);
+      narrow(lds, range, each, ByCount{lds.count}, (double)kept);
     } while (range.low != range.high && range.states > 1);
     each([&](uint32_t i) {
       if (i >= range.low && i <= range.high) lds.answer[1] = (long long)~i;
@@ -1297,18 +1343,16 @@ struct Settling {
   const WideRow<T>& row;
   Bins<THREADS>& lds;
   Listed<Key, ROOM>& list;
-  double scale;  // of masses
   __device__ __forceinline__ Settling(const WideRow<T>& row_, Bins<THREADS>& lds_, Listed<Key, ROOM>& list_)
-      : row(row_), lds(lds_), list(list_), scale(mass_scale(row_.n)) {}
+      : row(row_), lds(lds_), list(list_) {}
 
-  __device__ __forceinline__ Sum mass(Key k) const { return mass_of(row.weight.of_key(k), scale); }
   template <typename Fn>
   __device__ __forceinline__ void each_listed(Fn fn) const {
     const uint32_t count = list.count;
     for (uint32_t q = threadIdx.x; q < count; q += THREADS) fn(list.key[q]);
   }
 
-  // The key at which the mass reaches `reach`, among the listed ones.
+  // The key at which the weight reaches `reach`, among the listed ones.
   __device__ __forceinline__ void narrow_listed(KeyRange<Key>& range, double reach) {
     // the list's own range, which is a bin or two, instead of all keys
     Sum low = ~0ull, high = 0;
@@ -1318,18 +1362,17 @@ struct Settling {
     });
     range.low = (Key)block_all<THREADS>(low, lds.words, kMin);
     range.high = (Key)block_all<THREADS>(high, lds.words, kMax);
+    const ByMass by{row.weight, lds.mass, mass_scale(ROOM)};
     do {
-      narrow<true>(lds, range, [&](auto fn) { each_listed(fn); }, [&](Key k) { return mass(k); }, reach);
+      narrow(lds, range, [&](auto fn) { each_listed(fn); }, by, reach);
     } while (range.low != range.high);
   }
 
   // Ends `kept` in the states on the range's key: those with less than the target before them, one at least.
   __device__ __forceinline__ void end_on_key(Prefix<Key>& kept, const KeyRange<Key>& range, double reach, bool in_list) {
-    const double each = (double)mass(range.low), above = (double)range.above;
+    const double each = row.weight.of_key(range.low);
     Sum ties = range.states;
-    if (each > 0.0) ties = (Sum)fmin(fmax(ceil((reach - above) / each), 1.0), (double)range.states);
-    while (ties > 1 && above + (double)(ties - 1) * each >= reach) --ties;
-    while (ties < range.states && above + (double)ties * each < reach) ++ties;
+    if (each > 0.0) ties = (Sum)fmin(fmax(ceil((reach - range.above) / each), 1.0), (double)range.states);
     const int bound = range.low == kept.key ? kept.last : row.n;
     kept.key = range.low;
     kept.last = ties < range.states ? last_kept<T>(row.x, row.n, range.low, ties, lds, list, in_list) : bound;
@@ -1380,8 +1423,8 @@ __device__ __forceinline__ int draw_shared_row(const WideRow<T>& row, const Shar
   if (threadIdx.x == 0) list.count = count;
   __syncthreads();
   Prefix<Key> kept{row.floor, row.n};
-  KeyRange<Key> range{row.floor, row.best, (unsigned long long)llrint(certain * settling.scale), 0ull, true};
-  const double reach = row.s.top_p * row_total * settling.scale;
+  KeyRange<Key> range{row.floor, row.best, certain, 0ull, true};
+  const double reach = row.s.top_p * row_total;
   if (count != 0) {  // none: the share is not reached, all of the prefix is kept
     settling.narrow_listed(range, reach);
     settling.end_on_key(kept, range, reach, true);
@@ -1401,8 +1444,7 @@ __device__ __forceinline__ int draw_wide_row(const WideRow<T>& row, double row_t
   const int n = row.n;
   const T* x = row.x;
   Settling<T, THREADS, ROOM> settling(row, lds, list);
-  const auto mass = [&](Key k) { return settling.mass(k); };
-  const auto no_mass = [](auto) { return 0ull; };
+  const ByCount by_count{lds.count};
 
   // the states of a prefix in bins lowest..highest, by key
   const auto each_in = [&](const Prefix<Key>& in, int lowest, int highest, auto fn) {
@@ -1436,45 +1478,46 @@ __device__ __forceinline__ int draw_wide_row(const WideRow<T>& row, double row_t
         if (KeyOf<W>::key(v) >= all.key) fn(v);
       });
     };
-    const Found f = find_bin<false>(lds, each_state, [&](W v) { return row.steps.bin(v); }, no_mass, 0ull, (double)s.top_k);
+    const Found f = find_bin(lds, each_state, [&](W v) { return row.steps.bin(v); }, by_count, 0.0, (double)s.top_k);
     KeyRange<Key> range{row.floor, row.best, f.above, f.states, true};
     const auto each_key = [&](auto fn) {
       each_in(all, f.bin, f.bin, [&](int, Key k) { fn(k); });
     };
-    while (range.low != range.high && range.states > ROOM) narrow<false>(lds, range, each_key, no_mass, (double)s.top_k);
+    while (range.low != range.high && range.states > ROOM) narrow(lds, range, each_key, by_count, (double)s.top_k);
     const bool in_list = range.states <= ROOM;
     if (in_list) {
       fill_list(all, f.bin, f.bin, range.low, range.high);
-      while (range.low != range.high) narrow<false>(lds, range, each_listed, no_mass, (double)s.top_k);
+      while (range.low != range.high) narrow(lds, range, each_listed, by_count, (double)s.top_k);
     }
     kept.key = range.low;
-    const Sum ties = (Sum)s.top_k - range.above;
+    const Sum ties = (Sum)s.top_k - (Sum)range.above;
     if (ties < range.states) kept.last = last_kept<T>(x, n, range.low, ties, lds, list, in_list);
   }
 
   bool added = false;
   if (s.has_top_p()) {
-    const double target = s.top_p * (s.has_top_k() ? add_up<T, THREADS>(row, kept, lds.words) : row_total);
-    const double reach = target * settling.scale;
+    const double reach = s.top_p * (s.has_top_k() ? add_up<T, THREADS>(row, kept, lds.words) : row_total);
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < 4; ++b) lds.mass[b * THREADS + threadIdx.x] = 0;
     __syncthreads();
     add_rough_masses<T, THREADS>(row, kept, 0, n, lds.mass);
     __syncthreads();
-    const int2 around = bins_around<THREADS>(lds.mass, target, n, lds.words);
+    const int2 around = bins_around<THREADS>(lds.mass, reach, n, lds.words);
     clear_list();
     const double certain = add_up<T, THREADS>(row, kept, around.x, around.y, 0, row.segments, lds.words,
                                               [&](int i, Key k) { list.add(i, k); });
-    KeyRange<Key> range{kept.key, row.best, (Sum)llrint(certain * settling.scale), 0ull, true};
+    KeyRange<Key> range{kept.key, row.best, certain, 0ull, true};
     const bool whole_list = list.count <= ROOM;  // the list holds all those around the threshold
     bool in_list = whole_list;                   // ... those on its key
     if (!in_list) {
       const auto each_key = [&](auto fn) {
         each_in(kept, around.x, around.y, [&](int, Key k) { fn(k); });
       };
+      static_assert(ROOM >= Bins<THREADS>::kBins, "the list's memory holds the rests");
+      const ByMassAndRest by{row.weight, lds.mass, list.rest, mass_scale(n)};
       do {
-        narrow<true>(lds, range, each_key, mass, reach);
+        narrow(lds, range, each_key, by, reach);
       } while (range.low != range.high && range.states > ROOM);
       in_list = range.states <= ROOM;
       if (in_list) fill_list(kept, around.x, around.y, range.low, range.high);

@@ -473,3 +473,36 @@ def test_a_share_that_min_p_does_not_leave(dtype, states, rows):
         return min(times)
 
     assert shortest(**settings) < 10 * shortest(top_p=0.95)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64], ids=str)
+@pytest.mark.parametrize("states,tail", [(1 << 24, [-26.625]), (1 << 20, [-30.0]), ((1 << 20) + 3, [-28.5, -28.75, -29.0]),
+                                         (70001, [-22.0, -22.5]), (16000, [-18.0])], ids=str)
+def test_a_tail_that_only_counts_together(states, tail, dtype):
+    """One state of weight 1, and a tail in which every state is next to nothing but top-p's threshold lies: 0.5 states
+    behind the k-th of a key that hundreds of thousands share.  Weights, sums and the expected state in closed form
+    (a running sum of the tail would round more of it away): a border is off by about 2^-53 of the row where the
+    weights are, against half a state, 2^-45 of it at the least."""
+    from bayesiannetwork_amd.samplers import draw_states
+
+    keys = torch.tensor(tail, dtype=dtype)
+    levels = np.arange(states) % len(tail)
+    levels[0] = -1
+    x = keys[torch.from_numpy(levels).clamp(min=0)]
+    x[0] = 0.0
+    w = np.exp(keys.double().numpy())
+    sizes = np.array([(levels == k).sum() for k in range(len(tail))])
+    total = 1.0 + float((sizes * w).sum())
+    end = len(tail) // 2  # the key on which the share ends
+    kept = int(sizes[end] * 0.37)
+    p = (1.0 + float((sizes[:end] * w[:end]).sum()) + (kept + 0.5) * w[end]) / total
+    assert 0.5 * w[end] > 100 * 2.0**-53 and p < 1.0
+    numbers = [np.cumsum(levels == k) for k in range(len(tail))]  # states of each key up to an index
+    upto = 1.0 + sum(numbers[k] * w[k] for k in range(end)) + np.minimum(numbers[end], kept + 1) * w[end]
+    drawn = np.flatnonzero(np.diff(upto, prepend=0.0) > 0)
+    picks = drawn[[1, len(drawn) // 7, len(drawn) // 2, len(drawn) - 2, len(drawn) - 1]]
+    before = np.concatenate([[0.0], upto])[picks]
+    u = np.append((before + upto[picks]) / 2 / upto[-1], 1.0)
+    want = np.append(picks, drawn[-1])
+    got = draw_states(x.cuda()[None].expand(len(u), states), torch.from_numpy(u).cuda(), top_p=float(p))
+    assert got.cpu().tolist() == want.tolist()

@@ -1231,15 +1231,18 @@ struct WideRow {
 };
 constexpr double kListScale = 1125899906842624.0;  // 2^50: at most 4096 weights add up
 
-// Masses by logit of a prefix's states in [begin, end), from weights of single precision.
+// Masses by logit of a prefix's states in [begin, end), from weights of single precision (of double where the
+// temperature leaves that no room).
 constexpr double kRoughScale = 274877906944.0;  // 2^38: 2^24 weights add up within 62 bits
 template <typename T, int THREADS>
 __device__ __forceinline__ void add_rough_masses(const WideRow<T>& row, const Prefix<KeyType<T>>& in, int begin, int end,
                                  unsigned long long* mass) {
   using W = typename Value<T>::Wide;
+  const bool usable = row.weight.rough_is_usable();
   for_each_state<T, THREADS>(row.x, begin, end, [&](int i, W v) {
     if (!in.has(i, KeyOf<W>::key(v))) return;
-    atomicAdd(&mass[row.steps.bin(v)], mass_of((double)row.weight.rough(v), kRoughScale));
+    const double w = usable ? (double)row.weight.rough(v) : row.weight((double)v);
+    atomicAdd(&mass[row.steps.bin(v)], mass_of(w, kRoughScale));
   });
 }
 

@@ -478,12 +478,17 @@ __global__ void __launch_bounds__(kShortThreads, 2) draw_short(const Draws a, in
   const Setting s = row_setting(a, r);
   const int n = (int)s.n, first = lane * E;
   W x[E];
-  if (E >= V && first + E <= a.width) {  // a shorter row has room behind it
+  if (E >= V && n >= V) {  // (nothing behind the row's n states is read)
+    Raw raw[E / V > 0 ? E / V : 1];
 #pragma unroll
-    for (int k = 0; k + V <= E; k += V) {
-      const Pack<T> p = load_pack(row + first + k);
+    for (int k = 0; k < E / V; ++k) raw[k] = raw_of(load_pack(row + pack_start(first + k * V, n, V)));
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[k + j] = first + k + j < n ? Value<T>::widen(p.v[j]) : (W)-INFINITY;
+    for (int k = 0; k < E / V; ++k) {
+      const int from = first + k * V, by = from - pack_start(from, n, V);
+      if (__any(by > 0 && by < V)) raw[k] = moved_down<sizeof(T)>(raw[k], by);
+      const Pack<T> p = pack_of<T>(raw[k]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[k * V + j] = from + j < n ? Value<T>::widen(p.v[j]) : (W)-INFINITY;
     }
   } else {
 #pragma unroll
@@ -1018,7 +1023,7 @@ __device__ __forceinline__ int draw_row(const Draws& a, int64_t r, LongShared<Ke
     static_assert(sizeof(lds.hits) >= kListed * kLanes, "a byte per pack");
     const int part = lane % kLanes, slots = (int)listed * kLanes;
     const W lowest = (W)floor_value<W>(floor);
-    const auto first_of = [&](int from) { return std::max(std::min(from, n - V), 0); };  // a row's last pack ends with it
+    const auto first_of = [&](int from) { return n < V ? 0 : pack_start(from, n, V); };
     for (int base = wave * kTogether; base < (int)listed; base += kAhead * kStride) {
       Raw raw[kAhead];
       int from[kAhead];
@@ -1026,7 +1031,14 @@ __device__ __forceinline__ int draw_row(const Draws& a, int64_t r, LongShared<Ke
       for (int u = 0; u < kAhead; ++u) {
         const int q = std::min(base + u * kStride + lane / kLanes, (int)listed - 1);
         from[u] = lds.listed[q] * PIECE + part * V;
-        raw[u] = raw_of(load_pack(x + first_of(from[u])));
+        if (n >= V) {
+          raw[u] = raw_of(load_pack(x + first_of(from[u])));
+        } else {
+          Pack<T> p;
+#pragma unroll
+          for (int j = 0; j < V; ++j) p.v[j] = j < n ? x[j] : Value<T>::round(-INFINITY);
+          raw[u] = raw_of(p);
+        }
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "../../include/bn_hip.h"
+#include "row_loads.h"
 
 #include <cstdint>
 
@@ -75,11 +76,8 @@ __device__ __forceinline__ void store_pack_streamed(T* p, const Pack<T>& v) {
   __builtin_nontemporal_store(__builtin_bit_cast(Words, v), reinterpret_cast<Words*>(p));
 }
 
-// The 16 bytes as four registers.  kept() hides where they came from, so that what was unpacked from them
+// A pack and its registers.  kept() hides where they came from, so that what was unpacked from them
 // before (twice the registers for 16-bit types) is not kept alive for later use instead.
-struct Raw {
-  uint32_t w[4];
-};
 template <typename T>
 __device__ __forceinline__ Raw raw_of(const Pack<T>& p) {
   return __builtin_bit_cast(Raw, p);

@@ -529,3 +529,33 @@ def test_temperatures_beyond_single_precision(states, temperature):
         # the row of one level has exact sums
         got = draw_states(x.cuda(), u.cuda(), **settings)
         _check(got, x.numpy(), u.numpy(), settings, exact_sums=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("states", [16, 37, 64, 250, 1000, 2048, 2500, 20000])
+def test_a_last_row_that_ends_its_buffer(states, dtype):
+    """Through the C ABI: the buffer ends with the last row's own states, whose padding does not exist; and rows whose
+    lengths run through all places of a pack."""
+    import ctypes
+
+    from bayesiannetwork_amd.inference_machines.hip_spa import _native
+
+    gen = torch.Generator().manual_seed(states)
+    lib = _native.load()
+    for last in (1, 3, 7, 9, 16, states - 1):
+        counts = torch.tensor([min(n, states) for n in (1, 2, 5, 8, 11, 14, 17, 20, 23, 30, 65, 66, states)] + [last])
+        rows = counts.numel()
+        x = torch.randn((rows, states), generator=gen).to(dtype)
+        u = torch.rand((rows,), generator=gen, dtype=torch.float64)
+        flat = x.flatten()[: (rows - 1) * states + last].cuda()
+        dc, du = counts.cuda(), u.cuda()
+        need = lib.bn_draw_states_workspace_bytes(_native.DTYPE_CODES[dtype], rows, states)
+        workspace = torch.empty((max(need, 1),), dtype=torch.uint8, device="cuda")
+        for settings in (dict(), dict(top_p=0.8), dict(top_k=3, temperature=2.0), dict(temperature=0.0)):
+            filters = _native.DrawFilters(1.0, 0, 1.0, 0.0)
+            for k, v in settings.items():
+                setattr(filters, k, v)
+            out = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
+            _native.launch(flat.device, lib.bn_draw_states, _native.DTYPE_CODES[dtype], flat.data_ptr(), rows, states, states,
+                           dc.data_ptr(), 1, du.data_ptr(), ctypes.byref(filters), workspace.data_ptr(), out.data_ptr())
+            _check(out, [x[r, : int(counts[r])].double().numpy() for r in range(rows)], u.numpy(), settings)

@@ -2,6 +2,9 @@
 of them is decided on the host, before anything reaches a GPU."""
 
 import ctypes
+import os
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -143,3 +146,12 @@ def test_gradient_set_calls_check_their_arguments():
     assert lib.bn_gradient_set_norm(None, B, B, None) == -1
     assert lib.bn_gradient_set_clip(None, 1.0, B, B, None) == -1
     assert lib.bn_gradient_set_destroy(None) == 0
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="no host compiler")
+def test_loads_stay_inside_their_rows(tmp_path):
+    """The arithmetic of draw_states' loads, on the host: a padded row may be the last thing in its buffer."""
+    source = os.path.join(os.path.dirname(os.path.abspath(__file__)), "row_loads_check.cpp")
+    program = str(tmp_path / "row_loads_check")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-o", program, source], check=True)
+    subprocess.run([program], check=True)

@@ -708,7 +708,7 @@ struct ByMassAndRest {
   __device__ __forceinline__ void add(int bin, Key k) const {
     const double scaled = weight.of_key(k) * scale, whole = floor(scaled);
     atomicAdd(&mass[bin], mass_of(whole, 1.0));
-    atomicAdd(&rest[bin], mass_of(scaled - whole, scale));
+    if (scaled != whole) atomicAdd(&rest[bin], mass_of(scaled - whole, scale));
   }
   __device__ __forceinline__ double of(int bin) const { return ((double)mass[bin] + (double)rest[bin] * unit) * unit; }
 };

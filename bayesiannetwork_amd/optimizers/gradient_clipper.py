@@ -56,6 +56,9 @@ class HipGradientClipper:
             for i, (g, o) in enumerate(zip(gradients, outputs)):
                 if g.shape != o.shape or g.dtype != o.dtype or g.device != o.device:
                     raise ValueError(f"out[{i}] must have the shape, type and device of gradients[{i}]")
+        # one tensor for each version counter among the outputs: views share their base's
+        written = (o if o._base is None else o._base for o in outputs)
+        self._written = list({id(t): t for t in written}.values())
         self._device = gradients[0].device
         self._gradients, self._outputs = gradients, outputs  # the set holds their addresses
         self._lib = _native.load()
@@ -91,8 +94,11 @@ class HipGradientClipper:
 
     def clip(self, max_norm: float) -> torch.Tensor:
         """Writes the gradients, scaled by ``max_norm / norm`` where the norm exceeds ``max_norm``, to
-        their outputs; returns the norm before scaling (float64 scalar on the device)."""
+        their outputs; returns the norm before scaling (float64 scalar on the device).  As after any
+        operation in place, a backward pass that needs what the outputs held before raises."""
         max_norm = float(max_norm)
         if not 0.0 < max_norm < float("inf"):
             raise ValueError(f"max_norm must be positive and finite, not {max_norm}")
-        return self._call(self._lib.bn_gradient_set_clip, max_norm)
+        norm = self._call(self._lib.bn_gradient_set_clip, max_norm)
+        torch.autograd.graph.increment_version(self._written)  # autograd does not see what a kernel writes
+        return norm

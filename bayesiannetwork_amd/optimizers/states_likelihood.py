@@ -91,12 +91,14 @@ def states_log_likelihood_and_gradient(logits: torch.Tensor, states: torch.Tenso
     once where a row fits a block's registers.  Nothing is recorded for autograd.
 
     ``weights``: ``[rows]`` of ll's type.  ``out``: where the gradient goes, of the logits' shape
-    and type; it may be ``logits`` itself, whose values the gradient then replaces.
+    and type; it may be ``logits`` itself, whose values the gradient then replaces.  As after any
+    operation in place, a backward pass that needs what ``out`` held before raises.
     """
     states, counts = _check(logits, states, num_states)
     if weights is not None:
         _rows.check_per_row(weights, logits, (_ll_dtype(logits),), "weights")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
     else:
         _rows.check_logits(out, "out")
@@ -106,4 +108,6 @@ def states_log_likelihood_and_gradient(logits: torch.Tensor, states: torch.Tenso
             raise ValueError("out must not require a gradient (pass its .detach())")
     ll = torch.empty((logits.shape[0],), device=logits.device, dtype=_ll_dtype(logits))
     _gradient(logits, states, counts, None, weights, ll, out)
+    if given:
+        torch.autograd.graph.increment_version(out)  # autograd does not see what a kernel writes
     return ll, out

@@ -194,3 +194,28 @@ def test_learning_a_conditional_model():
     upto = torch.cumsum(torch.softmax(rows.cpu(), dim=1), dim=1)
     plain = draw_states(rows, u.cuda())
     assert torch.equal(plain.cpu().long(), (upto <= u[:, None] * upto[:, -1:]).sum(dim=1))
+
+
+def test_a_backward_pass_that_needs_unclipped_gradients_raises():
+    from bayesiannetwork_amd.optimizers import HipGradientClipper
+
+    x = torch.randn((50,), generator=torch.Generator().manual_seed(1)).cuda()
+    for make in (lambda: x.clone(), lambda: x.clone()[3:40], lambda: torch.split(x.clone(), [20, 30])[1]):
+        g = make()
+        factor = torch.ones_like(g, requires_grad=True)
+        product = factor * g  # keeps g
+        clipper = HipGradientClipper([g])
+        clipper.norm()
+        product.sum().backward(retain_graph=True)
+        assert torch.equal(factor.grad, g)
+        clipper.clip(1e9)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.sum().backward()
+    # clipped copies elsewhere: the gradients stay as they are, the copies' buffer is the one that changes
+    grads = [x.clone(), x.clone()]
+    flat = torch.empty((100,), device="cuda")
+    versions = [g._version for g in grads] + [flat._version]
+    HipGradientClipper(grads, out=list(torch.split(flat, [50, 50]))).clip(1.0)
+    assert [g._version for g in grads] == versions[:2] and flat._version > versions[2]
+    with torch.inference_mode():
+        HipGradientClipper([x.clone()]).clip(1.0)

@@ -294,3 +294,34 @@ def test_captured_and_on_another_stream(n):
         torch.cuda.synchronize()
         want_ll, want = states_log_likelihood_and_gradient(x, states)
         assert torch.equal(ll, want_ll) and torch.equal(gradient, want)
+
+
+@pytest.mark.parametrize("n", [6, 300, 5000])
+def test_a_backward_pass_that_needs_overwritten_logits_raises(n):
+    """The gradient written over logits that an earlier result, or the operation that made them, has kept."""
+    from bayesiannetwork_amd.optimizers import states_log_likelihood, states_log_likelihood_and_gradient
+
+    gen = torch.Generator().manual_seed(n)
+    x, states = torch.randn((4, n), generator=gen).cuda(), torch.randint(0, n, (4,), generator=gen).cuda()
+    leaf = x.clone().requires_grad_(True)
+    ll = states_log_likelihood(leaf, states)
+    states_log_likelihood_and_gradient(leaf.detach(), states, out=leaf.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        ll.sum().backward()
+    leaf = x.clone().requires_grad_(True)
+    y = torch.tanh(leaf)  # keeps its result
+    _, gradient = states_log_likelihood_and_gradient(y.detach(), states, out=y.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(gradient)
+    # a gradient of its own memory disturbs nothing
+    leaf = x.clone().requires_grad_(True)
+    ll = states_log_likelihood(leaf, states)
+    version = leaf._version
+    out = torch.empty_like(x)
+    states_log_likelihood_and_gradient(leaf.detach(), states)
+    states_log_likelihood_and_gradient(leaf.detach(), states, out=out)
+    ll.sum().backward()
+    assert leaf._version == version
+    _check(ll, leaf.grad, x.cpu(), states.cpu(), torch.ones((4,)), torch.full((4,), n))
+    with torch.inference_mode():
+        states_log_likelihood_and_gradient(x.clone(), states, out=torch.empty_like(x))

@@ -12,6 +12,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import rows as _rows
 from ..inference_machines.hip_spa import _native
@@ -75,8 +76,12 @@ def states_log_likelihood(logits: torch.Tensor, states: torch.Tensor, *,
     large) means the row was not observed: log-likelihood 0, gradient 0.  ``num_states`` (int32 /
     int64 ``[rows]``): how many states each row has, the rest being padding that is not read and gets
     gradient 0.  Logits of ``-inf`` are impossible states; a row with NaN or ``+inf`` gives NaN.
+    Derivatives are of first order and reverse mode: logits with a tangent (``forward_ad``) are refused.
     """
     states, counts = _check(logits, states, num_states)
+    # (a dual tensor requires no gradient, and its address is that of its values alone)
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(logits).tangent is not None:
+        raise NotImplementedError("states_log_likelihood has no forward-mode derivative: the logits carry a tangent")
     if torch.is_grad_enabled() and logits.requires_grad:
         return _StatesLogLikelihood.apply(logits, states, counts)
     return _forward(logits, states, counts, False)[0]

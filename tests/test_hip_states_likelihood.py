@@ -325,3 +325,22 @@ def test_a_backward_pass_that_needs_overwritten_logits_raises(n):
     _check(ll, leaf.grad, x.cpu(), states.cpu(), torch.ones((4,)), torch.full((4,), n))
     with torch.inference_mode():
         states_log_likelihood_and_gradient(x.clone(), states, out=torch.empty_like(x))
+
+
+def test_logits_with_a_tangent_are_refused():
+    from torch.autograd import forward_ad
+
+    from bayesiannetwork_amd.optimizers import states_log_likelihood
+
+    x, states = torch.randn((3, 4), generator=torch.Generator().manual_seed(0)).cuda(), torch.tensor([0, 1, 2]).cuda()
+    want = states_log_likelihood(x, states)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: states_log_likelihood(dual, states),
+                     lambda: states_log_likelihood(dual.clone().requires_grad_(True), states)):
+            with pytest.raises(NotImplementedError):
+                call()
+        with torch.no_grad(), pytest.raises(NotImplementedError):
+            states_log_likelihood(dual, states)
+        assert torch.equal(states_log_likelihood(x, states), want)  # no tangent
+        assert torch.equal(states_log_likelihood(forward_ad.unpack_dual(dual).primal, states), want)

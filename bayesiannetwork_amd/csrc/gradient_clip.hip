@@ -15,8 +15,10 @@
 // and through the cache 316; reading and writing 1.6 GB without any reuse would be 300).
 //
 // Squares are summed in double: the square of any float32 is finite there, and the conversions keep
-// up with the loads several times over.  A wave's chunks, a block's waves and the blocks are summed
-// in an order that depends on the set alone - no atomics, the same bits every time.
+// up with the loads several times over.  Those of float64 gradients may leave double's range on either side while
+// the norm does not: such tensors are summed at three scales, and the one that fits is taken.  A wave's chunks, a
+// block's waves and the blocks are summed in an order that depends on the set alone - no atomics, the same bits
+// every time.
 #include "../../include/bn_hip.h"
 
 #include <algorithm>
@@ -48,38 +50,73 @@ constexpr int kMaxBlocks = 1024;  // 4 blocks of 4 waves on each of 256 CUs
 constexpr uintptr_t kLine = 128;  // bytes of a cache line
 constexpr int64_t kCacheBytes = (int64_t)256 << 20;
 
+// Sums of squares: as they are, and of float64 gradients also times 2^-600 and 2^600 each.  Where the first overflows
+// all that counts is in the second; where it is below 2^-800 there is no other type's element but zeros, and
+// none that the third has no room for.
+constexpr double kDown = 0x1p-600, kUp = 0x1p600, kTiny = 0x1p-800;
+struct Squares {
+  double sum = 0.0, large = 0.0, small = 0.0;
+  template <typename T>
+  __device__ __forceinline__ void add(T v) {
+    const double x = (double)Value<T>::widen(v);
+    sum = fma(x, x, sum);
+    if constexpr (sizeof(T) == 8) {
+      large = fma(x * kDown, x * kDown, large);
+      small = fma(x * kUp, x * kUp, small);
+    }
+  }
+};
+
 template <typename T>
-__device__ __forceinline__ double chunk_squares(const Chunk& c, int lane) {
+__device__ __forceinline__ void chunk_squares(const Chunk& c, int lane, Squares& squares) {
   constexpr int V = Value<T>::kVec;
   const T* g = static_cast<const T*>(c.source);
-  double sum = 0.0;
+  Squares own;  // summed by itself: a chunk's order is the same wherever it is taken
   const int packs = c.count / V;
 #pragma unroll 4
   for (int i = lane; i < packs; i += 64) {
     const Pack<T> p = load_pack(g + (size_t)i * V);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const double x = (double)Value<T>::widen(p.v[j]);
-      sum = fma(x, x, sum);
-    }
+    for (int j = 0; j < V; ++j) own.add(p.v[j]);
   }
   const int i = packs * V + lane;
-  if (i < c.count) {
-    const double x = (double)Value<T>::widen(g[i]);
-    sum = fma(x, x, sum);
+  if (i < c.count) own.add(g[i]);
+  squares.sum += own.sum;
+  if constexpr (sizeof(T) == 8) {
+    squares.large += own.large;
+    squares.small += own.small;
   }
-  return sum;
 }
 
+// max_norm / norm, or 1.  Where double has no room for that quotient (the other types' products are 0 then) float64
+// gradients are divided by the norm and multiplied by max_norm, in the order that stays in range: |g| <= norm.
+struct Factor {
+  double factor;
+  double before = 1.0, inverse, after = 1.0;
+  __device__ __forceinline__ Factor(double norm, double max_norm) {
+    // a NaN norm leaves no gradient usable: every element becomes NaN; an infinite one gives factor 0
+    factor = inverse = norm <= max_norm ? 1.0 : max_norm / norm;
+    if (factor < 0x1p-900 && !isinf(norm)) {
+      const double down = norm > 1.0 ? kDown : 1.0;
+      before = down * fmax(max_norm, 1.0);
+      inverse = 1.0 / (norm * down);
+      after = fmin(max_norm, 1.0);
+    }
+  }
+};
+
 template <typename T>
-__device__ __forceinline__ T scaled(T v, double factor) {
+__device__ __forceinline__ T scaled(T v, const Factor& f) {
   // one product in double; the 16-bit types pass through float32 on the way, whose step is 2^-13 (half)
   // and 2^-16 (bfloat16) of theirs
-  return Value<T>::round((typename Value<T>::Wide)((double)Value<T>::widen(v) * factor));
+  if constexpr (sizeof(T) == 8)
+    return v * f.before * f.inverse * f.after;
+  else
+    return Value<T>::round((float)((double)Value<T>::widen(v) * f.factor));
 }
 
 template <typename T, bool STREAM>
-__device__ __forceinline__ void chunk_scale(const Chunk& c, int lane, double factor) {
+__device__ __forceinline__ void chunk_scale(const Chunk& c, int lane, const Factor& factor) {
   constexpr int V = Value<T>::kVec;
   const T* g = static_cast<const T*>(c.source);
   T* out = static_cast<T*>(c.output);
@@ -98,7 +135,7 @@ __device__ __forceinline__ void chunk_scale(const Chunk& c, int lane, double fac
   if (i < c.count) out[i] = scaled<T>(g[i], factor);
 }
 
-// sum over the block, the same in every thread
+// sum over the block, the same in every thread (a barrier between one sum and the next is the caller's)
 __device__ __forceinline__ double block_sum(double v, double* lds) {
   v = lanes_sum<64>(v);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
@@ -109,34 +146,52 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
   return total;
 }
 
+// `partials`: every block's sum; where the set has float64 gradients (`doubles`), then the large and the small ones.
 __global__ void __launch_bounds__(kThreads) gradient_squares(const Chunk* __restrict__ chunks, int64_t n_chunks,
-                                                            double* __restrict__ partials) {
+                                                            int doubles, double* __restrict__ partials) {
   __shared__ double lds[kWaves];
   const int lane = threadIdx.x & 63;
-  double sum = 0.0;
+  Squares squares;
   for (int64_t k = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); k < n_chunks; k += (int64_t)gridDim.x * kWaves) {
     const Chunk c = chunks[k];
     switch (c.dtype) {
-      case BN_F32: sum += chunk_squares<float>(c, lane); break;
-      case BN_F64: sum += chunk_squares<double>(c, lane); break;
-      case BN_F16: sum += chunk_squares<__half>(c, lane); break;
-      default: sum += chunk_squares<__hip_bfloat16>(c, lane); break;
+      case BN_F32: chunk_squares<float>(c, lane, squares); break;
+      case BN_F64: chunk_squares<double>(c, lane, squares); break;
+      case BN_F16: chunk_squares<__half>(c, lane, squares); break;
+      default: chunk_squares<__hip_bfloat16>(c, lane, squares); break;
     }
   }
-  const double total = block_sum(sum, lds);
+  const double total = block_sum(squares.sum, lds);
   if (threadIdx.x == 0) partials[blockIdx.x] = total;
+  if (doubles) {
+    __syncthreads();
+    const double large = block_sum(squares.large, lds);
+    __syncthreads();
+    const double small = block_sum(squares.small, lds);
+    if (threadIdx.x == 0) {
+      partials[gridDim.x + blockIdx.x] = large;
+      partials[2 * gridDim.x + blockIdx.x] = small;
+    }
+  }
 }
 
-__device__ __forceinline__ double norm_of(const double* __restrict__ partials, int n_partials, double* lds) {
-  double sum = 0.0;
-  for (int i = threadIdx.x; i < n_partials; i += kThreads) sum += partials[i];
-  return sqrt(block_sum(sum, lds));
+__device__ __forceinline__ double norm_of(const double* __restrict__ partials, int n_partials, int doubles, double* lds) {
+  const auto total = [&](const double* from) {
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < n_partials; i += kThreads) sum += from[i];
+    return block_sum(sum, lds);
+  };
+  const double sum = total(partials);
+  const bool over = isinf(sum);
+  if (!doubles || !(over || sum < kTiny)) return sqrt(sum);
+  __syncthreads();
+  return sqrt(total(partials + (over ? 1 : 2) * n_partials)) * (over ? kUp : kDown);
 }
 
 __global__ void __launch_bounds__(kThreads) gradient_norm_finish(const double* __restrict__ partials, int n_partials,
-                                                                double* __restrict__ norm_out) {
+                                                                int doubles, double* __restrict__ norm_out) {
   __shared__ double lds[kWaves];
-  const double norm = norm_of(partials, n_partials, lds);
+  const double norm = norm_of(partials, n_partials, doubles, lds);
   if (threadIdx.x == 0) *norm_out = norm;
 }
 
@@ -144,12 +199,11 @@ __global__ void __launch_bounds__(kThreads) gradient_norm_finish(const double* _
 template <bool STREAM>
 __global__ void __launch_bounds__(kThreads) gradient_scale(const Chunk* __restrict__ chunks, int64_t n_chunks,
                                                           const double* __restrict__ partials, int n_partials,
-                                                          double max_norm, double* __restrict__ norm_out) {
+                                                          int doubles, double max_norm, double* __restrict__ norm_out) {
   __shared__ double lds[kWaves];
-  const double norm = norm_of(partials, n_partials, lds);
+  const double norm = norm_of(partials, n_partials, doubles, lds);
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
-  // a NaN norm leaves no gradient usable: every element becomes NaN; an infinite one gives factor 0
-  const double factor = norm <= max_norm ? 1.0 : max_norm / norm;
+  const Factor factor(norm, max_norm);
   const int lane = threadIdx.x & 63;
   for (int64_t k = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); k < n_chunks; k += (int64_t)gridDim.x * kWaves) {
     const Chunk c = chunks[n_chunks - 1 - k];
@@ -174,6 +228,7 @@ struct bn_gradient_set {
   int64_t n_chunks = 0;
   int64_t bytes = 0;  // of all gradients
   int blocks = 1;
+  int doubles = 0;  // whether any gradient is of float64
   Chunk* d_chunks = nullptr;
 };
 
@@ -236,6 +291,7 @@ int build_set(int32_t n, const int32_t* dtypes, const int64_t* sizes, const void
            static_cast<char*>(outputs[last + 1]) == o + count * es)
       count += sizes[++last];
     set->bytes += count * es;
+    if (dtypes[t] == BN_F64 && count > 0) set->doubles = 1;
     int64_t here = (int64_t)((kLine - reinterpret_cast<uintptr_t>(o) % kLine) % kLine) / es;
     if (here == 0) here = kChunkBytes / es;
     for (int64_t done = 0; done < count; done += here, here = kChunkBytes / es) {
@@ -258,7 +314,8 @@ int launch_squares(const bn_gradient_set* set, double* partials, hipStream_t s) 
   int device = -1;
   if (hipGetDevice(&device) != hipSuccess || device != set->device)
     return fail(BN_ERR_STATE, "the gradient set belongs to another HIP device than the current one");
-  hipLaunchKernelGGL(gradient_squares, dim3(set->blocks), dim3(kThreads), 0, s, set->d_chunks, set->n_chunks, partials);
+  hipLaunchKernelGGL(gradient_squares, dim3(set->blocks), dim3(kThreads), 0, s, set->d_chunks, set->n_chunks, set->doubles,
+                     partials);
   BN_HIP_CHECK(hipGetLastError());
   return BN_OK;
 }
@@ -312,7 +369,7 @@ int bn_gradient_set_destroy(bn_gradient_set* set) {
 }
 
 int64_t bn_gradient_set_workspace_bytes(const bn_gradient_set* set) {
-  return set ? (int64_t)set->blocks * (int64_t)sizeof(double) : -1;
+  return set ? (int64_t)set->blocks * (set->doubles ? 3 : 1) * (int64_t)sizeof(double) : -1;
 }
 
 int bn_gradient_set_norm(bn_gradient_set* set, void* workspace_dev, double* norm_out_dev, void* stream) {
@@ -320,7 +377,8 @@ int bn_gradient_set_norm(bn_gradient_set* set, void* workspace_dev, double* norm
   hipStream_t s = static_cast<hipStream_t>(stream);
   double* partials = static_cast<double*>(workspace_dev);
   if (int rc = launch_squares(set, partials, s)) return rc;
-  hipLaunchKernelGGL(gradient_norm_finish, dim3(1), dim3(kThreads), 0, s, partials, set->blocks, norm_out_dev);
+  hipLaunchKernelGGL(gradient_norm_finish, dim3(1), dim3(kThreads), 0, s, partials, set->blocks, set->doubles,
+                     norm_out_dev);
   BN_HIP_CHECK(hipGetLastError());
   return BN_OK;
 }
@@ -334,10 +392,10 @@ int bn_gradient_set_clip(bn_gradient_set* set, double max_norm, void* workspace_
   if (int rc = launch_squares(set, partials, s)) return rc;
   if (2 * set->bytes > kCacheBytes)
     hipLaunchKernelGGL(gradient_scale<true>, dim3(set->blocks), dim3(kThreads), 0, s, set->d_chunks, set->n_chunks,
-                       partials, set->blocks, max_norm, norm_out_dev);
+                       partials, set->blocks, set->doubles, max_norm, norm_out_dev);
   else
     hipLaunchKernelGGL(gradient_scale<false>, dim3(set->blocks), dim3(kThreads), 0, s, set->d_chunks, set->n_chunks,
-                       partials, set->blocks, max_norm, norm_out_dev);
+                       partials, set->blocks, set->doubles, max_norm, norm_out_dev);
   BN_HIP_CHECK(hipGetLastError());
   return BN_OK;
 }

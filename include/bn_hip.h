@@ -579,8 +579,10 @@ int bn_states_log_likelihood_gradient(int dtype, const void* logits_dev, int64_t
  * A set names its tensors once (addresses, sizes and types, which may differ from tensor to tensor);
  * every call is then two launches, however many tensors there are (the reference's models have
  * one CPT per node, 785 in dev_experiments/mnist/mnist.py, and no gradient).  Squares are summed in
- * double, in an order that depends on the set alone.  A NaN norm makes every output NaN; an infinite
- * one gives factor 0 (so infinite gradients become NaN, the others 0): callers look at the norm.
+ * double, in an order that depends on the set alone, and at scales of their own where those of float64
+ * gradients leave its range: the norm is infinite only if it is beyond 1.8e308 itself.  A NaN norm makes every
+ * output NaN; an infinite one gives factor 0 (so infinite gradients become NaN, the others 0): callers look at
+ * the norm.
  *   sizes        elements of each tensor (contiguous; 0 is skipped)
  *   outputs_dev  where each tensor's clipped copy goes: its own address (in place) or memory that no
  *                tensor of the set overlaps; anything else is refused

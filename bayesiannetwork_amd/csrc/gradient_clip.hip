@@ -359,11 +359,15 @@ int bn_gradient_set_create(int32_t num_tensors, const int32_t* dtypes, const int
 
 int bn_gradient_set_destroy(bn_gradient_set* set) {
   if (!set) return BN_OK;
+  // the last reference to a set may go while some stream is being captured, which hipFree would end otherwise
+  hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+  (void)hipThreadExchangeStreamCaptureMode(&mode);
   int prev = 0;
   (void)hipGetDevice(&prev);
   (void)hipSetDevice(set->device);
   if (set->d_chunks) (void)hipFree(set->d_chunks);
   (void)hipSetDevice(prev);
+  (void)hipThreadExchangeStreamCaptureMode(&mode);
   delete set;
   return BN_OK;
 }

@@ -37,7 +37,8 @@ class HipGradientClipper:
     are read where they lie at every call: keep them (fill them in place rather than
     replacing them).  ``out``: tensors of the same shapes and types for the clipped copies; without it the
     gradients themselves are scaled.  Listing one tensor twice in place, or an output over
-    another tensor, is an error.  Build a clipper outside of graph capture; its calls may be captured.
+    another tensor, is an error.  Build a clipper outside of graph capture; its calls may be captured, and
+    the clipper is kept as long as their graph is replayed.
 
     The norm is summed in float64, in an order that depends on the list alone.  With a NaN among the
     gradients the norm and everything scaled by it is NaN; with an infinite norm the factor is 0.

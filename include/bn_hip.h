@@ -586,9 +586,10 @@ int bn_states_log_likelihood_gradient(int dtype, const void* logits_dev, int64_t
  *   sizes        elements of each tensor (contiguous; 0 is skipped)
  *   outputs_dev  where each tensor's clipped copy goes: its own address (in place) or memory that no
  *                tensor of the set overlaps; anything else is refused
- * Creation allocates and copies a table (not under graph capture).  A set is bound to the device it was created on, and the tensors must stay where they
- * are while it is used.  The other calls allocate nothing, may be captured, and need a
- * workspace each when they may overlap.  0 < max_norm < inf.
+ * Creation allocates and copies a table (not under graph capture).  A set is bound to the device it was created
+ * on, and the tensors must stay where they are while it is used.  The other calls allocate nothing, may be
+ * captured, and need a workspace each when they may overlap; a captured call reads the set's table, so the set is
+ * destroyed after the last replay.  Destruction may fall into a capture.  0 < max_norm < inf.
  */
 typedef struct bn_gradient_set bn_gradient_set;
 int bn_gradient_set_create(int32_t num_tensors, const int32_t* dtypes, const int64_t* sizes,

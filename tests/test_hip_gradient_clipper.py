@@ -250,3 +250,28 @@ def test_float64_gradients_whose_squares_leave_the_range(size, others, max_norm)
     for v, o in zip(big.tolist(), out[0].cpu().tolist()):
         want = Fraction(v) * factor
         assert abs(Fraction(o) - want) <= want * (Fraction(2.0**-47) + Fraction(2.0**-51)) + unit
+
+
+def test_a_clipper_that_goes_while_a_graph_is_captured():
+    from bayesiannetwork_amd.optimizers import HipGradientClipper
+
+    gen = torch.Generator().manual_seed(4)
+    grads = [torch.randn((n,), generator=gen).cuda() for n in (7, 30000)]
+    out = [torch.empty_like(g) for g in grads]
+    clipper, other = HipGradientClipper(grads, out=out), HipGradientClipper([g.clone() for g in grads])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        clipper.clip(2.0)
+        other.clip(2.0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        del other
+        norm = clipper.clip(2.0)
+    for _ in range(3):
+        for g in grads:
+            g.copy_(torch.randn(g.shape, generator=gen))
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(norm, out, grads, 2.0)

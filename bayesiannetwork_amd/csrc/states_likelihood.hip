@@ -654,7 +654,8 @@ int check_rows(int dtype, const Rows& a) {
   return BN_OK;
 }
 
-// The gradient may replace the logits, row for row; any other overlap would change a row that is still read.
+// The gradient may replace the logits, row for row, or have columns of its own between them (the same stride); any
+// other overlap would change a row that is still read.
 int check_gradient(int dtype, const Rows& a) {
   if (a.rows == 0) return BN_OK;
   if (!a.gradient) return fail(BN_ERR_INVALID, "null argument");
@@ -665,7 +666,13 @@ int check_gradient(int dtype, const Rows& a) {
   const uintptr_t x_end = x + ((uintptr_t)(a.rows - 1) * a.stride + a.width) * es;
   const uintptr_t g_end = g + ((uintptr_t)(a.rows - 1) * a.gradient_stride + a.width) * es;
   const bool same = x == g && (a.rows == 1 || a.stride == a.gradient_stride);
-  if (!same && x < g_end && g < x_end)
+  const uintptr_t row = (uintptr_t)a.width * es, pitch = (uintptr_t)a.stride * es;
+  bool between = false;
+  if (a.stride == a.gradient_stride && a.stride >= 2 * a.width) {
+    const uintptr_t behind = g >= x ? (g - x) % pitch : pitch - (x - g) % pitch;  // of a row's start, within the pitch
+    between = behind >= row && behind <= pitch - row;
+  }
+  if (!same && !between && x < g_end && g < x_end)
     return fail(BN_ERR_INVALID, "the gradient lies over the logits without being the same rows");
   return BN_OK;
 }

@@ -563,8 +563,8 @@ int bn_states_log_likelihood(int dtype, const void* logits_dev, int64_t rows, in
  *   totals_dev given   the backward pass of an earlier bn_states_log_likelihood: reads the logits
  *                      once; ll_out_dev must be NULL
  *   totals_dev NULL    log-likelihood (to ll_out_dev, may be NULL) and gradient in one call
- * The gradient may replace the logits (same address and stride); any other overlap with them is
- * refused.  Neither call allocates; both may be captured into a graph.
+ * The gradient may replace the logits (same address and stride) or have columns of its own in the same
+ * buffer (same stride); any other overlap of the two address ranges is refused.  Neither call allocates; both may be captured into a graph.
  */
 int bn_states_log_likelihood_gradient(int dtype, const void* logits_dev, int64_t rows, int64_t num_states,
                                       int64_t row_stride, const int64_t* row_states_dev, const void* states_dev,

@@ -344,3 +344,28 @@ def test_logits_with_a_tangent_are_refused():
             states_log_likelihood(dual, states)
         assert torch.equal(states_log_likelihood(x, states), want)  # no tangent
         assert torch.equal(states_log_likelihood(forward_ad.unpack_dual(dual).primal, states), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("n", [1, 13, 900, 5000])
+def test_gradients_in_columns_between_the_logits(n, dtype):
+    from bayesiannetwork_amd.optimizers import states_log_likelihood_and_gradient
+
+    gen = torch.Generator().manual_seed(n)
+    x = torch.randn((9, n), generator=gen).to(dtype)
+    states = torch.randint(0, n, (9,), generator=gen).cuda()
+    ll, gradient = states_log_likelihood_and_gradient(x.cuda(), states)
+    for first, second in ((0, n), (n, 0), (1, n + 3), (n + 2, 2)):
+        buffer = torch.full((9, 2 * n + 5), 42.0, dtype=dtype, device="cuda")
+        logits, out = buffer[:, first : first + n], buffer[:, second : second + n]
+        logits.copy_(x)
+        got, _ = states_log_likelihood_and_gradient(logits, states, out=out)
+        assert torch.equal(got, ll) and torch.equal(out, gradient) and torch.equal(logits.cpu(), x)
+        out.fill_(0.0)
+        logits.fill_(0.0)
+        assert float((buffer == 42.0).sum()) == 9 * 5
+    if n > 1:
+        buffer = torch.zeros((9, 2 * n + 5), dtype=dtype, device="cuda")
+        for first, second in ((0, n - 1), (n, 1), (n + 4, 5)):
+            with pytest.raises(RuntimeError, match="lies over"):
+                states_log_likelihood_and_gradient(buffer[:, first : first + n], states, out=buffer[:, second : second + n])

@@ -155,3 +155,14 @@ def test_loads_stay_inside_their_rows(tmp_path):
     program = str(tmp_path / "row_loads_check")
     subprocess.run(["g++", "-std=c++17", "-O1", "-o", program, source], check=True)
     subprocess.run([program], check=True)
+
+
+@pytest.mark.parametrize("change", [
+    dict(stride=9, g_stride=9, gradient=A + 3 * 4), dict(stride=9, g_stride=9, gradient=A + 6 * 4),
+    dict(stride=9, g_stride=9, gradient=A + (9 + 8) * 4), dict(stride=9, g_stride=9, logits=A + 6 * 4, gradient=A),
+    dict(stride=9, g_stride=10, gradient=A + 4 * 4), dict(stride=7, g_stride=7, gradient=A + 4 * 4),
+    dict(stride=9, g_stride=9, logits=A + 3 * 4, gradient=A),
+])
+def test_gradient_columns_that_meet_the_logits(change):
+    assert _gradient(**change) == -1
+    assert "lies over" in _native.load().bn_last_error().decode()

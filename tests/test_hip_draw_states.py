@@ -559,3 +559,52 @@ def test_a_last_row_that_ends_its_buffer(states, dtype):
             _native.launch(flat.device, lib.bn_draw_states, _native.DTYPE_CODES[dtype], flat.data_ptr(), rows, states, states,
                            dc.data_ptr(), 1, du.data_ptr(), ctypes.byref(filters), workspace.data_ptr(), out.data_ptr())
             _check(out, [x[r, : int(counts[r])].double().numpy() for r in range(rows)], u.numpy(), settings)
+
+
+def _oracle_on_gpu(x, u, counts, temperature, top_k, top_p, min_p):
+    """_oracle for many rows at once, in float64 on the GPU; settings are numbers."""
+    rows, n = x.shape
+    place = torch.arange(n, device="cuda")[None, :]
+    x = torch.where(place < counts[:, None], x.double(), -float("inf"))
+    w = torch.exp((x - x.max(1, keepdim=True).values) / temperature)
+    by_key, order = torch.sort(x, dim=1, descending=True, stable=True)
+    sorted_w = torch.gather(w, 1, order)
+    top = torch.where(place < (top_k or n), sorted_w, 0.0)
+    upto = top.cumsum(1)
+    total = upto[:, -1:]
+    kept = (place < (top_k or n)) & (upto - top < top_p * total) if top_p < 1 else place < torch.full_like(counts, top_k or n)[:, None]
+    margin = torch.ones((rows,), device="cuda", dtype=torch.float64)
+    if top_p < 1:
+        margin = torch.minimum(margin, (upto / total - top_p).abs().min(1).values)
+    if min_p > 0:
+        margin = torch.minimum(margin, (sorted_w - min_p).abs().min(1).values)
+    kept &= sorted_w >= min_p
+    w = torch.where(torch.zeros_like(kept).scatter_(1, order, kept), w, 0.0)
+    upto = w.cumsum(1)
+    target = u.double()[:, None] * upto[:, -1:]
+    margin = torch.minimum(margin, ((upto - target).abs() / upto[:, -1:]).min(1).values)
+    state = (upto <= target).sum(1)
+    return torch.where(counts > 0, state, -1), margin
+
+
+# 16 states per lane, in groups of 1 to 64 lanes: from these numbers of rows on
+@pytest.mark.parametrize("ragged", [False, True], ids=["full", "ragged"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("rows,states", [(262147, 5), (262145, 16), (131075, 17), (131073, 32), (65537, 50), (65539, 64),
+                                         (32769, 100), (32771, 128), (16387, 130), (16385, 256), (5003, 300), (3001, 1024)])
+def test_many_rows(rows, states, dtype, ragged):
+    from bayesiannetwork_amd.samplers import draw_states
+
+    gen = torch.Generator(device="cuda").manual_seed(rows + states)
+    x = (2.0 * torch.randn((rows, states), generator=gen, device="cuda")).to(dtype)
+    u = torch.rand((rows,), generator=gen, device="cuda", dtype=torch.float64) * 0.999
+    counts = torch.randint(0, states + 1, (rows,), generator=gen, device="cuda") if ragged else torch.full((rows,), states, device="cuda")
+    padded = x.masked_fill(torch.arange(states, device="cuda")[None, :] >= counts[:, None], float("nan"))
+    for settings in (dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0), dict(temperature=0.8, top_k=4, top_p=1.0, min_p=0.0),
+                     dict(temperature=1.3, top_k=0, top_p=0.9, min_p=0.0), dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.05),
+                     dict(temperature=1.1, top_k=9, top_p=0.85, min_p=0.03)):
+        want, margin = _oracle_on_gpu(x, u, counts, **settings)
+        got = draw_states(padded, u, **({**settings, "num_states": counts} if ragged else settings))
+        decided = (margin > 1e-10) | (counts == 0)
+        assert decided.double().mean() > 0.99
+        assert torch.equal(got[decided].long(), want[decided])

@@ -369,3 +369,79 @@ def test_gradients_in_columns_between_the_logits(n, dtype):
         for first, second in ((0, n - 1), (n, 1), (n + 4, 5)):
             with pytest.raises(RuntimeError, match="lies over"):
                 states_log_likelihood_and_gradient(buffer[:, first : first + n], states, out=buffer[:, second : second + n])
+
+
+def _check_on_gpu(ll, gradient, x, states, weights, counts):
+    """The definition over many rows at once, in float64 on the GPU, with the tolerances above."""
+    dtype, (rows, n) = x.dtype, x.shape
+    eps = 2.0**-53 if dtype == torch.float64 else 2.0**-24
+    inside = torch.arange(n, device="cuda")[None, :] < counts[:, None]
+    wide = torch.where(inside, x.double(), -float("inf"))
+    seen = (states >= 0) & (states < counts)
+    row, target = torch.arange(rows, device="cuda"), torch.where(seen, states, 0)
+    best = wide.max(dim=1, keepdim=True).values
+    wide = torch.where(seen[:, None], wide - best, 0.0)
+    total = torch.logsumexp(wide, dim=1)
+    want_ll = torch.where(seen, wide[row, target] - total, 0.0)
+    depth = n / 64 + 16
+    assert torch.all((ll.detach().double() - want_ll).abs() <= depth * eps + eps * want_ll.abs())
+    p = torch.where(seen[:, None], torch.exp(wide - total[:, None]), 0.0)
+    want = -p
+    want[row, target] += seen.double()
+    want *= weights.double()[:, None]
+    slack = weights.double().abs()[:, None] * (depth + 64) * eps * p + (torch.finfo(dtype).eps / 2 + 2 * eps) * want.abs()
+    assert torch.all((gradient.double() - want).abs() <= slack + SMALLEST[dtype])
+
+
+# Rows beyond which a group of lanes takes several of them (by the bytes of a row), and the rows a block takes one after
+# the other; the last groups and turns are not full.
+@pytest.mark.parametrize("ragged", [False, True], ids=["full", "ragged"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("rows,bytes_of_a_row", [
+    (262147, 30), (262149, 60), (131079, 125), (65541, 256), (32771, 500), (16389, 1000), (16389, 2000), (8201, 4000),
+    (2307, 10000), (1801, 30000), (601, 50000), (601, 130000), (601, 200000)])
+def test_many_rows(rows, bytes_of_a_row, dtype, ragged):
+    from bayesiannetwork_amd.optimizers import states_log_likelihood, states_log_likelihood_and_gradient
+
+    n = bytes_of_a_row * 8 // torch.finfo(dtype).bits
+    gen = torch.Generator(device="cuda").manual_seed(rows + n)
+    x = (3.0 * torch.randn((rows, n), generator=gen, device="cuda")).to(dtype)
+    states = torch.randint(-1, n, (rows,), generator=gen, device="cuda")
+    weights = torch.rand((rows,), generator=gen, device="cuda", dtype=torch.float64) - 0.3
+    weights = weights if dtype == torch.float64 else weights.float()
+    counts = torch.randint(0, n + 1, (rows,), generator=gen, device="cuda") if ragged else torch.full((rows,), n, device="cuda")
+    if ragged:
+        x.masked_fill_(torch.arange(n, device="cuda")[None, :] >= counts[:, None], float("nan"))
+    given = dict(num_states=counts) if ragged else {}
+    ll, gradient = states_log_likelihood_and_gradient(x, states, weights, **given)
+    _check_on_gpu(ll, gradient, x, states, weights, counts)
+    leaf = x.clone().requires_grad_(True)
+    again = states_log_likelihood(leaf, states, **given)
+    (backward,) = torch.autograd.grad(again, leaf, grad_outputs=weights)
+    _check_on_gpu(again, backward, x, states, weights, counts)
+    states_log_likelihood_and_gradient(x, states, weights, out=x, **given)
+    assert torch.equal(x, gradient)
+
+
+def test_backward_of_more_packs_than_32_bits_count():
+    """8200 rows of 2^22 states, all the same logits: 4.3e9 packs of 16 bytes.  The pass is elementwise, so each row is,
+    bit for bit, what a call for that row alone gives."""
+    from bayesiannetwork_amd.optimizers import states_log_likelihood
+
+    rows, n = 8200, 1 << 22
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("needs 69 GB for the gradient")
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn((1, n), generator=gen, device="cuda").half()
+    states = torch.randint(0, n, (rows,), generator=gen, device="cuda")
+    weights = torch.rand((rows,), generator=gen, device="cuda") + 0.5
+    leaf = x.expand(rows, n).requires_grad_(True)
+    (gradient,) = torch.autograd.grad(states_log_likelihood(leaf, states), leaf, grad_outputs=weights)
+    assert gradient.shape == (rows, n)
+    for r in (0, 1, 4095, 4096, 8190, 8191, 8192, 8199):
+        one = x.clone().requires_grad_(True)
+        (want,) = torch.autograd.grad(states_log_likelihood(one, states[r : r + 1]), one, grad_outputs=weights[r : r + 1])
+        assert torch.equal(gradient[r], want[0]), r
+    del gradient
+    torch.cuda.empty_cache()

@@ -137,7 +137,7 @@ __device__ __forceinline__ Setting row_setting(const Draws& a, int64_t r) {
 // a polynomial of degree 9 in f (interpolating (2^f - 1) / f at the Chebyshev nodes of [-1/2, 1/2]: 4e-14
 // relative, exactly 1 at f = 0).  k comes from adding 1.5 * 2^52, whose sum carries it in its low bits, and goes
 // into an exponent by shifting: 17 of the 30 instructions that block_summaries spends on a state, and it is bound by
-// their issue, 4.6 cycles each (256 x 131072 bfloat16, every row weighed: 35 us).
+// their issue, 5.3 cycles each (256 x 131072 bfloat16, every row weighed: 33 us; profiles/row_operators_counters.txt).
 struct Weight {
   double best;
   double rate;    // log2(e) / T; T is taken within 1e-290 .. 1e290
@@ -1656,7 +1656,7 @@ __global__ void __launch_bounds__(kShareThreads) draw_wide_sums(const Draws a) {
   const Prefix<Key> in{row.floor, row.n};
   if (threadIdx.x == 0) list.count = 0;
   __syncthreads();
-  const double certain = add_up<T, kShareThreads>(row, Prefix<Key>{row.floor, row.n}, around.x, around.y, begin, end, words,
+  const double certain = add_up<T, kShareThreads>(row, in, around.x, around.y, begin, end, words,
                                                   [&](int i, Key k) { list.add(i, k); });
   // the share's states around the threshold go behind those of the shares before
   if (threadIdx.x == 0) {

@@ -91,8 +91,8 @@ struct Total {
 };
 
 // ll of a row, in double: the difference to the largest logit is not rounded together with the
-// logarithm, so a row whose state is nearly certain keeps its small value's digits.  `target` is the
-// state's logit.
+// logarithm, so a row whose state is nearly certain keeps its small value down to the last bit of the sum (6e-8 for
+// all types but float64).  `target` is the state's logit.
 template <typename T, typename W>
 __device__ __forceinline__ void finish_row(const Rows& a, int64_t r, bool observed, W target, const Total<W>& total) {
   double ll = 0.0;
@@ -295,11 +295,12 @@ __device__ __forceinline__ W block_sum(W v, W* lds) {
 // relative to its own largest one and keeps them; once the block has agreed on the row's maximum and sum, one
 // factor per thread turns them into the gradient.  So every logit costs one exponential, and its register is
 // free again before the block has met: the next row's logits are requested then and arrive while this row is
-// reduced and written.  4096 rows of 64000 bfloat16 states, 1.05 GB, take 190 us, 5.5 TB/s; loading, reducing
+// reduced and written.  4096 rows of 64000 bfloat16 states, 1.05 GB, take 191 us, 5.5 TB/s, in a long run of calls
+// (a copy of the same tensors 196; the first 50 calls, as in profiles/row_operators_kernels.txt, 203); loading, reducing
 // and storing one after the other took 353 us (a CU holds one such row, and its memory pipe idled in
 // between), reading the row twice instead 318 us.
-// The gradient is stored past the caches' order: 190 us against 203 there, 8.7 against 10.3 at 1000 rows of
-// 5003 float32, where what reads it next is no slower for it (18.7 against 20.7 us together); between about
+// The gradient is stored past the caches' order, which takes 13 us from that and 1.6 from 1000 rows of
+// 5003 float32 (9.7 us now), where what reads it next is no slower for it (18.7 against 20.7 us together); between about
 // 100 and 256 MB the next reader loses more than is won here (4096 x 16000: 44 against 46 us alone, 99
 // against 92 together).
 // HOLD: false where the exponentials do not fit the registers beside the logits.  They are taken twice then, and

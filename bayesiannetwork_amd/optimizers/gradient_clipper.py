@@ -35,7 +35,8 @@ class HipGradientClipper:
 
     ``gradients``: tensors on one GPU, each float32, float64, float16 or bfloat16 and contiguous, any sizes.  They
     are read where they lie at every call: keep them (fill them in place rather than
-    replacing them).  ``out``: tensors of the same shapes and types for the clipped copies; without it the
+    replacing them: ``zero_grad(set_to_none=False)``; after its default, which drops ``.grad``, the clipper would
+    scale the dropped tensors).  ``out``: tensors of the same shapes and types for the clipped copies; without it the
     gradients themselves are scaled.  Listing one tensor twice in place, or an output over
     another tensor, is an error.  Build a clipper outside of graph capture; its calls may be captured, and
     the clipper is kept as long as their graph is replayed.

@@ -36,7 +36,8 @@ def draw_states(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: Se
     ``top_k`` and ``min_p`` off and 1 switches ``top_p`` off.
 
     ``num_states`` (int32 / int64 ``[rows]``): how many states each row has; the rest is padding
-    and not read.  A row without anything to draw from gives -1: no states, all ``-inf``, a NaN or
+    and not read.  Sums are taken in double: a border within 1e-11 of a row's weight may be decided either way.
+    A row without anything to draw from gives -1: no states, all ``-inf``, a NaN or
     ``+inf`` among its states, a uniform number outside [0, 1], a bad temperature of its own.
     """
     _rows.check_logits(logits)

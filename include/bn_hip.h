@@ -534,7 +534,8 @@ int64_t bn_draw_states_workspace_bytes(int dtype, int64_t rows, int64_t num_stat
  *   out_dev          int32 [rows]
  * Rows need no alignment beyond their type's.  The call allocates nothing and may be captured into a
  * graph; calls that may overlap need a workspace each.  Sums are taken in one fixed order: the same
- * inputs give the same states.
+ * inputs give the same states.  Weights are doubles to 4e-14 of themselves; a border (of top_p, min_p or u) that lies
+ * within 1e-11 of the row's weight may be decided either way.
  */
 int bn_draw_states(int dtype, const void* logits_dev, int64_t rows, int64_t num_states, int64_t row_stride,
                    const int64_t* row_states_dev, int uniform_dtype, const void* uniforms_dev,
@@ -544,8 +545,8 @@ int bn_draw_states(int dtype, const void* logits_dev, int64_t rows, int64_t num_
  * Log-likelihood of one observed state per row of logits:
  *   ll_out_dev[r] = x[r][s_r] - log sum_i exp(x[r][i])
  * and the sums themselves, for the gradient below, to totals_out_dev[rows][2]: the row's largest logit and
- * sum_i exp(x[r][i] - largest), as doubles (may be NULL).  Rows, row_stride and row_states_dev as in bn_draw_states; states_dev[rows] are unsigned bytes
- * (state_bytes 1), int32 (4) or int64 (8).  ll_out_dev is float for BN_F32, BN_F16 and BN_BF16,
+ * sum_i exp(x[r][i] - largest), as doubles (may be NULL).  Rows, row_stride and row_states_dev as in
+ * bn_draw_states; states_dev[rows] are unsigned bytes (state_bytes 1), int32 (4) or int64 (8).  ll_out_dev is float for BN_F32, BN_F16 and BN_BF16,
  * double for BN_F64.  A state that is none of its row's states means "not observed", as in
  * bn_enter_evidence_states: log-likelihood 0, gradient 0.  A row of -inf only has -inf (and gradient
  * 0), a row with a NaN or +inf among its states NaN.  With the rows' softmax as CPT rows, this
